@@ -860,7 +860,7 @@ def main():
         hdt = time.perf_counter() - h0
         if world > 1:
             t = torch.tensor([hdt], dtype=torch.float64, device=dev)
-            torch.distributed.all_reduce(t, op=torch.distributed.ReduceOp.MAX)
+            D.all_reduce(t, op=torch.distributed.ReduceOp.MAX)
             hdt = float(t.item())
         host_read = dict(steps=n_hr, ms_per_step=round(hdt / n_hr * 1e3, 3), mean_loss=round(acc / n_hr, 6),
                          note="the same replayed step followed by float(loss) on the host, as the reference's loop does "
@@ -880,7 +880,7 @@ def main():
             print(f"[stamps] {t_us:9.1f} us  {name}", file=sys.stderr)
     if world > 1:
         t = torch.tensor([dt], dtype=torch.float64, device=dev)
-        torch.distributed.all_reduce(t, op=torch.distributed.ReduceOp.MAX)
+        D.all_reduce(t, op=torch.distributed.ReduceOp.MAX)
         dt = float(t.item())
     final_loss = float(last.detach()) if last is not None else None
     insitu = None

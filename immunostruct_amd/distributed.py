@@ -48,6 +48,32 @@ def init_from_env(backend=None):
     return rank, local_rank, world
 
 
+def _through_host(t):
+    """gloo moves bytes with host threads: its collectives on device tensors have hung where several ranks share one GPU (each rank's
+    copies wait on a device the others keep busy).  Such a tensor goes through a host copy that is complete before the call."""
+    return t.is_cuda and dist.get_backend() == "gloo"
+
+
+def all_reduce(t, op=dist.ReduceOp.SUM, async_op=False):
+    """``dist.all_reduce`` in place; under gloo a device tensor is reduced through host memory and the call is synchronous (no handle)"""
+    if not _through_host(t):
+        return dist.all_reduce(t, op=op, async_op=async_op)
+    host = t.detach().cpu()
+    dist.all_reduce(host, op=op)
+    t.detach().copy_(host)
+    return None
+
+
+def broadcast(t, src=0):
+    """``dist.broadcast`` in place; under gloo a device tensor goes through host memory"""
+    if not _through_host(t):
+        dist.broadcast(t, src=src)
+        return
+    host = t.detach().cpu()
+    dist.broadcast(host, src=src)
+    t.detach().copy_(host)
+
+
 def collectives_forced():
     """one rank, but the collectives are issued all the same (IMMUNOSTRUCT_FORCE_COLLECTIVE=1 under an initialised group)"""
     return os.environ.get("IMMUNOSTRUCT_FORCE_COLLECTIVE") == "1" and dist.is_initialized()
@@ -175,7 +201,7 @@ class FlatGradReducer:
         if self._collective:
             if self.divide:
                 b["flat"].div_(self.world)
-            work = dist.all_reduce(b["flat"], op=dist.ReduceOp.SUM, async_op=async_op)
+            work = all_reduce(b["flat"], async_op=async_op)
         for p, v in zip(b["params"], b["views"]):
             p.grad = v
         return work
@@ -202,10 +228,10 @@ def time_all_reduce(reducer, repeats=10):
                 dist.barrier()
                 torch.cuda.synchronize() if scratch.is_cuda else None
                 t0 = time.perf_counter()
-            dist.all_reduce(scratch, op=dist.ReduceOp.SUM)
+            all_reduce(scratch)
         torch.cuda.synchronize() if scratch.is_cuda else None
         t = torch.tensor([(time.perf_counter() - t0) / repeats * 1e3], dtype=torch.float64, device=scratch.device)
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        all_reduce(t, op=dist.ReduceOp.MAX)
         out.append(dict(floats=int(scratch.numel()), ms=round(float(t.item()), 4)))
     return out
 
@@ -216,7 +242,7 @@ def broadcast_parameters(module, src=0):
         return
     with torch.no_grad():
         for t in list(module.parameters()) + list(module.buffers()):
-            dist.broadcast(t, src=src)
+            broadcast(t, src=src)
 
 
 def shard_indices(num_items, epoch, seed, rank, world, drop_last=True):

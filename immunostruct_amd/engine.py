@@ -314,8 +314,9 @@ class CapturedTrainStep:
             # every rank replays the same form or the collectives stop matching: a form is a candidate only where EVERY rank
             # captured it (an eager MIN all-reduce of the two success flags; one rank's failure withdraws the form everywhere)
             import torch.distributed as dist
+            from .distributed import all_reduce
             have = torch.tensor([1.0 if k in self.graph_c else 0.0 for k in ("graph", "graph2")], device=self.y.device)
-            dist.all_reduce(have, op=dist.ReduceOp.MIN)
+            all_reduce(have, op=dist.ReduceOp.MIN)
             for k, ok in zip(("graph", "graph2"), have.tolist()):
                 if ok < 0.5 and k in self.graph_c:
                     del self.graph_c[k]
@@ -420,6 +421,7 @@ class CapturedTrainStep:
         steps taken for this leave no trace in the model or the optimizer"""
         import time
         import torch.distributed as dist
+        from .distributed import all_reduce
         multi = dist.is_initialized() and dist.get_world_size() > 1
         snap = _snapshot(model, optimizer)
         cands = ([(True, r) for r in self._reserved_candidates] if True in self._forms else []) + \
@@ -438,7 +440,7 @@ class CapturedTrainStep:
             times.append(time.perf_counter() - t0)
         t = torch.tensor(times, dtype=torch.float64, device=self.y.device)
         if multi:
-            dist.all_reduce(t, op=dist.ReduceOp.MAX)      # every rank takes the same decision
+            all_reduce(t, op=dist.ReduceOp.MAX)      # every rank takes the same decision
         t = [1e3 * v / steps for v in t.tolist()]
         two = [i for i, (f, _) in enumerate(cands) if f is True]
         ser = [i for i, (f, _) in enumerate(cands) if f is False]

@@ -95,7 +95,7 @@ def check_split(rank, world, dev, overlap="1"):
     # the ranks' parameters after the steps are the same BITS (same reduced gradients, same update)
     mine = torch.cat([p.detach().reshape(-1) for p in model.parameters()])
     root = mine.clone()
-    dist.broadcast(root, src=0)
+    D.broadcast(root, src=0)
     assert torch.equal(mine, root), f"rank {rank}: parameters differ from rank 0's after {steps} steps"
     # one rank, whole batch, eager, no collective
     ref.train()
@@ -149,7 +149,7 @@ def check_tail(rank, world, dev):
             for p in ref.parameters():
                 if p.grad is None:
                     p.grad = torch.zeros_like(p)
-                dist.all_reduce(p.grad)
+                D.all_reduce(p.grad)
                 p.grad /= world
             ropt.step()
     torch.cuda.synchronize()

@@ -36,7 +36,7 @@ def main():
                           model_save_path_finetune=os.path.join(tmp, f"f{rank}.pt"))
     tr, va = train_model_device(cfg, dev, model, dds, list(range(96)), list(range(96, 112)), opt, losses.regression_loss, seed=5)
     assert all(map(lambda v: v == v, tr + va)), "non-finite loss"
-    flat = torch.cat([p.detach().reshape(-1) for p in model.parameters()])
+    flat = torch.cat([p.detach().reshape(-1) for p in model.parameters()]).cpu()      # (gloo: host tensors only)
     gathered = [torch.zeros_like(flat) for _ in range(world)]
     dist.all_gather(gathered, flat)
     spread = max(float((g - gathered[0]).abs().max()) for g in gathered)
