@@ -24,7 +24,7 @@ _P, _I, _F, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlo
 
 # symbol -> argtypes ; keep in sync with include/immunostruct_hip.h
 _RETURNS_LONGLONG = {"is_attn_colmean_probs_floats", "is_contrastive_scratch_floats", "is_contrastive_work_floats",
-                     "is_linear_dgrad_scratch_floats"}
+                     "is_linear_dgrad_scratch_floats", "is_diff_attention_work_floats", "is_group_norm_work_floats"}
 SIGNATURES = {
     "is_version": [],
     "is_last_error_string": [],
@@ -94,6 +94,14 @@ SIGNATURES = {
     "is_vae_latent_bwd_wgrad": [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P],
     "is_recon_mse": [_P, _P, _P, _LL, _F, _P, _P],
     "is_vae_loss": [_P, _P, _P, _LL, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _F, _F, _F, _F, _P, _P, _P, _P],
+    "is_rotary": [_P, _LL, _LL, _LL, _P, _I, _P, _LL, _LL, _LL, _P, _I, _P, _I, _LL, _LL, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P],
+    "is_diff_attention_splits": [_I, _I, _I, _I],
+    "is_diff_attention_work_floats": [_I, _I, _I, _I, _I],
+    "is_diff_attention_fwd": [_P, _P],
+    "is_diff_attention_bwd": [_P, _P],
+    "is_group_norm_work_floats": [_P, _I],
+    "is_group_norm_fwd": [_P, _P],
+    "is_group_norm_bwd": [_P, _P],
 }
 
 
@@ -134,6 +142,26 @@ class RandJob(ctypes.Structure):
 class CopyJob(ctypes.Structure):
     """one job of is_multi_copy"""
     _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("bytes", ctypes.c_longlong)]
+
+
+class DiffAttention(ctypes.Structure):
+    """arguments of is_diff_attention_{fwd,bwd} (mirrors `IsDiffAttention` in include/immunostruct_hip.h)"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "lam", "lengths", "o", "o2", "lse", "work", "d_o", "dots", "dq", "dk",
+                                               "dv_out", "dlam")] + \
+               [(n, ctypes.c_longlong) for n in ("q_b", "q_n", "q_h", "k_b", "k_n", "k_h", "v_b", "v_n", "v_h")] + \
+               [(n, ctypes.c_int) for n in ("batch", "nq", "nk", "heads", "kv_heads", "d", "dv", "causal", "type", "lam_type", "splits",
+                                            "group", "vec")] + [("scale", ctypes.c_float)]
+
+
+class GroupNorm(ctypes.Structure):
+    """arguments of is_group_norm_{fwd,bwd} (mirrors `IsGroupNorm` in include/immunostruct_hip.h)"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "lengths", "y", "stats", "work", "dy", "dx", "dweight", "dbias")] + \
+               [(n, ctypes.c_longlong) for n in ("x_b", "x_n")] + \
+               [(n, ctypes.c_int) for n in ("batch", "n", "channels", "groups", "activation", "type", "weight_type", "pad")] + \
+               [("eps", ctypes.c_float)]
+
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # the `type` argument of the sequence operators
 
 
 _lib = None
@@ -199,6 +227,20 @@ def rows_ld(t):
     if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
     return t, int(t.stride(0))
+
+
+def last_contiguous(t):
+    """the tensor itself, or a contiguous copy where its innermost dimension is not laid out element by element (a broadcast input)"""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def same_device(first, *tensors):
+    """the device every given tensor lives on; raises when one is elsewhere"""
+    require_device(first, *tensors)
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    return first.device
 
 
 def check(code, what):

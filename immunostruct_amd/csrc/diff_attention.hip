@@ -1,0 +1,77 @@
+// Differential attention: the C ABI's entry points (kernels and their reasons: diff_attention.h).
+#include "diff_attention.h"
+
+using namespace is;
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// what both directions check; fills in the derived fields
+int prepare(da::Args& a) {
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.lam == nullptr || a.o == nullptr) return -22;
+  if (a.batch < 1 || a.nq < 1 || a.nk < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.d < 1 || a.dv < 1) return -22;
+  if (a.type < TYPE_F32 || a.type > TYPE_F16 || (a.lam_type != TYPE_F32 && a.lam_type != a.type) || a.causal < 0 || a.causal > 2) return -22;
+  if (!(a.scale > 0.0f) || !(a.scale < INFINITY) || a.splits < 1) return -22;
+  a.group = a.heads / a.kv_heads;
+  const long long rows = (long long)a.nq * a.group, big = 0x7fffff00LL;
+  if (rows > big || a.nk > big || (rows / 32 + 1) * a.splits * a.kv_heads > big / a.batch || (rows + 3) * a.kv_heads > big / a.batch ||
+      (a.nk / 32 + 1LL) * a.kv_heads > big / a.batch) return -22;
+  if (da::class_of(a) == 0) return -38;
+  const int n = a.type == TYPE_F32 ? 4 : 8;
+  const long long strides = a.q_b | a.q_n | a.q_h | a.k_b | a.k_n | a.k_h | a.v_b | a.v_n | a.v_h;
+  a.vec = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.o) && aligned16(a.o2) && aligned16(a.d_o) && aligned16(a.dq) &&
+          aligned16(a.dk) && aligned16(a.dv_out) && strides % n == 0 && a.d % n == 0 && a.dv % n == 0;
+  return 0;
+}
+
+int run(const da::Args& a, bool backward, const char* entry, void* stream) {
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a.type == TYPE_F32) da::run_f32(a, backward, st);
+  else if (a.type == TYPE_BF16) da::run_bf16(a, backward, st);
+  else da::run_f16(a, backward, st);
+  return launch_status(entry);
+}
+
+}  // namespace
+
+extern "C" {
+
+// Splits of the keys: enough workgroups for 256 CUs where the rows alone do not give them (a wave works on 32 rows; up to 32 rows are one
+// wave per workgroup, four of which fill a CU), at least 128 keys each.
+int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk) {
+  if (batch < 1 || kv_heads < 1 || rows < 1 || nk < 1) return 1;
+  const long long groups = (rows <= 32 ? 1LL : (rows + 127LL) / 128) * kv_heads * batch;
+  const long long want = (rows <= 32 ? 1024 : 512) / groups, most = (nk + 127LL) / 128;
+  const long long s = want < most ? want : most;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+long long is_diff_attention_work_floats(int batch, int kv_heads, int rows, int dv, int splits) {
+  return splits <= 1 ? 0 : 2LL * batch * kv_heads * splits * rows * (dv + 2);
+}
+
+int is_diff_attention_fwd(const IsDiffAttention* args, void* stream) {
+  if (args == nullptr) return fail("is_diff_attention_fwd", -22);
+  da::Args a = *args;
+  a.d_o = nullptr;
+  a.dq = a.dk = a.dv_out = a.dlam = nullptr;
+  const int rc = prepare(a);
+  if (rc != 0) return fail("is_diff_attention_fwd", rc);
+  if ((a.lse == nullptr) != (a.o2 == nullptr) || (a.splits > 1 && a.work == nullptr)) return fail("is_diff_attention_fwd", -22);
+  return run(a, false, "is_diff_attention_fwd", stream);
+}
+
+int is_diff_attention_bwd(const IsDiffAttention* args, void* stream) {
+  if (args == nullptr) return fail("is_diff_attention_bwd", -22);
+  da::Args a = *args;
+  a.splits = 1;
+  const int rc = prepare(a);
+  if (rc != 0) return fail("is_diff_attention_bwd", rc);
+  if (a.o2 == nullptr || a.lse == nullptr || a.d_o == nullptr || a.dots == nullptr || a.dq == nullptr || a.dk == nullptr ||
+      a.dv_out == nullptr || a.dlam == nullptr)
+    return fail("is_diff_attention_bwd", -22);
+  return run(a, true, "is_diff_attention_bwd", stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,205 @@
+// Matrix-core tiles of the sequence-attention kernels: element types, LDS tile layouts, operand moves (gfx950).
+//
+// Every product is built from 32 x 32 output tiles; lane l, r = l & 31, g = l >> 5.  An operand "chunk" is 16 bytes of one row: 8 elements
+// of a 16-bit type (one v_mfma_f32_32x32x16) or 4 floats (four v_mfma_f32_32x32x2_f32).  Chunk 2 j + g of row r is lane (r, g)'s share of
+// step j, for A and B alike, so the k order inside a step never matters.
+//   accumulator register t of lane (r, g): row 8 (t >> 2) + 4 g + (t & 3), column r.
+// A product whose LEFT operand was just accumulated reuses it in place: accumulator rows 8 u + 4 g .. + 3 are the k values of lane group g
+// in step u, and the other operand is read TRANSPOSED from its row-major LDS tile in the same order (ds_read_b64_tr_b16: four rows of one
+// column per lane; 32-bit: four plain reads).  No score ever travels through LDS.
+#pragma once
+#include "common.h"
+
+namespace is {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+enum { TYPE_F32 = 0, TYPE_BF16 = 1, TYPE_F16 = 2 };      // the C ABI's `type` argument
+
+// 16 bytes <-> floats
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(u32x4_t c, float (&x)[4]) {
+    const f32x4 v = __builtin_bit_cast(f32x4, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  }
+  static __device__ __forceinline__ u32x4_t pack(const float (&x)[4]) { return __builtin_bit_cast(u32x4_t, f32x4{x[0], x[1], x[2], x[3]}); }
+};
+template <typename T> struct Vec {
+  static constexpr int N = 8;
+  typedef T V __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ void unpack(u32x4_t c, float (&x)[8]) {
+    const V v = __builtin_bit_cast(V, c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+  }
+  static __device__ __forceinline__ u32x4_t pack(const float (&x)[8]) {
+    V v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)x[i];
+    return __builtin_bit_cast(u32x4_t, v);
+  }
+};
+
+// a chunk of a row in global memory: elements [c * N, c * N + N) of which the first `len` of the row exist (the rest are 0).
+// vec: rows are 16-byte aligned and `len` is a multiple of N, so a chunk is there whole or not at all.
+template <typename T>
+__device__ __forceinline__ u32x4_t load_chunk(const T* row, int c, int len, bool vec) {
+  constexpr int N = Vec<T>::N;
+  u32x4_t out = {0u, 0u, 0u, 0u};
+  if (vec) {
+    if (c * N < len) out = *reinterpret_cast<const u32x4_t*>(row + c * N);
+  } else {
+    T x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = c * N + i < len ? row[c * N + i] : (T)0.0f;
+    __builtin_memcpy(&out, x, 16);
+  }
+  return out;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma_chunk(u32x4_t a, u32x4_t b, f32x16 c) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+    return c;
+  } else if constexpr (__is_same(T, __bf16)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+// Row-major LDS tile of N-element rows, addressed in 16-byte chunks.
+//   16-bit types: rows are a power of two >= 64 bytes, no padding; chunk c of a row sits at slot c ^ swizzle(row), chosen so that both the
+//   row-per-lane b128 reads (16 rows, one chunk) and the transposed reads (4 rows x 64 bytes per 32 lanes) touch all 64 banks once.
+//   float: one chunk of padding per row (b128 rows conflict-free; the b32 transposed reads are 2-way, hidden behind the 64-cycle MFMAs).
+template <typename T, int N>
+struct Tile {
+  static constexpr int CHUNKS = N * (int)sizeof(T) / 16;
+  static constexpr int STRIDE = N * (int)sizeof(T) + (sizeof(T) == 4 ? 16 : 0);
+  static constexpr int bytes(int rows) { return rows * STRIDE; }
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (sizeof(T) == 4) return 0;
+    else if constexpr (CHUNKS >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (CHUNKS == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+  }
+  static __device__ __forceinline__ int offset(int row, int chunk) { return row * STRIDE + ((chunk ^ swizzle(row)) << 4); }
+  // lane (r, g)'s share of step j of the rows [row0, row0 + 32)
+  static __device__ __forceinline__ u32x4_t rows(const char* tile, int row0, int j, int lane) {
+    return *reinterpret_cast<const u32x4_t*>(tile + offset(row0 + (lane & 31), 2 * j + (lane >> 5)));
+  }
+};
+
+// acc (32 x 32) += tile rows [row0, row0 + 32) . b, b = the register-resident other operand (N / (2 Vec::N) steps)
+template <typename T, int N>
+__device__ __forceinline__ void mm_tile(f32x16& acc, const char* tile, int row0, const u32x4_t (&b)[N / (2 * Vec<T>::N)], int lane) {
+#pragma unroll
+  for (int j = 0; j < N / (2 * Vec<T>::N); ++j) acc = mfma_chunk<T>(Tile<T, N>::rows(tile, row0, j, lane), b[j], acc);
+}
+
+// acc[m][t] (32 x 32: rows = columns 32 t .. of the tile, columns = p's columns) += (tile rows [row0, row0 + 32))^T . p[m]
+template <typename T, int N, int NT, int NB>
+__device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NB][NT], const char* tile, int row0, const f32x16 (&p)[NB], int lane) {
+  const int g = lane >> 5;
+  if constexpr (sizeof(T) == 4) {
+    const char* base = tile + (row0 + 4 * g) * Tile<T, N>::STRIDE + (lane & 31) * 4;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float a = *reinterpret_cast<const float*>(base + (8 * u + e) * Tile<T, N>::STRIDE + t * 128);
+#pragma unroll
+          for (int m = 0; m < NB; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[m][4 * u + e], acc[m][t], 0, 0, 0);
+        }
+  } else {
+    typedef T V __attribute__((ext_vector_type(8)));
+    const int i = lane & 15, row = 4 * g + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4_t b[NB];
+#pragma unroll
+      for (int m = 0; m < NB; ++m) {
+        V v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T)p[m][8 * h + e];      // one rounding to the inputs' type: what the matrix instruction takes
+        b[m] = __builtin_bit_cast(u32x4_t, v);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        u32x2 half[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int rr = row0 + 8 * (2 * h + w) + row;
+          const char* at = tile + Tile<T, N>::offset(rr, 4 * t + c) + (i & 1) * 8;
+          half[w] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+        }
+        const u32x4_t a = {half[0][0], half[0][1], half[1][0], half[1][1]};
+#pragma unroll
+        for (int m = 0; m < NB; ++m) acc[m][t] = mfma_chunk<T>(a, b[m], acc[m][t]);
+      }
+    }
+  }
+}
+
+// ROWS rows of N elements, global -> registers -> LDS by NTHREADS threads; `row(i)` gives the address of tile row i
+template <typename T, int N, int ROWS, int NTHREADS>
+struct Stage {
+  static constexpr int TOTAL = ROWS * Tile<T, N>::CHUNKS, PER = (TOTAL + NTHREADS - 1) / NTHREADS;
+  u32x4_t v[PER];
+  template <typename RowF>
+  __device__ __forceinline__ void load(int tid, RowF row, int len, bool vec) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int s = tid + k * NTHREADS;
+      if (TOTAL % NTHREADS == 0 || s < TOTAL) v[k] = load_chunk<T>(row(s / Tile<T, N>::CHUNKS), s % Tile<T, N>::CHUNKS, len, vec);
+    }
+  }
+  __device__ __forceinline__ void store(int tid, char* tile) const {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int s = tid + k * NTHREADS;
+      if (TOTAL % NTHREADS == 0 || s < TOTAL)
+        *reinterpret_cast<u32x4_t*>(tile + Tile<T, N>::offset(s / Tile<T, N>::CHUNKS, s % Tile<T, N>::CHUNKS)) = v[k];
+    }
+  }
+};
+
+// four consecutive elements of an output row (columns [col, col + 4) of which those below `len` exist)
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int col, int len, f32x4 x, bool vec) {
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  if (vec) {
+    if (col < len) {
+      V4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)x[e];
+      *reinterpret_cast<V4*>(row + col) = v;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < len) row[col + e] = (T)x[e];
+  }
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// workgroup `id` of `total` -> position in the work list such that every XCD (id mod 8) gets one contiguous range of it: neighbours share
+// an XCD's L2
+__device__ __forceinline__ int xcd_order(int id, int total) {
+  const int x = id & 7, k = id >> 3, q = total >> 3, rem = total & 7;
+  return x * q + (x < rem ? x : rem) + k;
+}
+
+}  // namespace is

@@ -8,9 +8,11 @@ stream.  There is no fallback path: CPU tensors raise ``HipExtensionError``.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
+import contextlib
 import ctypes
 import os
 
@@ -1757,3 +1759,278 @@ def vae_loss(recon, x, mu, logvar, logit, y, mode, pos_weight, c_pred, c_mse, c_
     return VaeLossFn.apply(recon, x, mu, logvar, logit, y, mode, pos_weight, c_pred, c_mse, c_kld, pre)
 
 
+# ---- operators of attention blocks over sequences (csrc/rotary.hip, diff_attention*.hip, group_norm.hip) ----------------------------------
+# fp32, bf16 and fp16; they run on the tensors' own device and its current stream, also where that device is not the current one.
+
+def _on(device):
+    """context that makes ``device`` the current one (nothing to do, and nothing spent, where it is already)"""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _sequence_type(name, *tensors):
+    """raises unless the operator's tensors have one element type that the kernels are built for"""
+    t = tensors[0].dtype
+    if t not in _lib.TYPES:
+        raise ValueError(f"{name}: expected float32, bfloat16 or float16 tensors, got {t}")
+    if any(u is not None and u.dtype != t for u in tensors):
+        raise ValueError(f"{name}: tensors of different types {[u.dtype for u in tensors if u is not None]}")
+
+
+def _check_lengths(name, lengths, batch):
+    if lengths is None:
+        return None
+    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch:
+        raise ValueError(f"{name}: lengths has to be an int32 tensor of ({batch},)")
+    return lengths.contiguous()
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _rotary_launch(q, k, freq, positions, layout, amplitude, inverse):
+    lib = _lib.load()
+    b, n, _, width = q.shape
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    if b == 0 or n == 0:
+        return outs
+    args = []
+    for t, o in zip((q, k), outs):
+        if t is None:
+            args += [None, 0, 0, 0, None, 0]
+        else:
+            t = _lib.last_contiguous(t)      # (a copy, where one is made, lives until the launch below is enqueued on its stream)
+            args += [_lib.ptr(t), t.stride(0), t.stride(1), t.stride(2), _lib.ptr(o), t.shape[2]]
+    pos = (None, 0, 0, 0)
+    if positions is not None:
+        pos = (_lib.ptr(positions), int(positions.dtype == torch.int64), positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1))
+    with _on(q.device), KernelTimer.span("rotary"):
+        _lib.check(lib.is_rotary(*args, *pos, freq.data_ptr(), b, n, width, 2 * freq.numel(), int(layout == "interleaved"), int(inverse),
+                                 amplitude, _lib.TYPES[q.dtype], _lib.stream_ptr()), "is_rotary")
+    return outs
+
+
+class RotaryFn(torch.autograd.Function):
+    """q (B, n, heads, width) and k (B, n, kv_heads, width) turned by their positions in one launch (``csrc/rotary.hip``); the backward is
+    the opposite turn."""
+
+    @staticmethod
+    def forward(ctx, q, k, freq, positions, layout, amplitude):
+        ctx.set_materialize_grads(False)
+        ctx.cfg = (freq, layout, amplitude)
+        ctx.save_for_backward(positions)
+        q_out, k_out = _rotary_launch(q, k, freq, positions, layout, amplitude, False)
+        return q_out if k is None else (q_out, k_out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk=None):
+        (positions,) = ctx.saved_tensors
+        freq, layout, amplitude = ctx.cfg
+        if gq is not None:
+            gq, gk = _rotary_launch(gq, gk, freq, positions, layout, amplitude, True)
+        elif gk is not None:
+            gk, _ = _rotary_launch(gk, None, freq, positions, layout, amplitude, True)
+        return gq, gk, None, None, None, None
+
+
+def rotary(q, k, freq, positions=None, layout="half", amplitude=1.0):
+    """Rotary positions: the first ``2 * len(freq)`` elements of every head turned in pairs, ``(a, b) -> amplitude * (a cos t - b sin t,
+    a sin t + b cos t)`` with ``t = position * freq[pair]``; the rest of the head is copied.
+
+    ``q`` (B, n, heads, width) and ``k`` (B, n, kv_heads, width) or None; any strides, fp32 / bf16 / fp16.  ``freq``: radians per position,
+    a float64 tensor on the HOST (``nn.RotaryEmbedding`` holds one).  ``positions``: int32 / int64 (n,) or (B, n) on the device, None = 0 ...
+    n - 1; angles are formed in 64 bits.  ``layout``: "half" pairs element p with p + len(freq), "interleaved" 2 p with 2 p + 1.  Returns
+    (q', k'), k' None without k."""
+    _sequence_type("rotary", q, k)
+    if q.dim() != 4 or q.shape[2] < 1 or (k is not None and (k.dim() != 4 or k.shape[2] < 1 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise ValueError("rotary: expected q (B, n, heads, width) and k (B, n, kv_heads, width)")
+    if freq.is_cuda or freq.dtype != torch.float64 or freq.dim() != 1 or not 1 <= freq.numel() <= 256 or 2 * freq.numel() > q.shape[3]:
+        raise ValueError("rotary: freq has to be a float64 host tensor of 1 ... min(256, width / 2) frequencies")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"rotary: unknown layout {layout!r}")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64)
+                                  or tuple(positions.shape) not in ((q.shape[1],), (q.shape[0], q.shape[1]))):
+        raise ValueError("rotary: positions has to be an int32 / int64 tensor of (n,) or (B, n)")
+    _lib.same_device(q, k, positions)
+    freq, amplitude = freq.contiguous(), float(amplitude)
+    if not _needs_grad(q, k):
+        return tuple(_rotary_launch(q, k, freq, positions, layout, amplitude, False))
+    out = RotaryFn.apply(q, k, freq, positions, layout, amplitude)
+    return out if k is not None else (out, None)
+
+
+_CAUSAL = {None: 0, "start": 1, "end": 2}
+
+
+def _diff_forward(q, k, v, lam, lengths, causal, scale, need):
+    """launches of the forward pass -> (out, o2, lse, arguments); o2 and lse (what the backward needs) are None unless ``need``"""
+    lib = _lib.load()
+    b, nq, h2, d = q.shape
+    nk, hk, dv = v.shape[1:]
+    heads = h2 // 2
+    rows = nq * heads // hk
+    out = torch.empty(b, nq, heads, dv, dtype=q.dtype, device=q.device)
+    o2 = torch.empty_like(out) if need else None
+    lse = torch.empty(b, hk, 2, rows, dtype=torch.float32, device=q.device) if need else None
+    if out.numel() == 0 or nk == 0:      # nobody asks, or there is nothing to see
+        return out.zero_(), o2, lse, None
+    splits = lib.is_diff_attention_splits(b, hk, rows, nk)
+    floats = lib.is_diff_attention_work_floats(b, hk, rows, dv, splits)
+    work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    ptr = lambda t: None if t is None else t.data_ptr()
+    a = _lib.DiffAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), ptr(lengths), out.data_ptr(), ptr(o2), ptr(lse), ptr(work),
+                           None, None, None, None, None, None, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                           b, nq, nk, heads, hk, d, dv, causal, _lib.TYPES[q.dtype], _lib.TYPES[lam.dtype], splits, 0, 0, scale)
+    with _on(q.device), KernelTimer.span("diff_attention_fwd"):
+        _lib.check(lib.is_diff_attention_fwd(ctypes.byref(a), _lib.stream_ptr()), "is_diff_attention_fwd")
+    return out, o2, lse, a
+
+
+class DifferentialAttentionFn(torch.autograd.Function):
+    """The difference of two softmax maps over shared values (``csrc/diff_attention.h``); see :func:`differential_attention`."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, lengths, causal, scale):
+        q, k, v, lam = (_lib.last_contiguous(t) for t in (q, k, v, lam))
+        out, o2, lse, ctx.args = _diff_forward(q, k, v, lam, lengths, causal, scale, True)
+        ctx.save_for_backward(q, k, v, lam, lengths, out, o2, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        lib = _lib.load()
+        q, k, v, lam, lengths, out, o2, lse = ctx.saved_tensors
+        dq, dk, dv, dlam = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, lam))
+        if ctx.args is None:
+            return dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), None, None, None
+        g = g.contiguous()
+        dots = torch.empty_like(lse)
+        a = _lib.DiffAttention.from_buffer_copy(ctx.args)      # (the forward's arguments with this call's buffers; its workspace is gone)
+        a.work, a.splits = None, 1
+        a.d_o, a.dots, a.dq, a.dk, a.dv_out, a.dlam = (t.data_ptr() for t in (g, dots, dq, dk, dv, dlam))
+        with _on(q.device), KernelTimer.span("diff_attention_bwd"):
+            _lib.check(lib.is_diff_attention_bwd(ctypes.byref(a), _lib.stream_ptr()), "is_diff_attention_bwd")
+        return dq, dk, dv, dlam, None, None, None
+
+
+def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
+    """Differential attention: per head ``(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v``.
+
+    ``q`` (B, nq, 2 heads, d): head h's two maps are heads 2 h and 2 h + 1; ``k`` (B, nk, 2 kv_heads, d) likewise; ``v`` (B, nk, kv_heads, dv);
+    heads a multiple of kv_heads (query head h reads key head h // (heads / kv_heads)).  fp32 (d <= 64, dv <= 128), bf16 or fp16 (d <= 128,
+    dv <= 256); any strides.  ``lam`` (heads,): in the same type or fp32, learned (its gradient is returned).
+    ``lengths`` (B,) int32: keys at or behind a sample's length do not exist (whatever their memory holds); all nk without it.
+    ``causal``: None; "start": query i is position i and sees keys <= i; "end": the queries are the sample's last nq positions, i.e. new
+    tokens over a cache, and see keys <= i + length - nq.  ``scale``: a positive number, d ** -0.5 by default.
+    A query that sees no key gives zeros and passes no gradient.  Returns (B, nq, heads, dv).  Deterministic; scores, softmax statistics
+    and sums are 32-bit, softmax weights and score gradients are rounded once to the inputs' type for the matrix products."""
+    _sequence_type("differential_attention", q, k, v)
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or lam.dim() != 1:
+        raise ValueError("differential_attention: expected q (B, nq, 2 heads, d), k (B, nk, 2 kv_heads, d), v (B, nk, kv_heads, dv), lam (heads,)")
+    b, nq, h2, d = q.shape
+    nk, hk, dv = v.shape[1:]
+    if (min(h2, hk, d, dv) < 1 or h2 % 2 or (h2 // 2) % hk or tuple(k.shape) != (b, nk, 2 * hk, d) or v.shape[0] != b or lam.shape[0] != h2 // 2):
+        raise ValueError(f"differential_attention: shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, lam {tuple(lam.shape)}")
+    if lam.dtype not in (torch.float32, q.dtype):
+        raise ValueError(f"differential_attention: lam has to be float32 or {q.dtype}")
+    if causal not in _CAUSAL:
+        raise ValueError(f"differential_attention: causal has to be None, 'start' or 'end', got {causal!r}")
+    lengths = _check_lengths("differential_attention", lengths, b)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("differential_attention: scale has to be a positive number")
+    limit = 64 if q.dtype == torch.float32 else 128
+    if d > limit or dv > 2 * limit:
+        raise NotImplementedError(f"differential_attention: heads of {d} / values of {dv} elements (the kernels: up to {limit} / {2 * limit} in {q.dtype})")
+    _lib.same_device(q, k, v, lam, lengths)
+    if not _needs_grad(q, k, v, lam):
+        return _diff_forward(*(_lib.last_contiguous(t) for t in (q, k, v, lam)), lengths, _CAUSAL[causal], scale, False)[0]
+    return DifferentialAttentionFn.apply(q, k, v, lam, lengths, _CAUSAL[causal], scale)
+
+
+_ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "relu": 3}
+
+
+def _group_norm_launch(x, weight, bias, lengths, groups, eps, activation):
+    """-> (y, stats, arguments); x (B, n, channels) with a unit innermost stride"""
+    lib = _lib.load()
+    b, n, c = x.shape
+    y = torch.empty(b, n, c, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y, None, None
+    stats = torch.empty(b, groups, 2, dtype=torch.float32, device=x.device)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    a = _lib.GroupNorm(x.data_ptr(), ptr(weight), ptr(bias), ptr(lengths), y.data_ptr(), stats.data_ptr(), None, None, None, None, None,
+                       x.stride(0), x.stride(1), b, n, c, groups, activation, _lib.TYPES[x.dtype],
+                       0 if weight is None else _lib.TYPES[weight.dtype], 0, eps)
+    floats = lib.is_group_norm_work_floats(ctypes.byref(a), 0)
+    work = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
+    a.work = ptr(work)
+    with _on(x.device), KernelTimer.span("group_norm_fwd"):
+        _lib.check(lib.is_group_norm_fwd(ctypes.byref(a), _lib.stream_ptr()), "is_group_norm_fwd")
+    return y, stats, a
+
+
+class GroupNormFn(torch.autograd.Function):
+    """Group norm with an activation, channels last (``csrc/group_norm.hip``); see :func:`group_norm`.  x (B, n, channels)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, lengths, groups, eps, activation):
+        x = _lib.last_contiguous(x)
+        y, stats, ctx.args = _group_norm_launch(x, weight, bias, lengths, groups, eps, activation)
+        ctx.save_for_backward(x, weight, bias, lengths, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        lib = _lib.load()
+        x, weight, bias, lengths, stats = ctx.saved_tensors
+        dx, dw, db = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, weight, bias))
+        if ctx.args is None:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None, None, None
+        a = _lib.GroupNorm.from_buffer_copy(ctx.args)
+        g = g.contiguous()
+        floats = lib.is_group_norm_work_floats(ctypes.byref(a), 1)
+        work = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
+        a.y, a.dy, a.dx = None, g.data_ptr(), dx.data_ptr()
+        a.dweight, a.dbias, a.work = (None if t is None else t.data_ptr() for t in (dw, db, work))
+        with _on(x.device), KernelTimer.span("group_norm_bwd"):
+            _lib.check(lib.is_group_norm_bwd(ctypes.byref(a), _lib.stream_ptr()), "is_group_norm_bwd")
+        return dx, dw, db, None, None, None, None
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lengths=None):
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)``, channels last: ``x`` (B, ..., channels), mean and variance of each sample over all
+    positions in between and the ``channels / groups`` channels of each group.  (B * n, channels) therefore normalises every row on its own.
+
+    fp32 / bf16 / fp16 with 32-bit statistics; ``weight`` and ``bias`` (channels,) in x's type or fp32, both or neither; ``activation``: None
+    ("none"), "silu", "gelu" (erf), "relu".  ``lengths`` (B,) int32, for x (B, n, channels): rows at or behind a sample's length are not part
+    of it -- they are not read, come back as zeros and get no gradient."""
+    _sequence_type("group_norm", x)
+    if x.dim() < 2 or groups < 1 or x.shape[-1] < 1 or x.shape[-1] % groups:
+        raise ValueError(f"group_norm: expected x (B, ..., channels) with channels a multiple of {groups} groups, got {tuple(x.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"group_norm: unknown activation {activation!r}")
+    if (weight is None) != (bias is None):
+        raise ValueError("group_norm: weight and bias come together")
+    if weight is not None:
+        c = (x.shape[-1],)
+        if tuple(weight.shape) != c or tuple(bias.shape) != c or weight.dtype != bias.dtype or weight.dtype not in (torch.float32, x.dtype):
+            raise ValueError(f"group_norm: weight and bias have to be ({c[0]},) in float32 or {x.dtype}")
+        weight, bias = weight.contiguous(), bias.contiguous()
+    if lengths is not None and x.dim() != 3:
+        raise ValueError("group_norm: lengths goes with x (B, n, channels)")
+    lengths = _check_lengths("group_norm", lengths, x.shape[0])
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("group_norm: eps has to be a number >= 0")
+    _lib.same_device(x, weight, bias, lengths)
+    x3 = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
+    if _needs_grad(x, weight, bias):
+        y = GroupNormFn.apply(x3, weight, bias, lengths, int(groups), eps, _ACTIVATIONS[activation])
+    else:
+        y = _group_norm_launch(_lib.last_contiguous(x3), weight, bias, lengths, int(groups), eps, _ACTIVATIONS[activation])[0]
+    return y.view(x.shape)

@@ -8,6 +8,8 @@ Drop-in replacements (same names, argument meaning and return values) for
 * ``torch_geometric.nn.global_mean_pool(x, batch)`` / ``global_max_pool`` --
   reference ``models/hybrid_models.py:97,331``, ``ablation_models.py:296-297``.
 
+Beside them, for attention blocks over residues (``models.layers.DifferentialAttention`` is one): ``RotaryEmbedding`` and ``GroupNorm``.
+
 ``EGNNConv`` keeps DGL's parameter layout (``edge_mlp.{0,2}``,
 ``node_mlp.{0,2}``, ``coord_mlp.{0,2}``) so reference checkpoints load
 unchanged.  How the layer is evaluated differs from DGL by design:
@@ -20,6 +22,8 @@ unchanged.  How the layer is evaluated differs from DGL by design:
   (``csrc/egnn_layer_fwd.hip``).
 """
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn as nn
@@ -155,3 +159,79 @@ def global_mean_pool(x, batch, size=None):
 
 def global_max_pool(x, batch, size=None):
     return HF.segment_pool(x, _seg_ptr_from_batch(batch, size), "max")
+
+
+class RotaryEmbedding(nn.Module):
+    """Rotary positions of attention heads: ``forward(q, k, positions=None) -> (q', k')`` (``functional.rotary``).
+
+    ``dims``: how many leading elements of a head are turned (even); ``layout``: "half" | "interleaved"; frequencies ``base ** (-2 p / dims)``.
+    ``scaling`` stretches them for contexts longer than the trained one, ``factor`` times as long:
+
+    * ``dict(kind="linear", factor=s)``: every frequency divided by s;
+    * ``dict(kind="ntk", factor=s)``: base raised by ``s ** (dims / (dims - 2))``;
+    * ``dict(kind="yarn", factor=s, original_length=n, beta_fast=32, beta_slow=1, amplitude=None)``: pairs that turn more than ``beta_fast``
+      times over the original length keep their frequency, those below ``beta_slow`` turns are divided by s, a linear ramp between; q and k are
+      scaled by ``amplitude`` (``0.1 ln s + 1``).
+
+    The frequencies are 64-bit numbers on the host and travel with the launch: no table, no length limit, nothing to move between devices."""
+
+    def __init__(self, dims, base=10000.0, layout="half", scaling=None):
+        super().__init__()
+        if dims < 2 or dims % 2 or dims > 512:
+            raise ValueError("RotaryEmbedding: dims has to be an even number of 2 ... 512")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"RotaryEmbedding: unknown layout {layout!r}")
+        if not base > 1:
+            raise ValueError("RotaryEmbedding: base has to be above 1")
+        self.dims, self.base, self.layout, self.scaling = dims, float(base), layout, dict(scaling) if scaling else None
+        self.amplitude = 1.0
+        pair = torch.arange(dims // 2, dtype=torch.float64)
+        cfg = dict(self.scaling or {})
+        kind, s = cfg.pop("kind", None), float(cfg.pop("factor", 1.0))
+        if kind not in (None, "linear", "ntk", "yarn") or not 1.0 <= s < math.inf or (self.scaling and kind is None):
+            raise ValueError(f"RotaryEmbedding: unknown scaling {scaling!r}")
+        if kind == "ntk":
+            if dims == 2:
+                raise ValueError("RotaryEmbedding: 'ntk' needs at least two pairs")
+            base = self.base * s ** (dims / (dims - 2.0))
+        freq = float(base) ** (-2.0 * pair / dims)
+        if kind == "linear":
+            freq = freq / s
+        elif kind == "yarn":
+            length, fast, slow = float(cfg.pop("original_length")), float(cfg.pop("beta_fast", 32.0)), float(cfg.pop("beta_slow", 1.0))
+            amplitude = cfg.pop("amplitude", None)
+            if length <= 0 or not fast > slow > 0:
+                raise ValueError(f"RotaryEmbedding: unknown scaling {scaling!r}")
+            at = [dims * math.log(length / (2.0 * math.pi * turns)) / (2.0 * math.log(self.base)) for turns in (fast, slow)]
+            low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
+            ramp = ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+            freq = freq * (1.0 - ramp) + freq / s * ramp
+            self.amplitude = 0.1 * math.log(s) + 1.0 if amplitude is None else float(amplitude)
+        if cfg:
+            raise ValueError(f"RotaryEmbedding: unknown scaling options {sorted(cfg)}")
+        self.freq = freq      # (a plain attribute: no part of state_dict, untouched by .half() / .to())
+
+    def forward(self, q, k=None, positions=None):
+        return HF.rotary(q, k, self.freq, positions, self.layout, self.amplitude)
+
+    def extra_repr(self):
+        return f"{self.dims}, base={self.base:g}, layout={self.layout!r}, scaling={self.scaling}"
+
+
+class GroupNorm(nn.Module):
+    """Group norm with an activation over channels-last features (``functional.group_norm``): (B, ..., channels), for padded batches of
+    residue graphs or sequences with ``lengths``.  Parameters as ``torch.nn.GroupNorm``'s."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError("num_channels must be divisible by num_groups")
+        self.num_groups, self.num_channels, self.eps, self.activation = num_groups, num_channels, eps, activation
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x, lengths=None):
+        return HF.group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation, lengths)
+
+    def extra_repr(self):
+        return f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.weight is not None}, activation={self.activation!r}"

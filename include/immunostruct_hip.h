@@ -427,6 +427,66 @@ int is_vae_loss(const float* recon, const float* x, float* d_recon, long long re
                 float pos_weight, float c_pred, float c_mse, float c_kld, float* partials, float* out, float* total,
                 void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Attention-block operators on sequences (csrc/rotary.hip, diff_attention*.hip, group_norm.hip).  `type` (and lam_type / weight_type):
+ * 0 fp32, 1 bf16, 2 fp16; every sum, statistic and accumulator is 32-bit.  Strides are in elements; the innermost dimension has stride 1.
+ *
+ * is_rotary   x (batch, n, heads, width) -> out (contiguous): the first `part` elements of every head turned in pairs by position *
+ *             freq[p] radians (freq: HOST array of part / 2 doubles; interleaved = 0: pairs (p, p + part / 2), 1: (2 p, 2 p + 1)),
+ *             scaled by `amplitude`; the rest copied.  inverse = 1 turns the other way (the backward pass).  A second tensor (k,
+ *             kv_heads; NULL with 0) is turned in the same launch.  positions: int32 / int64 (positions64) with strides pos_b, pos_n,
+ *             or NULL: position = index in n.  part even, <= width, part / 2 <= 256.                                             */
+int is_rotary(const void* q, long long q_b, long long q_n, long long q_h, void* q_out, int heads,
+              const void* k, long long k_b, long long k_n, long long k_h, void* k_out, int kv_heads,
+              const void* positions, int positions64, long long pos_b, long long pos_n, const double* freq,
+              int batch, int n, int width, int part, int interleaved, int inverse, float amplitude, int type, void* stream);
+
+/* Differential attention: o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v per head, two maps of shared values.
+ *   q (batch, nq, 2 heads, d): head h's maps are heads 2 h and 2 h + 1; k (batch, nk, 2 kv_heads, d) likewise; v (batch, nk, kv_heads, dv);
+ *   heads a multiple of kv_heads; lam (heads) in `type` or fp32; lengths (batch) int32 or NULL: keys at or behind a sample's length do
+ *   not exist.  causal: 0 every key, 1 query i sees keys <= i, 2 the queries are the last nq positions (keys <= i + length - nq).
+ *   A row that sees no key gives 0 and no gradient.  d <= 128 and dv <= 256 (fp32: 64 and 128); -38 beyond.
+ * is_diff_attention_fwd: reads q, k, v, lam, lengths; writes o (batch, nq, heads, dv); lse (batch, kv_heads, 2, nq heads / kv_heads; fp32) and
+ *   o2 (like o: the second map's product) are what the backward needs, both or neither.  splits = is_diff_attention_splits(...) ranges of
+ *   the keys per row (1: none); splits > 1 needs work[is_diff_attention_work_floats(...)] (rows = nq heads / kv_heads in both).
+ * is_diff_attention_bwd: reads those and d_o (contiguous); writes dq, dk, dv_out (contiguous), dlam (lam's type); dots: scratch of lse's
+ *   size.  group and vec are set by the library.  No atomics: bitwise reproducible.                                                  */
+typedef struct {
+  const void *q, *k, *v, *lam;
+  const int* lengths;
+  void *o, *o2;
+  float *lse, *work;
+  const void* d_o;
+  float* dots;
+  void *dq, *dk, *dv_out, *dlam;
+  long long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
+  int batch, nq, nk, heads, kv_heads, d, dv, causal, type, lam_type, splits, group, vec;
+  float scale;
+} IsDiffAttention;
+int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk);
+long long is_diff_attention_work_floats(int batch, int kv_heads, int rows, int dv, int splits);
+int is_diff_attention_fwd(const IsDiffAttention* args, void* stream);
+int is_diff_attention_bwd(const IsDiffAttention* args, void* stream);
+
+/* Group norm with an activation, channels last: x (batch, n, channels), statistics over a sample's rows below its length (lengths: int32 or
+ * NULL: all n) and the channels / groups channels of a group; y = act((x - mean) rstd weight + bias); activation: 0 none, 1 SiLU, 2 GELU
+ * (erf), 3 ReLU.  Rows behind the length give 0 and get no gradient.  weight, bias (channels) of weight_type, both or neither NULL.
+ * is_group_norm_fwd writes y (contiguous) and stats (batch, groups, 2) = mean, rstd (fp32); is_group_norm_bwd reads x, stats, dy (contiguous)
+ * and writes dx (contiguous), dweight, dbias (NULL with weight).  work[is_group_norm_work_floats(...)] floats of scratch for either.   */
+typedef struct {
+  const void *x, *weight, *bias;
+  const int* lengths;
+  void* y;
+  float *stats, *work;
+  const void* dy;
+  void *dx, *dweight, *dbias;
+  long long x_b, x_n;
+  int batch, n, channels, groups, activation, type, weight_type, pad;
+  float eps;
+} IsGroupNorm;
+long long is_group_norm_work_floats(const IsGroupNorm* args, int backward);
+int is_group_norm_fwd(const IsGroupNorm* args, void* stream);
+int is_group_norm_bwd(const IsGroupNorm* args, void* stream);
 
 #ifdef __cplusplus
 }

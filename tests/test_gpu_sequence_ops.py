@@ -1,0 +1,349 @@
+"""Rotary positions, differential attention and group norm against their plain 64-bit forms (oracle.sequence_ref), place by place within the
+bounds that count the kernels' roundings; and as they are used: strided inputs, masks that leave nothing, other streams, captured graphs."""
+import itertools
+
+import pytest
+import torch
+
+from immunostruct_amd import functional as HF
+from immunostruct_amd import nn as HN
+from oracle import sequence_ref as SR
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+NAMES = {torch.float32: "fp32", torch.bfloat16: "bf16", torch.float16: "fp16"}
+each_type = pytest.mark.parametrize("dtype", TYPES, ids=[NAMES[t] for t in TYPES])
+
+
+def _randn(*shape, dtype, seed, mean=0.0, std=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=gen) * std + mean).to(dtype).cuda()
+
+
+def _within(got, want, what):
+    value, bound = want
+    got = got.detach().cpu().double()
+    assert got.shape == value.shape, what
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    off = (got - value).abs()
+    worst = (off / bound.clamp(min=1e-300)).masked_fill(off == 0, 0.0)
+    assert bool((off <= bound).all()), f"{what}: {float(worst.max()):.2f} x the bound at {tuple(int(i) for i in (worst == worst.max()).nonzero()[0])}"
+
+
+# ---- rotary ---------------------------------------------------------------------------------------------------------------
+@each_type
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("b,n,heads,kv,width,dims,start", [
+    (1, 1, 1, 1, 2, 2, 0), (2, 5, 3, 1, 16, 16, 0), (3, 17, 4, 2, 24, 10, 7), (2, 33, 2, 2, 64, 32, 1_000_003), (1, 3, 5, 1, 80, 80, 2 ** 33),
+    (4, 190, 2, 2, 32, 32, 0), (2, 9, 40, 8, 128, 64, 131072)])
+def test_rotary(cuda_device, dtype, layout, b, n, heads, kv, width, dims, start):
+    q, k = _randn(b, n, heads, width, dtype=dtype, seed=1).requires_grad_(True), _randn(b, n, kv, width, dtype=dtype, seed=2).requires_grad_(True)
+    pos = (start + torch.arange(n) * 3 + torch.arange(b)[:, None]).cuda()
+    rope = HN.RotaryEmbedding(dims, layout=layout, scaling=dict(kind="yarn", factor=4.0, original_length=4096) if dims > 8 else None)
+    gq, gk = _randn(b, n, heads, width, dtype=dtype, seed=3), _randn(b, n, kv, width, dtype=dtype, seed=4)
+    out = rope(q, k, pos)
+    grads = torch.autograd.grad(out, (q, k), (gq, gk))
+    for x, o, g, d, name in ((q, out[0], gq, grads[0], "q"), (k, out[1], gk, grads[1], "k")):
+        _within(o, SR.rotary(x, rope.freq, pos, layout, rope.amplitude), name)
+        _within(d, SR.rotary(g, rope.freq, pos, layout, rope.amplitude, inverse=True), "d" + name)
+
+
+def test_rotary_positions_and_strides(cuda_device):
+    """int32 and one-dimensional positions, none at all, a broadcast one; q and k as views of one projection; only one of them needing grad"""
+    b, n, d = 3, 7, 32
+    rope = HN.RotaryEmbedding(d)
+    qkv = _randn(b, n, 6, d, dtype=torch.bfloat16, seed=5)
+    q, k = qkv[:, :, :4], qkv[:, :, 4:]
+    base = rope(q.contiguous(), k.contiguous())
+    for pos in (None, torch.arange(n, device="cuda", dtype=torch.int32), torch.arange(n, device="cuda").expand(b, n),
+                torch.arange(2 * n, device="cuda")[::2] // 2):
+        got = rope(q, k, pos)
+        assert all(torch.equal(x, y) for x, y in zip(got, base))
+    turned = rope(q.transpose(1, 2).contiguous().transpose(1, 2), k.expand(b, n, 2, d))      # head-major memory
+    assert all(torch.equal(x, y) for x, y in zip(turned, base))
+    alone, none = rope(q)
+    assert none is None and torch.equal(alone, base[0])
+    odd = torch.zeros(b, n, 4, d + 1, dtype=torch.bfloat16, device="cuda")[..., 1:]      # rows that are not 16-byte aligned
+    odd.copy_(q)
+    assert torch.equal(rope(odd)[0], base[0])
+    shared = _randn(1, n, 1, d, dtype=torch.float32, seed=6).expand(b, n, 4, d)      # a broadcast input: its gradient is a sum
+    leaf = shared[:1, :, :1].clone().requires_grad_(True)
+    out, _ = rope(leaf.expand(b, n, 4, d))
+    out.sum().backward()
+    one = leaf.detach().clone().requires_grad_(True)
+    rope(one)[0].sum().backward()
+    assert torch.allclose(leaf.grad, 12 * one.grad, rtol=1e-6, atol=1e-6)
+    kk = k.clone().requires_grad_(True)
+    (rope(q, kk)[1].float().sum()).backward()
+    assert kk.grad is not None
+    assert [t.shape for t in rope(q[:0], k[:0])] == [(0, n, 4, d), (0, n, 2, d)]
+
+
+# ---- differential attention ---------------------------------------------------------------------------------------------------
+def _attention_inputs(dtype, b, nq, nk, h, hk, d, dv, lam_dtype=None):
+    lam = _randn(h, dtype=lam_dtype or dtype, seed=14, mean=0.5, std=0.2)
+    return (_randn(b, nq, 2 * h, d, dtype=dtype, seed=11), _randn(b, nk, 2 * hk, d, dtype=dtype, seed=12), _randn(b, nk, hk, dv, dtype=dtype, seed=13), lam)
+
+
+SHAPES = [      # b, nq, nk, heads, kv_heads, d, dv, lengths, causal
+    (1, 1, 1, 1, 1, 1, 1, None, None), (2, 3, 5, 2, 1, 4, 8, [5, 0], None), (1, 33, 31, 1, 1, 8, 16, None, "start"),
+    (3, 70, 70, 4, 2, 16, 32, [70, 33, 1], "start"), (2, 45, 130, 2, 2, 32, 64, [130, 64], "end"), (2, 129, 65, 3, 1, 24, 48, [65, 20], "end"),
+    (2, 190, 190, 1, 1, 32, 64, [190, 171], None), (1, 257, 300, 4, 1, 64, 128, None, "end"), (4, 1, 700, 8, 2, 64, 128, [700, 1, 0, 333], "end"),
+    (1, 40, 513, 2, 1, 40, 72, [512], None), (2, 5, 40, 1, 1, 20, 7, [40, 3], "end")]
+WIDE = [(2, 37, 70, 4, 2, 128, 256, [70, 9], None), (1, 130, 130, 1, 1, 96, 192, None, "start"), (3, 1, 300, 4, 4, 128, 256, [300, 0, 17], "end")]
+
+
+@each_type
+@pytest.mark.parametrize("shape", SHAPES + WIDE, ids=lambda s: "-".join(str(x) for x in s[:7]) + f"-{s[8]}")
+def test_differential_attention(cuda_device, dtype, shape):
+    b, nq, nk, h, hk, d, dv, lengths, causal = shape
+    if dtype == torch.float32 and d > 64:
+        with pytest.raises(NotImplementedError):
+            HF.differential_attention(*_attention_inputs(dtype, b, nq, nk, h, hk, d, dv))
+        return
+    q, k, v, lam = (t.requires_grad_(True) for t in _attention_inputs(dtype, b, nq, nk, h, hk, d, dv))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    do = _randn(b, nq, h, dv, dtype=dtype, seed=15)
+    want = SR.differential_attention(q, k, v, lam, lengths, causal, d ** -0.5, do)
+    with torch.no_grad():
+        _within(HF.differential_attention(q, k, v, lam, lens, causal), want["o"], "o (no gradient)")
+    out = HF.differential_attention(q, k, v, lam, lens, causal)
+    _within(out, want["o"], "o")
+    grads = torch.autograd.grad(out, (q, k, v, lam), do)
+    for g, name in zip(grads, ("dq", "dk", "dv", "dlam")):
+        _within(g, want[name], name)
+    again = torch.autograd.grad(HF.differential_attention(q, k, v, lam, lens, causal), (q, k, v, lam), do)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again)), "not reproducible"
+
+
+def test_attention_garbage_behind_the_lengths(cuda_device):
+    """whatever stands at or behind a sample's length (NaN, infinities) has no effect, and those keys get zero gradients"""
+    for dtype, causal in itertools.product(TYPES, (None, "start", "end")):
+        q, k, v, lam = _attention_inputs(dtype, 3, 50, 90, 2, 1, 32, 64)
+        lens = torch.tensor([90, 41, 0], dtype=torch.int32, device="cuda")
+        do = _randn(3, 50, 2, 64, dtype=dtype, seed=16)
+
+        def run(fill):
+            kk, vv = k.clone(), v.clone()
+            for i, n in enumerate(lens.tolist()):
+                kk[i, n:], vv[i, n:] = fill, fill
+            leaves = [t.clone().requires_grad_(True) for t in (q, kk, vv, lam)]
+            out = HF.differential_attention(*leaves, lens, causal)
+            return (out,) + torch.autograd.grad(out, leaves, do)
+
+        clean = run(0.0)
+        for fill in (float("nan"), float("inf"), torch.finfo(dtype).min):
+            assert all(torch.equal(x, y) for x, y in zip(clean, run(fill)))
+        assert not clean[2][1, 41:].any() and not clean[3][1, 41:].any() and not clean[2][2].any() and not clean[0][2].any()
+
+
+def test_attention_strides_scale_and_types(cuda_device):
+    dtype = torch.bfloat16
+    q, k, v, lam = _attention_inputs(dtype, 2, 70, 70, 4, 2, 32, 64)
+    base = HF.differential_attention(q, k, v, lam)
+    pack = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2)], dim=2)      # one projection's output
+    qs, ks, vs = pack.split([8 * 32, 4 * 32, 2 * 64], dim=2)
+    assert torch.equal(HF.differential_attention(qs.view(2, 70, 8, 32), ks.view(2, 70, 4, 32), vs.view(2, 70, 2, 64), lam), base)
+    head_major = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    assert torch.equal(HF.differential_attention(*head_major, lam), base)
+    odd = []      # rows that are not 16-byte aligned
+    for t in (q, k, v):
+        o = torch.zeros(*t.shape[:3], t.shape[3] + 1, dtype=dtype, device="cuda")[..., 1:]
+        odd.append(o.copy_(t))
+    assert torch.equal(HF.differential_attention(*odd, lam), base)
+    column = [t.transpose(2, 3).contiguous().transpose(2, 3) for t in (q, k, v)]      # an innermost stride that is not 1: copied
+    assert torch.equal(HF.differential_attention(*column, lam), base)
+    want = SR.differential_attention(q, k, v, lam.float(), None, None, 0.3, base)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, lam.float())]
+    out = HF.differential_attention(*leaves, scale=0.3)
+    _within(out, want["o"], "o")
+    for g, name in zip(torch.autograd.grad(out, leaves, base), ("dq", "dk", "dv", "dlam")):
+        _within(g, want[name], name)
+    # a broadcast batch: the gradient is the sum over what it was broadcast to
+    leaf = k[:1].clone().requires_grad_(True)
+    HF.differential_attention(q, leaf.expand(2, -1, -1, -1), v, lam).float().sum().backward()
+    assert leaf.grad.shape == (1, 70, 4, 32)
+    assert HF.differential_attention(q[:, :0], k, v, lam).shape == (2, 0, 4, 64)
+    empty = HF.differential_attention(q, k[:, :0].detach().requires_grad_(True), v[:, :0], lam)
+    assert not empty.any() and empty.requires_grad
+
+
+def test_attention_large_scores_and_offsets(cuda_device):
+    """scores far apart (the running maximum moves at the end), all equal, and of magnitude 1e4"""
+    for dtype in TYPES:
+        q, k, v, lam = _attention_inputs(dtype, 1, 40, 200, 1, 1, 32, 64)
+        k = k * torch.linspace(0.01, 12.0, 200, device="cuda")[:, None, None].to(dtype)
+        want = SR.differential_attention(q, k, v, lam, None, None, 32 ** -0.5)
+        _within(HF.differential_attention(q, k, v, lam), want["o"], "rising scores")
+        want = SR.differential_attention(q, k.flip(1), v, lam, None, None, 32 ** -0.5)
+        _within(HF.differential_attention(q, k.flip(1), v, lam), want["o"], "falling scores")
+        flat = torch.zeros_like(k)
+        want = SR.differential_attention(q, flat, v, lam, None, None, 32 ** -0.5)
+        _within(HF.differential_attention(q, flat, v, lam), want["o"], "equal scores")
+
+
+def test_attention_cache_beyond_32_bit_offsets(cuda_device):
+    """one key head of a cache whose samples lie more than 2^31 elements apart"""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    big = torch.zeros(2, (2 ** 31 + 4096) // 64, 64, dtype=torch.bfloat16, device="cuda")
+    k, v = big[:, -96:, :32].unflatten(2, (2, 16)), big[:, -96:, 32:].unflatten(2, (1, 32))
+    kk, vv = _randn(2, 96, 2, 16, dtype=torch.bfloat16, seed=21), _randn(2, 96, 1, 32, dtype=torch.bfloat16, seed=22)
+    k.copy_(kk), v.copy_(vv)
+    q, lam = _randn(2, 3, 2, 16, dtype=torch.bfloat16, seed=23), _randn(1, dtype=torch.bfloat16, seed=24)
+    assert torch.equal(HF.differential_attention(q, k, v, lam), HF.differential_attention(q, kk, vv, lam))
+
+
+# ---- group norm -------------------------------------------------------------------------------------------------------------
+@each_type
+@pytest.mark.parametrize("activation", [None, "silu", "gelu", "relu"])
+@pytest.mark.parametrize("b,n,c,groups,lengths", [
+    (1, 1, 1, 1, None), (3, 1, 64, 8, None), (300, 1, 128, 4, None), (5, 1, 60, 4, None), (2, 1, 4096, 2, None), (2, 11, 64, 4, [11, 5]), (3, 190, 64, 8, [190, 77, 0]),
+    (2, 33, 6, 3, None), (2, 40, 100, 5, [40, 1]), (1, 2100, 96, 3, None), (2, 3000, 32, 32, [3000, 2999]), (2, 1300, 40, 1, [7, 1300]),
+    (3, 2, 2560, 8, [2, 1, 0])])
+def test_group_norm(cuda_device, dtype, activation, b, n, c, groups, lengths):
+    x = _randn(b, n, c, dtype=dtype, seed=31, mean=0.7, std=1.5).requires_grad_(True)
+    w, o = _randn(c, dtype=dtype, seed=32, mean=1.0, std=0.3).requires_grad_(True), _randn(c, dtype=dtype, seed=33, std=0.3).requires_grad_(True)
+    dy = _randn(b, n, c, dtype=dtype, seed=34)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = SR.group_norm(x, groups, w, o, 1e-5, activation, lengths, dy)
+    y = HF.group_norm(x, groups, w, o, activation=activation, lengths=lens)
+    _within(y, want["y"], "y")
+    grads = torch.autograd.grad(y, (x, w, o), dy)
+    for g, name in zip(grads, ("dx", "dweight", "dbias")):
+        _within(g, want[name], name)
+    again = torch.autograd.grad(HF.group_norm(x, groups, w, o, activation=activation, lengths=lens), (x, w, o), dy)
+    assert all(torch.equal(p, r) for p, r in zip(grads, again)), "not reproducible"
+
+
+def test_group_norm_forms(cuda_device):
+    """without parameters, fp32 parameters on 16-bit rows, strided rows, images, single rows, garbage behind the lengths, a large mean"""
+    x = _randn(2, 30, 64, dtype=torch.bfloat16, seed=41)
+    _within(HF.group_norm(x, 4), SR.group_norm(x, 4, None, None, 1e-5, None, None)["y"], "plain")
+    w, o = _randn(64, dtype=torch.float32, seed=42).requires_grad_(True), _randn(64, dtype=torch.float32, seed=43).requires_grad_(True)
+    leaf = x.clone().requires_grad_(True)
+    y = HF.group_norm(leaf, 4, w, o, activation="silu")
+    dy = _randn(2, 30, 64, dtype=torch.bfloat16, seed=44)
+    want = SR.group_norm(x, 4, w, o, 1e-5, "silu", None, dy)
+    _within(y, want["y"], "y")
+    for g, name in zip(torch.autograd.grad(y, (leaf, w, o), dy), ("dx", "dweight", "dbias")):
+        _within(g, want[name], name)
+    wide = torch.zeros(2, 30, 100, dtype=torch.bfloat16, device="cuda")
+    for at in (0, 8, 3):
+        wide[..., at:at + 64] = x
+        assert torch.equal(HF.group_norm(wide[..., at:at + 64], 4, w, o, activation="silu"), y)
+    assert torch.equal(HF.group_norm(x.transpose(1, 2).contiguous().transpose(1, 2), 4, w, o, activation="silu"), y)
+    assert torch.equal(HF.group_norm(x.view(2, 5, 6, 64), 4, w, o, activation="silu").view(2, 30, 64), y)
+    rows = HF.group_norm(x.view(60, 64), 4, w, o)
+    _within(rows.view(60, 1, 64), SR.group_norm(x.view(60, 1, 64), 4, w, o, 1e-5, None, None)["y"], "rows")
+    lens = torch.tensor([30, 12], dtype=torch.int32, device="cuda")
+    dirty = x.clone()
+    dirty[1, 12:] = float("nan")
+    clean = HF.group_norm(x, 4, w, o, lengths=lens)
+    assert torch.equal(HF.group_norm(dirty, 4, w, o, lengths=lens), clean) and not clean[1, 12:].any()
+    leaf = dirty.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(HF.group_norm(leaf, 4, w, o, lengths=lens), leaf, torch.where(dirty.isnan(), dirty, dy))
+    assert torch.isfinite(dx).all() and not dx[1, 12:].any()
+    far = _randn(2, 300, 32, dtype=torch.float32, seed=45, mean=1000.0)
+    _within(HF.group_norm(far, 2), SR.group_norm(far, 2, None, None, 1e-5, None, None)["y"], "large mean")
+    assert HF.group_norm(x[:0], 4, w, o).shape == (0, 30, 64) and HF.group_norm(x[:, :0], 4).shape == (2, 0, 64)
+
+
+# ---- as a program uses them ---------------------------------------------------------------------------------------------------
+def _block(q, k, v, lam, w, o, rope, lens):
+    q, k = rope(q, k)
+    y = HF.differential_attention(q, k, v, lam, lens, "start")
+    return HF.group_norm(y.flatten(2), y.shape[2], w, o, activation="silu", lengths=lens)
+
+
+def _block_inputs(dtype=torch.bfloat16):
+    q, k, v, lam = _attention_inputs(dtype, 3, 83, 83, 4, 2, 32, 64)
+    leaves = [q, k, v, lam, _randn(256, dtype=dtype, seed=51, mean=1.0, std=0.1), _randn(256, dtype=dtype, seed=52, std=0.1)]
+    return [t.requires_grad_(True) for t in leaves], torch.tensor([83, 40, 0], dtype=torch.int32, device="cuda")
+
+
+def test_block_gradients_against_differences(cuda_device):
+    """the three operators in a row: the directional derivative of a weighted sum, in fp32, against central differences in 64 bits of the
+    plain forms (a step of 1e-4: a truncation error of about 1e-8 of the third derivative, far below the 1e-3 asked)"""
+    leaves, lens = _block_inputs(torch.float32)
+    rope = HN.RotaryEmbedding(32)
+    dy = _randn(3, 83, 256, dtype=torch.float32, seed=53)
+    grads = torch.autograd.grad(_block(*leaves, rope, lens), leaves, dy)
+    dirs = [torch.randn(t.shape, generator=torch.Generator().manual_seed(60 + i)).double() for i, t in enumerate(leaves)]
+
+    def plain(step):
+        q, k, v, lam, w, o = (t.detach().cpu().double() + step * d for t, d in zip(leaves, dirs))
+        q = SR.rotary(q, rope.freq, None, "half", 1.0)[0]
+        k = SR.rotary(k, rope.freq, None, "half", 1.0)[0]
+        y = SR.differential_attention(q, k, v, lam, lens.tolist(), "start", 32 ** -0.5)["o"][0].flatten(2)
+        return (SR.group_norm(y, 4, w, o, 1e-5, "silu", lens.tolist())["y"][0] * dy.cpu().double()).sum()
+
+    want = float((plain(1e-4) - plain(-1e-4)) / 2e-4)
+    got = float(sum((g.cpu().double() * d).sum() for g, d in zip(grads, dirs)))
+    assert abs(got - want) <= 1e-3 * abs(want)
+
+
+def test_block_on_another_stream(cuda_device):
+    leaves, lens = _block_inputs()
+    rope = HN.RotaryEmbedding(32)
+    dy = _randn(3, 83, 256, dtype=torch.bfloat16, seed=53)
+    base = _block(*leaves, rope, lens)
+    base = (base,) + torch.autograd.grad(base, leaves, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = _block(*leaves, rope, lens)
+        got = (out,) + torch.autograd.grad(out, leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(base, got))
+
+
+def test_block_in_captured_graphs(cuda_device):
+    """forward and backward captured twice (two graphs, their own workspaces), replayed in turn with new inputs and eager work between: every
+    replay equals the eager result"""
+    rope = HN.RotaryEmbedding(32)
+    leaves, lens = _block_inputs()
+    dy = _randn(3, 83, 256, dtype=torch.bfloat16, seed=53)
+    cache_q, cache_k, cache_v, lam = _attention_inputs(torch.bfloat16, 2, 1, 600, 4, 2, 32, 64)      # split keys: a workspace
+    cache_len = torch.tensor([600, 77], dtype=torch.int32, device="cuda")
+
+    def step():
+        out = _block(*leaves, rope, lens)
+        grads = torch.autograd.grad(out, leaves, dy)
+        with torch.no_grad():
+            token = HF.differential_attention(cache_q, cache_k, cache_v, lam, cache_len, "end")
+        return (out, *grads, token)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held = step()
+        graphs.append((g, held))
+    for turn in range(3):
+        with torch.no_grad():
+            for t in leaves + [cache_q, cache_k]:
+                t.mul_(0.9).add_(0.01 * (turn + 1))
+            cache_len.fill_(100 * turn + 1)
+            lens.copy_(torch.tensor([83 - turn, 40 + turn, turn], dtype=torch.int32))
+        want = [t.clone() for t in step()]
+        for g, held in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(want, held))
+
+
+def test_token_equals_the_last_row_of_the_prompt(cuda_device):
+    """serving: the new token over the cache against the same position of the whole causal pass (another kernel and summation order)"""
+    for dtype in TYPES:
+        q, k, v, lam = _attention_inputs(dtype, 2, 300, 300, 4, 2, 64, 128)
+        whole = SR.differential_attention(q, k, v, lam, None, "start", 64 ** -0.5)["o"]
+        token = HF.differential_attention(q[:, -1:], k, v, lam, None, "end")
+        _within(token, (whole[0][:, -1:], whole[1][:, -1:]), "token")
+        _within(HF.differential_attention(q, k, v, lam, None, "start"), whole, "prompt")
