@@ -235,12 +235,14 @@ def last_contiguous(t):
 
 
 def same_device(first, *tensors):
-    """the device every given tensor lives on; raises when one is elsewhere"""
-    require_device(first, *tensors)
+    """raises unless all given tensors live on one ROCm device"""
+    index = first.get_device()      # (-1: host memory)
+    if index < 0:
+        require_device(first)
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            require_device(t)
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
-    return first.device
 
 
 def check(code, what):

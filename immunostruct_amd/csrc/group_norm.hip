@@ -2,6 +2,17 @@
 //
 //   xhat = (x - mean) rstd,  z = xhat w + b,  y = act(z)
 //   dz = dy act'(z),  dw = sum dz xhat,  db = sum dz,  t = dz w,  dx = rstd (t - mean(t) - xhat mean(t xhat))
+//
+// Bound by bytes: x in and y out; x, dy in and dx out.  Forms, chosen by size (plan()):
+//   rows  n = 1, a group is a power of two of 16-byte chunks, at most 64: a group lives in neighbouring lanes, every sum is a few lane moves,
+//         a workgroup walks many samples and keeps its channels' dw / db sums in registers.
+//   slab  a workgroup holds all rows of one sample's slice of whole groups in registers (up to 16 chunks a thread): one read, exact two-step
+//         variance, one write.  Slices are as narrow as 64-byte row segments allow, so that small batches still fill the chip.
+//   long  a sample does not fit: row blocks leave (mean, M2) / (sum t, sum t xhat) of every group, a second launch joins a sample's blocks and
+//         writes.  Block sums are taken about each thread's own first value, so a large mean costs no precision.
+//   any   groups of more than 256 chunks: one workgroup per (sample, group), re-reading.
+// Chunks are 16 bytes where pointers, strides and the group width allow, single elements otherwise (a chunk never straddles two groups).
+// dw and db: one record [2][channels] per workgroup (rows), sample (slab, any) or row block (long), summed in a fixed order by a last launch.
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
 
@@ -9,168 +20,812 @@ namespace is {
 namespace gn {
 
 typedef IsGroupNorm Args;
+enum Form { ROWS, SLAB, LONG, ANY };
+struct Plan {
+  Form form;
+  int ve;              // elements of a chunk
+  int slice, slices;   // channels of a workgroup (whole groups), their number
+  int per_thread;      // slab: chunks a thread holds
+  int blocks, rows;    // long: row blocks of a sample, rows of one; rows: workgroups
+  int records;         // of dw / db
+};
 
 __device__ __forceinline__ int length_of(const Args& a, int b) {
   const int n = a.lengths != nullptr ? a.lengths[b] : a.n;
   return n < 0 ? 0 : (n > a.n ? a.n : n);
 }
-__device__ __forceinline__ float param(const void* p, int type, int c, float other) {
+template <typename T>
+__device__ __forceinline__ float param(const Args& a, const void* p, int c, float other) {
   if (p == nullptr) return other;
-  if (type == TYPE_F32) return reinterpret_cast<const float*>(p)[c];
-  if (type == TYPE_BF16) return (float)reinterpret_cast<const __bf16*>(p)[c];
-  return (float)reinterpret_cast<const _Float16*>(p)[c];
-}
-__device__ __forceinline__ void put(void* p, int type, int c, float v) {
-  if (type == TYPE_F32) reinterpret_cast<float*>(p)[c] = v;
-  else if (type == TYPE_BF16) reinterpret_cast<__bf16*>(p)[c] = (__bf16)v;
-  else reinterpret_cast<_Float16*>(p)[c] = (_Float16)v;
+  return a.weight_type == TYPE_F32 ? reinterpret_cast<const float*>(p)[c] : (float)reinterpret_cast<const T*>(p)[c];
 }
 __device__ __forceinline__ float act(float z, int kind) {
-  if (kind == 1) return z / (1.0f + __expf(-z));
+  if (kind == 1) return z * rcp_f(1.0f + __expf(-z));
   if (kind == 2) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
   if (kind == 3) return z > 0.0f ? z : (z != z ? z : 0.0f);
   return z;
 }
 __device__ __forceinline__ float act_slope(float z, int kind) {
   if (kind == 1) {
-    const float s = 1.0f / (1.0f + __expf(-z));
+    const float s = rcp_f(1.0f + __expf(-z));
     return s * (1.0f + z * (1.0f - s));
   }
   if (kind == 2) return 0.5f * (1.0f + erff(z * 0.70710678118654752440f)) + z * 0.39894228040143267794f * __expf(-0.5f * z * z);
   if (kind == 3) return z > 0.0f ? 1.0f : 0.0f;
   return 1.0f;
 }
-// sum over the 256 threads, in every thread
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
+
+// a chunk of VE elements (1: a single element in word 0)
+template <typename T, int VE>
+struct Chunk {
+  float x[VE];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VE == 1) x[0] = (float)*p;
+    else Vec<T>::unpack(*reinterpret_cast<const u32x4_t*>(p), x);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (VE == 1) *p = (T)x[0];
+    else *reinterpret_cast<u32x4_t*>(p) = Vec<T>::pack(x);
+  }
+};
+// the raw bits, for chunks that wait in registers
+template <typename T, int VE> struct Held {
+  typedef typename std::conditional<VE == 1, T, u32x4_t>::type Raw;
+  Raw v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void zero() { v = Raw{}; }
+  __device__ __forceinline__ void get(float (&x)[VE]) const {
+    if constexpr (VE == 1) x[0] = (float)v;
+    else Vec<T>::unpack(v, x);
+  }
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
   v = sum_over_r(v);
-  v += other_half(v);
+  return v + other_half(v);
+}
+__device__ __forceinline__ float block_sum(float v, float* scratch) {      // 256 threads; the sum in every thread
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
   return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
 }
 
-// one workgroup per (sample, group), any shape
+// Threads of a workgroup over a slice: thread = (row lane rl, column chunk col); cols chunks side by side, rl < lanes.
+struct Place {
+  int cols, lanes, col, rl;
+  bool on;
+  __device__ __forceinline__ Place(int slice, int ve) {
+    cols = slice / ve;
+    lanes = 256 / cols;
+    rl = threadIdx.x / cols;
+    col = threadIdx.x - rl * cols;
+    on = rl < lanes;
+  }
+};
+// sum of v over a slice's group (the threads of cpg neighbouring columns and every row lane), in each of its threads.  256 floats of LDS each.
+__device__ __forceinline__ float group_sum(float v, const Place& p, int cpg, float* all, float* out) {
+  const int groups = p.cols / cpg, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, each = p.lanes * cpg;
+  __syncthreads();
+  all[threadIdx.x] = p.on ? v : 0.0f;
+  __syncthreads();
+  for (int g = wave; g < groups; g += 4) {
+    float s = 0.0f;
+    for (int i = lane; i < each; i += 64) {
+      const int r = i / cpg;
+      s += all[r * p.cols + g * cpg + i - r * cpg];
+    }
+    s = wave_sum(s);
+    if (lane == 0) out[g] = s;
+  }
+  __syncthreads();
+  return out[p.on ? p.col / cpg : 0];
+}
+// the channels' sums of (dz xhat, dz) over the row lanes -> record [2][channels]
+template <int VE>
+__device__ __forceinline__ void channel_record(const float (&sw)[VE], const float (&sb)[VE], const Place& p, float* lds, float* record, int channels, int c0) {
+  const int width = p.cols * VE;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    __syncthreads();
+    if (p.on) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) lds[p.rl * width + p.col * VE + e] = m == 0 ? sw[e] : sb[e];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += 256) {
+      float s = 0.0f;
+      for (int r = 0; r < p.lanes; ++r) s += lds[r * width + c];
+      record[(long long)m * channels + c0 + c] = s;
+    }
+  }
+}
+
+// ---- rows: n = 1 ---------------------------------------------------------------------------------------------------------------------
+template <typename T, bool BACK>
+__global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, const int cols) {
+  constexpr int VE = Vec<T>::N;
+  __shared__ float lds[BACK ? 256 * VE : 1];
+  const int lanes = 256 / cols, rl = threadIdx.x / cols, cl = threadIdx.x - rl * cols;
+  const int c = (blockIdx.y * cols + cl) * VE, cg = cpg * VE;
+  const bool on = rl < lanes && c < a.channels;
+  const int cc = on ? c : 0, g = cc / cg;
+  float w[VE], o[VE], sw[VE], sb[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    w[e] = param<T>(a, a.weight, cc + e, 1.0f);
+    o[e] = param<T>(a, a.bias, cc + e, 0.0f);
+    sw[e] = sb[e] = 0.0f;
+  }
+  const float inv = 1.0f / (float)cg;
+  auto sum = [&](float v) {      // over the group's cpg neighbouring lanes (cpg divides 64 and the lanes of a group never straddle a wave)
+    for (int m = 1; m < cpg; m *= 2) v += __shfl_xor(v, m);
+    return v;
+  };
+  const int step = gridDim.x * lanes;
+  for (int b0 = blockIdx.x * lanes; b0 < a.batch; b0 += step) {      // uniform: every lane takes part in the lane moves
+    const int b = b0 + rl;
+    const bool live = on && b < a.batch && length_of(a, b < a.batch ? b : 0) > 0;
+    Chunk<T, VE> x, d;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x.x[e] = d.x[e] = 0.0f;
+    if (live) x.load(reinterpret_cast<const T*>(a.x) + b * a.x_b + c);
+    if constexpr (BACK) {
+      if (live) d.load(reinterpret_cast<const T*>(a.dy) + (long long)b * a.channels + c);
+    }
+    if constexpr (!BACK) {
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s += x.x[e];
+      const float mean = sum(s) * inv;
+      s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s += (x.x[e] - mean) * (x.x[e] - mean);
+      const float rstd = 1.0f / sqrtf(sum(s) * inv + a.eps);
+      if (on && b < a.batch) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x.x[e] = live ? act((x.x[e] - mean) * rstd * w[e] + o[e], a.activation) : 0.0f;
+        x.store(reinterpret_cast<T*>(a.y) + (long long)b * a.channels + c);
+        if (cl % cpg == 0) {
+          float* st = a.stats + 2 * ((long long)b * a.groups + g);
+          st[0] = mean;
+          st[1] = rstd;
+        }
+      }
+    } else {
+      float mean = 0.0f, rstd = 0.0f;
+      if (live) {
+        const float* st = a.stats + 2 * ((long long)b * a.groups + g);
+        mean = st[0];
+        rstd = st[1];
+      }
+      float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float hat = (x.x[e] - mean) * rstd;
+        const float dz = live ? d.x[e] * act_slope(hat * w[e] + o[e], a.activation) : 0.0f;
+        sw[e] += dz * hat;
+        sb[e] += dz;
+        x.x[e] = hat;
+        d.x[e] = dz * w[e];
+        t1 += d.x[e];
+        t2 += d.x[e] * hat;
+      }
+      t1 = sum(t1) * inv;
+      t2 = sum(t2) * inv;
+      if (on && b < a.batch) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) d.x[e] = live ? rstd * (d.x[e] - t1 - x.x[e] * t2) : 0.0f;
+        d.store(reinterpret_cast<T*>(a.dx) + (long long)b * a.channels + c);
+      }
+    }
+  }
+  if constexpr (BACK) {
+    if (a.weight != nullptr) {
+      const int width = cols * VE, c0 = blockIdx.y * width;
+      float* record = a.work + (long long)blockIdx.x * 2 * a.channels;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        __syncthreads();
+        if (rl < lanes) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) lds[rl * width + cl * VE + e] = m == 0 ? sw[e] : sb[e];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < width && c0 + i < a.channels; i += 256) {
+          float s = 0.0f;
+          for (int r = 0; r < lanes; ++r) s += lds[r * width + i];
+          record[(long long)m * a.channels + c0 + i] = s;
+        }
+      }
+    }
+  }
+}
+
+// ---- slab: a sample's slice in registers ------------------------------------------------------------------------------------------------
+template <typename T, int VE, int K>
+__global__ __launch_bounds__(256) void slab_fwd_kernel(const Args a, const int slice) {
+  __shared__ float all[256], out[256];
+  const int slices = a.channels / slice, b = blockIdx.x / slices, c0 = (blockIdx.x - b * slices) * slice, cg = a.channels / a.groups;
+  const int len = length_of(a, b), cpg = cg / VE;
+  const Place p(slice, VE);
+  const int c = c0 + p.col * VE;
+  const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + c;
+  T* y = reinterpret_cast<T*>(a.y) + (long long)b * a.n * a.channels + c;
+  Held<T, VE> h[K];
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int row = p.rl + k * p.lanes;
+    h[k].zero();
+    if (p.on && row < len) h[k].load(x + row * a.x_n);
+  }
+  float w[VE], o[VE], v[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    w[e] = p.on ? param<T>(a, a.weight, c + e, 1.0f) : 0.0f;
+    o[e] = p.on ? param<T>(a, a.bias, c + e, 0.0f) : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    h[k].get(v);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) s += v[e];
+  }
+  const float inv = 1.0f / ((float)(len > 0 ? len : 1) * (float)cg);
+  const float mean = group_sum(s, p, cpg, all, out) * inv;
+  s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (p.rl + k * p.lanes < len) {
+      h[k].get(v);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s += (v[e] - mean) * (v[e] - mean);
+    }
+  const float rstd = 1.0f / sqrtf(group_sum(s, p, cpg, all, out) * inv + a.eps);
+  if (!p.on) return;
+  if (p.rl == 0 && p.col % cpg == 0) {
+    float* st = a.stats + 2 * ((long long)b * a.groups + c / cg);
+    st[0] = mean;
+    st[1] = rstd;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int row = p.rl + k * p.lanes;
+    if (row < a.n) {
+      Chunk<T, VE> r;
+      h[k].get(r.x);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) r.x[e] = row < len ? act((r.x[e] - mean) * rstd * w[e] + o[e], a.activation) : 0.0f;
+      r.store(y + (long long)row * a.channels);
+    }
+  }
+}
+
+template <typename T, int VE, int K>
+__global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int slice) {
+  __shared__ float all[256], out[256], lds[256 * VE];
+  const int slices = a.channels / slice, b = blockIdx.x / slices, c0 = (blockIdx.x - b * slices) * slice, cg = a.channels / a.groups;
+  const int len = length_of(a, b), cpg = cg / VE;
+  const Place p(slice, VE);
+  const int c = c0 + p.col * VE;
+  const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + c;
+  const long long at = (long long)b * a.n * a.channels + c;
+  const T* dy = reinterpret_cast<const T*>(a.dy) + at;
+  T* dx = reinterpret_cast<T*>(a.dx) + at;
+  Held<T, VE> h[K], d[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int row = p.rl + k * p.lanes;
+    h[k].zero();
+    d[k].zero();
+    if (p.on && row < len) {
+      h[k].load(x + row * a.x_n);
+      d[k].load(dy + (long long)row * a.channels);
+    }
+  }
+  float w[VE], o[VE], sw[VE], sb[VE], v[VE], u[VE];
+  float mean = 0.0f, rstd = 0.0f;
+  if (p.on) {
+    const float* st = a.stats + 2 * ((long long)b * a.groups + c / cg);
+    mean = st[0];
+    rstd = st[1];
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    w[e] = p.on ? param<T>(a, a.weight, c + e, 1.0f) : 0.0f;
+    o[e] = p.on ? param<T>(a, a.bias, c + e, 0.0f) : 0.0f;
+    sw[e] = sb[e] = 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (p.rl + k * p.lanes < len) {
+      h[k].get(v);
+      d[k].get(u);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float hat = (v[e] - mean) * rstd, dz = u[e] * act_slope(hat * w[e] + o[e], a.activation);
+        sw[e] += dz * hat;
+        sb[e] += dz;
+      }
+    }
+  float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    t1 += sb[e] * w[e];
+    t2 += sw[e] * w[e];
+  }
+  const float inv = 1.0f / ((float)(len > 0 ? len : 1) * (float)cg);
+  t1 = group_sum(t1, p, cpg, all, out) * inv;
+  t2 = group_sum(t2, p, cpg, all, out) * inv;
+  if (p.on) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int row = p.rl + k * p.lanes;
+      if (row < a.n) {
+        Chunk<T, VE> r;
+        h[k].get(v);
+        d[k].get(u);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float hat = (v[e] - mean) * rstd, dz = u[e] * act_slope(hat * w[e] + o[e], a.activation);
+          r.x[e] = row < len ? rstd * (dz * w[e] - t1 - hat * t2) : 0.0f;
+        }
+        r.store(dx + (long long)row * a.channels);
+      }
+    }
+  }
+  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + (long long)b * 2 * a.channels, a.channels, c0);
+}
+
+// ---- long: row blocks ---------------------------------------------------------------------------------------------------------------------
+// workspace: pairs[sample][block][group][2], behind it the dw / db records.  Workgroup = (sample, block, slice)
+struct Block {
+  int b, block, c0, first, last, len;
+  __device__ __forceinline__ Block(const Args& a, const Plan& p) {
+    const int slices = p.slices;
+    int id = blockIdx.x;
+    c0 = id % slices * p.slice;
+    id /= slices;
+    block = id % p.blocks;
+    b = id / p.blocks;
+    len = length_of(a, b);
+    first = block * p.rows;
+    last = min(first + p.rows, len);
+  }
+};
+
+template <typename T, int VE>
+__global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan plan) {
+  __shared__ float all[256], out[256];
+  const Block k(a, plan);
+  const int cg = a.channels / a.groups, cpg = cg / VE;
+  const Place p(plan.slice, VE);
+  const int c = k.c0 + p.col * VE;
+  float s[VE], q[VE], base[VE];
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) s[e] = q[e] = base[e] = 0.0f;
+  if (p.on) {
+    const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
+    Chunk<T, VE> v;
+    int row = k.first + p.rl;
+    if (row < k.last) {
+      v.load(x + row * a.x_n);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) base[e] = v.x[e];
+      ++count;
+    }
+    for (row += p.lanes; row < k.last; row += p.lanes) {
+      v.load(x + row * a.x_n);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float t = v.x[e] - base[e];
+        s[e] += t;
+        q[e] += t * t;
+      }
+      ++count;
+    }
+  }
+  const float rows = (float)(k.last > k.first ? k.last - k.first : 0), total = rows * (float)cg;
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) sum += (float)count * base[e] + s[e];
+  const float mean = group_sum(sum, p, cpg, all, out) / (total > 0.0f ? total : 1.0f);
+  float m2 = 0.0f;
+  if (count > 0) {
+    const float n = (float)count;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float off = s[e] / n, far = base[e] + off - mean;      // this thread's channel mean about its base, and about the block's mean
+      m2 += (q[e] - s[e] * off) + n * far * far;
+    }
+  }
+  m2 = group_sum(m2, p, cpg, all, out);
+  if (p.on && p.rl == 0 && p.col % cpg == 0) {
+    float* at = a.work + 2 * (((long long)k.b * plan.blocks + k.block) * a.groups + c / cg);
+    at[0] = mean;
+    at[1] = m2;
+  }
+}
+
+// the two sums over a sample's blocks of pairs[..][group][2], for the slice's groups; `weigh` turns a block's pair into its two summands
+template <typename F>
+__device__ __forceinline__ void join_blocks(const Args& a, const Plan& plan, const Block& k, int cg, float (*out)[256], F weigh) {
+  // out[.][i] for the slice's group i: a wave per group
+  const int groups = plan.slice / cg, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int i = wave; i < groups; i += 4) {
+    float s0 = 0.0f, s1 = 0.0f;
+    for (int n = lane; n < plan.blocks; n += 64) {
+      const float* at = a.work + 2 * (((long long)k.b * plan.blocks + n) * a.groups + k.c0 / cg + i);
+      const int r0 = n * plan.rows, rows = min(r0 + plan.rows, k.len) - r0;
+      if (rows > 0) weigh(at[0], at[1], (float)rows, i, s0, s1);
+    }
+    s0 = wave_sum(s0);
+    s1 = wave_sum(s1);
+    if (lane == 0) {
+      out[0][i] = s0;
+      out[1][i] = s1;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int VE>
+__global__ __launch_bounds__(256) void long_apply_kernel(const Args a, const Plan plan) {
+  __shared__ float join[2][2][256];
+  const Block k(a, plan);
+  const int cg = a.channels / a.groups, cpg = cg / VE;
+  const float total = (float)(k.len > 0 ? k.len : 1);
+  // mean of the sample, then M2 about it
+  join_blocks(a, plan, k, cg, join[0], [&](float mean, float, float rows, int, float& s0, float&) { s0 += mean * (rows / total); });
+  join_blocks(a, plan, k, cg, join[1], [&](float mean, float m2, float rows, int i, float& s0, float&) {
+    const float off = mean - join[0][0][i];
+    s0 += m2 + rows * (float)cg * off * off;
+  });
+  const Place p(plan.slice, VE);
+  if (!p.on) return;
+  const int c = k.c0 + p.col * VE;
+  const float mean = join[0][0][p.col / cpg], rstd = 1.0f / sqrtf(join[1][0][p.col / cpg] / (total * (float)cg) + a.eps);
+  if (k.block == 0 && p.rl == 0 && p.col % cpg == 0) {
+    float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
+    st[0] = mean;
+    st[1] = rstd;
+  }
+  float w[VE], o[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    w[e] = param<T>(a, a.weight, c + e, 1.0f);
+    o[e] = param<T>(a, a.bias, c + e, 0.0f);
+  }
+  const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
+  T* y = reinterpret_cast<T*>(a.y) + (long long)k.b * a.n * a.channels + c;
+  const int end = min(k.first + plan.rows, a.n);
+  for (int row = k.first + p.rl; row < end; row += p.lanes) {
+    Chunk<T, VE> v;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v.x[e] = 0.0f;
+    if (row < k.len) {
+      v.load(x + row * a.x_n);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v.x[e] = act((v.x[e] - mean) * rstd * w[e] + o[e], a.activation);
+    }
+    v.store(y + (long long)row * a.channels);
+  }
+}
+
+template <typename T, int VE>
+__global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan plan) {
+  __shared__ float all[256], out[256], lds[256 * VE];
+  const Block k(a, plan);
+  const int cg = a.channels / a.groups, cpg = cg / VE;
+  const Place p(plan.slice, VE);
+  const int c = k.c0 + p.col * VE;
+  float w[VE], o[VE], sw[VE], sb[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    w[e] = p.on ? param<T>(a, a.weight, c + e, 1.0f) : 0.0f;
+    o[e] = p.on ? param<T>(a, a.bias, c + e, 0.0f) : 0.0f;
+    sw[e] = sb[e] = 0.0f;
+  }
+  if (p.on) {
+    const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
+    const float mean = st[0], rstd = st[1];
+    const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
+    const T* dy = reinterpret_cast<const T*>(a.dy) + (long long)k.b * a.n * a.channels + c;
+    for (int row = k.first + p.rl; row < k.last; row += p.lanes) {
+      Chunk<T, VE> v, d;
+      v.load(x + row * a.x_n);
+      d.load(dy + (long long)row * a.channels);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float hat = (v.x[e] - mean) * rstd, dz = d.x[e] * act_slope(hat * w[e] + o[e], a.activation);
+        sw[e] += dz * hat;
+        sb[e] += dz;
+      }
+    }
+  }
+  float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    t1 += sb[e] * w[e];
+    t2 += sw[e] * w[e];
+  }
+  t1 = group_sum(t1, p, cpg, all, out);
+  t2 = group_sum(t2, p, cpg, all, out);
+  const long long pairs = 2LL * a.batch * plan.blocks * a.groups, index = (long long)k.b * plan.blocks + k.block;
+  if (p.on && p.rl == 0 && p.col % cpg == 0) {
+    float* at = a.work + 2 * (index * a.groups + c / cg);
+    at[0] = t1;
+    at[1] = t2;
+  }
+  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0);
+}
+
+template <typename T, int VE>
+__global__ __launch_bounds__(256) void long_dx_kernel(const Args a, const Plan plan) {
+  __shared__ float join[2][256];
+  const Block k(a, plan);
+  const int cg = a.channels / a.groups, cpg = cg / VE;
+  join_blocks(a, plan, k, cg, join, [](float t1, float t2, float, int, float& s0, float& s1) {
+    s0 += t1;
+    s1 += t2;
+  });
+  const Place p(plan.slice, VE);
+  if (!p.on) return;
+  const int c = k.c0 + p.col * VE;
+  const float inv = 1.0f / ((float)(k.len > 0 ? k.len : 1) * (float)cg), t1 = join[0][p.col / cpg] * inv, t2 = join[1][p.col / cpg] * inv;
+  const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
+  const float mean = st[0], rstd = st[1];
+  float w[VE], o[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    w[e] = param<T>(a, a.weight, c + e, 1.0f);
+    o[e] = param<T>(a, a.bias, c + e, 0.0f);
+  }
+  const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
+  const long long at = (long long)k.b * a.n * a.channels + c;
+  const T* dy = reinterpret_cast<const T*>(a.dy) + at;
+  T* dx = reinterpret_cast<T*>(a.dx) + at;
+  const int end = min(k.first + plan.rows, a.n);
+  for (int row = k.first + p.rl; row < end; row += p.lanes) {
+    Chunk<T, VE> v, d;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) d.x[e] = 0.0f;
+    if (row < k.len) {
+      v.load(x + row * a.x_n);
+      d.load(dy + (long long)row * a.channels);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float hat = (v.x[e] - mean) * rstd, dz = d.x[e] * act_slope(hat * w[e] + o[e], a.activation);
+        d.x[e] = rstd * (dz * w[e] - t1 - hat * t2);
+      }
+    }
+    d.store(dx + (long long)row * a.channels);
+  }
+}
+
+// ---- any: one workgroup per (sample, group), re-reading -----------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void fwd_any_kernel(const Args a) {
+__global__ __launch_bounds__(256) void any_fwd_kernel(const Args a) {
   __shared__ float scratch[4];
   const int b = blockIdx.x / a.groups, g = blockIdx.x % a.groups, cg = a.channels / a.groups, len = length_of(a, b);
   const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + g * cg;
   T* y = reinterpret_cast<T*>(a.y) + ((long long)b * a.n) * a.channels + g * cg;
-  const long long count = (long long)len * cg, all = (long long)a.n * cg;
+  const float count = (float)(len > 0 ? len : 1) * (float)cg;
   float s = 0.0f;
-  for (long long i = threadIdx.x; i < count; i += 256) s += (float)x[i / cg * a.x_n + i % cg];
-  const float mean = block_sum(s, scratch) / (float)(count > 0 ? count : 1);
+  for (int row = 0; row < len; ++row)
+    for (int c = threadIdx.x; c < cg; c += 256) s += (float)x[row * a.x_n + c];
+  const float mean = block_sum(s, scratch) / count;
   s = 0.0f;
-  for (long long i = threadIdx.x; i < count; i += 256) {
-    const float d = (float)x[i / cg * a.x_n + i % cg] - mean;
-    s += d * d;
-  }
-  const float rstd = 1.0f / sqrtf(block_sum(s, scratch) / (float)(count > 0 ? count : 1) + a.eps);
+  for (int row = 0; row < len; ++row)
+    for (int c = threadIdx.x; c < cg; c += 256) {
+      const float d = (float)x[row * a.x_n + c] - mean;
+      s += d * d;
+    }
+  const float rstd = 1.0f / sqrtf(block_sum(s, scratch) / count + a.eps);
   if (threadIdx.x == 0) {
     a.stats[2 * (long long)blockIdx.x] = mean;
     a.stats[2 * (long long)blockIdx.x + 1] = rstd;
   }
-  for (long long i = threadIdx.x; i < all; i += 256) {
-    const long long row = i / cg;
-    const int c = (int)(i - row * cg);
-    float v = 0.0f;
-    if (row < len) {
-      const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
-      v = act(hat * param(a.weight, a.weight_type, g * cg + c, 1.0f) + param(a.bias, a.weight_type, g * cg + c, 0.0f), a.activation);
-    }
-    y[row * a.channels + c] = (T)v;
+  for (int c = threadIdx.x; c < cg; c += 256) {
+    const float w = param<T>(a, a.weight, g * cg + c, 1.0f), o = param<T>(a, a.bias, g * cg + c, 0.0f);
+    for (int row = 0; row < a.n; ++row)
+      y[row * (long long)a.channels + c] = (T)(row < len ? act(((float)x[row * a.x_n + c] - mean) * rstd * w + o, a.activation) : 0.0f);
   }
 }
 
-// per (sample, group): the channels' sums of dz and dz xhat (part[sample][2][channels]), then dx
 template <typename T>
-__global__ __launch_bounds__(256) void bwd_any_kernel(const Args a, float* part) {
-  __shared__ float scratch[4], col[2][256];
+__global__ __launch_bounds__(256) void any_bwd_kernel(const Args a) {
+  __shared__ float scratch[4];
   const int b = blockIdx.x / a.groups, g = blockIdx.x % a.groups, cg = a.channels / a.groups, len = length_of(a, b);
   const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + g * cg;
   const long long at = ((long long)b * a.n) * a.channels + g * cg;
   const T* dy = reinterpret_cast<const T*>(a.dy) + at;
   T* dx = reinterpret_cast<T*>(a.dx) + at;
   const float mean = a.stats[2 * (long long)blockIdx.x], rstd = a.stats[2 * (long long)blockIdx.x + 1];
-  int lanes = 1;
-  while (lanes < cg && lanes < 256) lanes *= 2;
-  const int cl = threadIdx.x % lanes, rl = threadIdx.x / lanes, rows = 256 / lanes;
   float t1 = 0.0f, t2 = 0.0f;
-  for (int c0 = 0; c0 < cg; c0 += lanes) {
-    const int c = c0 + cl;
-    const float w = c < cg ? param(a.weight, a.weight_type, g * cg + c, 1.0f) : 0.0f, bias = c < cg ? param(a.bias, a.weight_type, g * cg + c, 0.0f) : 0.0f;
-    float s1 = 0.0f, s2 = 0.0f;
-    if (c < cg)
-      for (int row = rl; row < len; row += rows) {
-        const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
-        const float dz = (float)dy[row * (long long)a.channels + c] * act_slope(hat * w + bias, a.activation);
-        s1 += dz;
-        s2 += dz * hat;
-      }
-    t1 += s1 * w;
-    t2 += s2 * w;
-    __syncthreads();
-    col[0][threadIdx.x] = s1;
-    col[1][threadIdx.x] = s2;
-    __syncthreads();
-    if (part != nullptr && rl == 0 && c < cg) {
-      for (int k = 1; k < rows; ++k) {
-        s1 += col[0][k * lanes + cl];
-        s2 += col[1][k * lanes + cl];
-      }
-      part[(2LL * b) * a.channels + g * cg + c] = s2;
-      part[(2LL * b + 1) * a.channels + g * cg + c] = s1;
+  for (int c = threadIdx.x; c < cg; c += 256) {
+    const float w = param<T>(a, a.weight, g * cg + c, 1.0f), o = param<T>(a, a.bias, g * cg + c, 0.0f);
+    float sb = 0.0f, sw = 0.0f;
+    for (int row = 0; row < len; ++row) {
+      const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
+      const float dz = (float)dy[row * (long long)a.channels + c] * act_slope(hat * w + o, a.activation);
+      sb += dz;
+      sw += dz * hat;
+    }
+    t1 += sb * w;
+    t2 += sw * w;
+    if (a.weight != nullptr) {
+      a.work[(2LL * b) * a.channels + g * cg + c] = sw;
+      a.work[(2LL * b + 1) * a.channels + g * cg + c] = sb;
     }
   }
-  const float count = (float)((long long)len * cg > 0 ? (long long)len * cg : 1);
+  const float count = (float)(len > 0 ? len : 1) * (float)cg;
   t1 = block_sum(t1, scratch) / count;
   t2 = block_sum(t2, scratch) / count;
-  const long long all = (long long)a.n * cg;
-  for (long long i = threadIdx.x; i < all; i += 256) {
-    const long long row = i / cg;
-    const int c = (int)(i - row * cg);
-    float v = 0.0f;
-    if (row < len) {
-      const float w = param(a.weight, a.weight_type, g * cg + c, 1.0f);
-      const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
-      const float dz = (float)dy[row * a.channels + c] * act_slope(hat * w + param(a.bias, a.weight_type, g * cg + c, 0.0f), a.activation);
-      v = rstd * (dz * w - t1 - hat * t2);
+  for (int c = threadIdx.x; c < cg; c += 256) {
+    const float w = param<T>(a, a.weight, g * cg + c, 1.0f), o = param<T>(a, a.bias, g * cg + c, 0.0f);
+    for (int row = 0; row < a.n; ++row) {
+      float v = 0.0f;
+      if (row < len) {
+        const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
+        const float dz = (float)dy[row * (long long)a.channels + c] * act_slope(hat * w + o, a.activation);
+        v = rstd * (dz * w - t1 - hat * t2);
+      }
+      dx[row * (long long)a.channels + c] = (T)v;
     }
-    dx[row * a.channels + c] = (T)v;
   }
 }
 
-// dweight, dbias = the sums of `records` records [2][channels], in order
-__global__ __launch_bounds__(256) void param_grad_kernel(const Args a, const float* part, int records) {
-  __shared__ float sum[4][64];
-  const int i = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, total = 2 * a.channels;
+// dweight, dbias = the sums of `records` records [2][channels]: 16 columns x 64 record lanes a workgroup, then the lanes in order
+template <typename T>
+__global__ __launch_bounds__(1024) void param_grad_kernel(const Args a, const float* part, int records) {
+  __shared__ float sum[64][17];
+  const int col = threadIdx.x & 15, r0 = threadIdx.x >> 4, i = blockIdx.x * 16 + col, total = 2 * a.channels;
   float s = 0.0f;
-  if (i < total)
-    for (int r = w; r < records; r += 4) s += part[(long long)r * total + i];
-  sum[w][threadIdx.x & 63] = s;
+  if (i < total) {
+#pragma unroll 4
+    for (int r = r0; r < records; r += 64) s += part[(long long)r * total + i];
+  }
+  sum[r0][col] = s;
   __syncthreads();
-  if (w == 0 && i < total) {
-    const int l = threadIdx.x;
-    s = (sum[0][l] + sum[1][l]) + (sum[2][l] + sum[3][l]);
-    put(i < a.channels ? a.dweight : a.dbias, a.weight_type, i % a.channels, s);
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) {
+    if (r0 < h) sum[r0][col] += sum[r0 + h][col];
+    __syncthreads();
+  }
+  if (r0 == 0 && i < total) {
+    void* out = i < a.channels ? a.dweight : a.dbias;
+    const int c = i < a.channels ? i : i - a.channels;
+    if (a.weight_type == TYPE_F32) reinterpret_cast<float*>(out)[c] = sum[0][col];
+    else reinterpret_cast<T*>(out)[c] = (T)sum[0][col];
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+bool sizes_ok(const Args& a) {
+  return a.batch >= 1 && a.n >= 1 && a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0 && a.channels <= (1 << 24) &&
+         (long long)a.batch * a.groups <= 0x3fffffffLL && a.type >= TYPE_F32 && a.type <= TYPE_F16;
+}
+
+// The form of a call, by sizes and alignment alone (dy, y and dx are contiguous; their pointers do not enter: x's alignment decides, and the
+// library's callers allocate theirs 16-byte aligned -- checked in run()).
+Plan plan(const Args& a) {
+  Plan p = {};
+  const int full = a.type == TYPE_F32 ? 4 : 8, size = a.type == TYPE_F32 ? 4 : 2, cg = a.channels / a.groups;
+  const bool chunks = (a.x_b | a.x_n) % full == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && cg % full == 0;
+  p.ve = chunks ? full : 1;
+  const int cpg = cg / p.ve;
+  if (a.n == 1 && chunks && cpg <= 64 && (cpg & (cpg - 1)) == 0) {
+    p.form = ROWS;
+    const int lanes_of = a.channels / p.ve < 256 ? a.channels / p.ve : 256;
+    const int per_pass = 256 / lanes_of, columns = (a.channels / p.ve + lanes_of - 1) / lanes_of;
+    const long long passes = ((long long)a.batch + per_pass - 1) / per_pass;
+    const long long most = 2048 / columns > 1 ? 2048 / columns : 1;      // 8 workgroups a CU
+    p.blocks = (int)(passes < most ? passes : most);
+    p.slice = lanes_of;
+    p.slices = columns;
+    p.records = p.blocks;
+    return p;
+  }
+  if (cpg > 256) {
+    p.form = ANY;
+    p.records = a.batch;
+    return p;
+  }
+  // slices of whole groups: 64 bytes of a row at least, more while that still leaves 1024 workgroups, 256 chunks at most
+  auto fits = [&](int gs) { return (long long)gs * cpg <= 256; };
+  int gs = 1;
+  for (int k = 1; k <= a.groups; ++k) {
+    if (!fits(k)) break;
+    if (a.groups % k != 0) continue;
+    const bool narrow = (long long)gs * cg * size < 64, many = (long long)a.batch * (a.groups / k) >= 1024;
+    if (k > gs && (narrow || many)) {
+      const int lanes = 256 / (k * cpg);
+      if (!narrow && (long long)lanes * 16 < a.n) break;      // wider would no longer fit a workgroup's registers
+      gs = k;
+    }
+  }
+  p.slice = gs * cg;
+  p.slices = a.groups / gs;
+  const int lanes = 256 / (gs * cpg), need = (a.n + lanes - 1) / lanes;
+  if (need <= 16) {
+    p.form = SLAB;
+    p.per_thread = need <= 1 ? 1 : need <= 4 ? 4 : 16;
+    p.records = a.batch;
+    return p;
+  }
+  p.form = LONG;
+  // rows as wide as 256 chunks allow; 1024 workgroups, 16 rows a thread at least
+  for (int k = 1; k <= a.groups && fits(k); ++k)
+    if (a.groups % k == 0) gs = k;
+  p.slice = gs * cg;
+  p.slices = a.groups / gs;
+  const int per = 256 / (gs * cpg) * 16;
+  const long long want = 1024 / ((long long)a.batch * p.slices) > 1 ? 1024 / ((long long)a.batch * p.slices) : 1, most = (a.n + per - 1) / per;
+  const int blocks = (int)(want < most ? want : most);
+  p.rows = (a.n + blocks - 1) / blocks;
+  p.blocks = (a.n + p.rows - 1) / p.rows;
+  p.records = a.batch * p.blocks;
+  return p;
+}
+
+long long work_floats(const Args& a, const Plan& p, bool backward) {
+  const long long pairs = p.form == LONG ? 2LL * a.batch * p.blocks * a.groups : 0;
+  return pairs + (backward && a.weight != nullptr ? 2LL * p.records * a.channels : 0);
+}
+
+template <typename T, int VE>
+void launch_slab(const Args& a, const Plan& p, bool backward, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)a.batch * p.slices);
+  if (backward) {
+    if (p.per_thread == 1) slab_bwd_kernel<T, VE, 1><<<grid, 256, 0, st>>>(a, p.slice);
+    else if (p.per_thread == 4) slab_bwd_kernel<T, VE, 4><<<grid, 256, 0, st>>>(a, p.slice);
+    else slab_bwd_kernel<T, VE, 16><<<grid, 256, 0, st>>>(a, p.slice);
+  } else {
+    if (p.per_thread == 1) slab_fwd_kernel<T, VE, 1><<<grid, 256, 0, st>>>(a, p.slice);
+    else if (p.per_thread == 4) slab_fwd_kernel<T, VE, 4><<<grid, 256, 0, st>>>(a, p.slice);
+    else slab_fwd_kernel<T, VE, 16><<<grid, 256, 0, st>>>(a, p.slice);
+  }
+}
+
+template <typename T, int VE>
+void launch_long(const Args& a, const Plan& p, bool backward, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)a.batch * p.blocks * p.slices);
+  if (backward) {
+    long_sum_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
+    long_dx_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
+  } else {
+    long_stat_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
+    long_apply_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
   }
 }
 
 template <typename T>
-void launch(const Args& a, bool backward, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)a.batch * a.groups);
-  if (!backward) {
-    fwd_any_kernel<T><<<grid, 256, 0, st>>>(a);
-    return;
+void launch(const Args& a, const Plan& p, bool backward, hipStream_t st) {
+  constexpr int N = Vec<T>::N;
+  if (p.form == ROWS) {
+    const int cpg = a.channels / a.groups / N;
+    const dim3 grid(p.blocks, p.slices);
+    if (backward) rows_kernel<T, true><<<grid, 256, 0, st>>>(a, cpg, p.slice);
+    else rows_kernel<T, false><<<grid, 256, 0, st>>>(a, cpg, p.slice);
+  } else if (p.form == SLAB) {
+    if (p.ve == 1) launch_slab<T, 1>(a, p, backward, st);
+    else launch_slab<T, N>(a, p, backward, st);
+  } else if (p.form == LONG) {
+    if (p.ve == 1) launch_long<T, 1>(a, p, backward, st);
+    else launch_long<T, N>(a, p, backward, st);
+  } else {
+    const unsigned grid = (unsigned)((long long)a.batch * a.groups);
+    if (backward) any_bwd_kernel<T><<<grid, 256, 0, st>>>(a);
+    else any_fwd_kernel<T><<<grid, 256, 0, st>>>(a);
   }
-  bwd_any_kernel<T><<<grid, 256, 0, st>>>(a, a.weight != nullptr ? a.work : nullptr);
-  if (a.weight != nullptr) param_grad_kernel<<<(2 * a.channels + 63) / 64, 256, 0, st>>>(a, a.work, a.batch);
-}
-
-bool sizes_ok(const Args& a) {
-  return a.batch >= 1 && a.n >= 1 && a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0 && a.channels <= (1 << 24) &&
-         (long long)a.batch * a.groups <= 0x7fffffffLL && a.type >= TYPE_F32 && a.type <= TYPE_F16;
+  if (backward && a.weight != nullptr) {
+    const float* records = a.work + work_floats(a, p, false);
+    param_grad_kernel<T><<<(2 * a.channels + 15) / 16, 1024, 0, st>>>(a, records, p.records);
+  }
 }
 
 int run(const Args* args, bool backward, const char* entry, void* stream) {
@@ -181,11 +836,15 @@ int run(const Args* args, bool backward, const char* entry, void* stream) {
     return fail(entry, -22);
   if (!backward && a.y == nullptr) return fail(entry, -22);
   if (backward && (a.dy == nullptr || a.dx == nullptr || (a.weight != nullptr && (a.dweight == nullptr || a.dbias == nullptr)))) return fail(entry, -22);
-  if (a.work == nullptr && is_group_norm_work_floats(args, backward ? 1 : 0) > 0) return fail(entry, -22);
+  const Plan p = plan(a);
+  const uintptr_t own = backward ? reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx) : reinterpret_cast<uintptr_t>(a.y);
+  if (p.ve > 1 && own % 16 != 0) return fail(entry, -22);
+  if (a.work == nullptr && work_floats(a, p, backward) > 0) return fail(entry, -22);
+  if ((long long)a.batch * (p.slices > 0 ? p.slices : 1) * (p.blocks > 0 ? p.blocks : 1) > 0x7fffffffLL) return fail(entry, -22);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a.type == TYPE_F32) launch<float>(a, backward, st);
-  else if (a.type == TYPE_BF16) launch<__bf16>(a, backward, st);
-  else launch<_Float16>(a, backward, st);
+  if (a.type == TYPE_F32) launch<float>(a, p, backward, st);
+  else if (a.type == TYPE_BF16) launch<__bf16>(a, p, backward, st);
+  else launch<_Float16>(a, p, backward, st);
   return launch_status(entry);
 }
 
@@ -196,7 +855,7 @@ extern "C" {
 
 long long is_group_norm_work_floats(const IsGroupNorm* args, int backward) {
   if (args == nullptr || !is::gn::sizes_ok(*args)) return 0;
-  return backward && args->weight != nullptr ? 2LL * args->batch * args->channels : 0;
+  return is::gn::work_floats(*args, is::gn::plan(*args), backward != 0);
 }
 int is_group_norm_fwd(const IsGroupNorm* args, void* stream) { return is::gn::run(args, false, "is_group_norm_fwd", stream); }
 int is_group_norm_bwd(const IsGroupNorm* args, void* stream) { return is::gn::run(args, true, "is_group_norm_bwd", stream); }

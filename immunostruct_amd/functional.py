@@ -12,7 +12,6 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-import contextlib
 import ctypes
 import os
 
@@ -1762,9 +1761,28 @@ def vae_loss(recon, x, mu, logvar, logit, y, mode, pos_weight, c_pred, c_mse, c_
 # ---- operators of attention blocks over sequences (csrc/rotary.hip, diff_attention*.hip, group_norm.hip) ----------------------------------
 # fp32, bf16 and fp16; they run on the tensors' own device and its current stream, also where that device is not the current one.
 
-def _on(device):
-    """context that makes ``device`` the current one (nothing to do, and nothing spent, where it is already)"""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _enqueue(name, entry, index, *args):
+    """one call of a C entry point on device ``index`` and that device's current stream (the arguments end with the stream)"""
+    if KernelTimer.enabled or index != _current_device():
+        with torch.cuda.device(index), KernelTimer.span(name):
+            code = entry(*args, _raw_stream(index))
+    else:      # (the common case spends nothing on contexts: small launches are bound by what the host does per call)
+        code = entry(*args, _raw_stream(index))
+    if code:
+        _lib.check(code, name)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _aligned(t):
+    """contiguous and 16-byte aligned (an incoming gradient may be any view)"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _sequence_type(name, *tensors):
@@ -1791,22 +1809,22 @@ def _needs_grad(*tensors):
 def _rotary_launch(q, k, freq, positions, layout, amplitude, inverse):
     lib = _lib.load()
     b, n, _, width = q.shape
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    args, outs = [], [None, None]
+    for i, t in enumerate((q, k)):
+        if t is None:
+            args += (None, 0, 0, 0, None, 0)
+        else:
+            # (a copy, where one is made, is freed behind the launch in the order of its stream)
+            t = _lib.last_contiguous(t)
+            outs[i] = torch.empty_like(t, memory_format=torch.contiguous_format)
+            args += (t.data_ptr(), *t.stride()[:3], outs[i].data_ptr(), t.shape[2])
     if b == 0 or n == 0:
         return outs
-    args = []
-    for t, o in zip((q, k), outs):
-        if t is None:
-            args += [None, 0, 0, 0, None, 0]
-        else:
-            t = _lib.last_contiguous(t)      # (a copy, where one is made, lives until the launch below is enqueued on its stream)
-            args += [_lib.ptr(t), t.stride(0), t.stride(1), t.stride(2), _lib.ptr(o), t.shape[2]]
     pos = (None, 0, 0, 0)
     if positions is not None:
-        pos = (_lib.ptr(positions), int(positions.dtype == torch.int64), positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1))
-    with _on(q.device), KernelTimer.span("rotary"):
-        _lib.check(lib.is_rotary(*args, *pos, freq.data_ptr(), b, n, width, 2 * freq.numel(), int(layout == "interleaved"), int(inverse),
-                                 amplitude, _lib.TYPES[q.dtype], _lib.stream_ptr()), "is_rotary")
+        pos = (positions.data_ptr(), positions.dtype == torch.int64, positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1))
+    _enqueue("is_rotary", lib.is_rotary, q.get_device(), *args, *pos, freq.data_ptr(), b, n, width, 2 * freq.numel(), layout == "interleaved",
+             inverse, amplitude, _lib.TYPES[q.dtype])
     return outs
 
 
@@ -1878,12 +1896,10 @@ def _diff_forward(q, k, v, lam, lengths, causal, scale, need):
     splits = lib.is_diff_attention_splits(b, hk, rows, nk)
     floats = lib.is_diff_attention_work_floats(b, hk, rows, dv, splits)
     work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    ptr = lambda t: None if t is None else t.data_ptr()
-    a = _lib.DiffAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), ptr(lengths), out.data_ptr(), ptr(o2), ptr(lse), ptr(work),
+    a = _lib.DiffAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(lengths), out.data_ptr(), _ptr(o2), _ptr(lse), _ptr(work),
                            None, None, None, None, None, None, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
                            b, nq, nk, heads, hk, d, dv, causal, _lib.TYPES[q.dtype], _lib.TYPES[lam.dtype], splits, 0, 0, scale)
-    with _on(q.device), KernelTimer.span("diff_attention_fwd"):
-        _lib.check(lib.is_diff_attention_fwd(ctypes.byref(a), _lib.stream_ptr()), "is_diff_attention_fwd")
+    _enqueue("is_diff_attention_fwd", lib.is_diff_attention_fwd, q.get_device(), ctypes.byref(a))
     return out, o2, lse, a
 
 
@@ -1902,7 +1918,7 @@ class DifferentialAttentionFn(torch.autograd.Function):
     def backward(ctx, g):
         lib = _lib.load()
         q, k, v, lam, lengths, out, o2, lse = ctx.saved_tensors
-        dq, dk, dv, dlam = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, lam))
+        dq, dk, dv, dlam = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, lam))
         if ctx.args is None:
             return dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), None, None, None
         g = g.contiguous()
@@ -1910,8 +1926,7 @@ class DifferentialAttentionFn(torch.autograd.Function):
         a = _lib.DiffAttention.from_buffer_copy(ctx.args)      # (the forward's arguments with this call's buffers; its workspace is gone)
         a.work, a.splits = None, 1
         a.d_o, a.dots, a.dq, a.dk, a.dv_out, a.dlam = (t.data_ptr() for t in (g, dots, dq, dk, dv, dlam))
-        with _on(q.device), KernelTimer.span("diff_attention_bwd"):
-            _lib.check(lib.is_diff_attention_bwd(ctypes.byref(a), _lib.stream_ptr()), "is_diff_attention_bwd")
+        _enqueue("is_diff_attention_bwd", lib.is_diff_attention_bwd, q.get_device(), ctypes.byref(a))
         return dq, dk, dv, dlam, None, None, None
 
 
@@ -1957,19 +1972,17 @@ def _group_norm_launch(x, weight, bias, lengths, groups, eps, activation):
     """-> (y, stats, arguments); x (B, n, channels) with a unit innermost stride"""
     lib = _lib.load()
     b, n, c = x.shape
-    y = torch.empty(b, n, c, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if y.numel() == 0:
         return y, None, None
     stats = torch.empty(b, groups, 2, dtype=torch.float32, device=x.device)
-    ptr = lambda t: None if t is None else t.data_ptr()
-    a = _lib.GroupNorm(x.data_ptr(), ptr(weight), ptr(bias), ptr(lengths), y.data_ptr(), stats.data_ptr(), None, None, None, None, None,
+    a = _lib.GroupNorm(x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(lengths), y.data_ptr(), stats.data_ptr(), None, None, None, None, None,
                        x.stride(0), x.stride(1), b, n, c, groups, activation, _lib.TYPES[x.dtype],
                        0 if weight is None else _lib.TYPES[weight.dtype], 0, eps)
     floats = lib.is_group_norm_work_floats(ctypes.byref(a), 0)
     work = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-    a.work = ptr(work)
-    with _on(x.device), KernelTimer.span("group_norm_fwd"):
-        _lib.check(lib.is_group_norm_fwd(ctypes.byref(a), _lib.stream_ptr()), "is_group_norm_fwd")
+    a.work = _ptr(work)
+    _enqueue("is_group_norm_fwd", lib.is_group_norm_fwd, x.get_device(), ctypes.byref(a))
     return y, stats, a
 
 
@@ -1988,17 +2001,16 @@ class GroupNormFn(torch.autograd.Function):
     def backward(ctx, g):
         lib = _lib.load()
         x, weight, bias, lengths, stats = ctx.saved_tensors
-        dx, dw, db = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, weight, bias))
+        dx, dw, db = (None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, weight, bias))
         if ctx.args is None:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None, None, None
         a = _lib.GroupNorm.from_buffer_copy(ctx.args)
-        g = g.contiguous()
+        g = _aligned(g)
         floats = lib.is_group_norm_work_floats(ctypes.byref(a), 1)
         work = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
         a.y, a.dy, a.dx = None, g.data_ptr(), dx.data_ptr()
-        a.dweight, a.dbias, a.work = (None if t is None else t.data_ptr() for t in (dw, db, work))
-        with _on(x.device), KernelTimer.span("group_norm_bwd"):
-            _lib.check(lib.is_group_norm_bwd(ctypes.byref(a), _lib.stream_ptr()), "is_group_norm_bwd")
+        a.dweight, a.dbias, a.work = _ptr(dw), _ptr(db), _ptr(work)
+        _enqueue("is_group_norm_bwd", lib.is_group_norm_bwd, x.get_device(), ctypes.byref(a))
         return dx, dw, db, None, None, None, None
 
 
