@@ -24,7 +24,8 @@ _P, _I, _F, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlo
 
 # symbol -> argtypes ; keep in sync with include/immunostruct_hip.h
 _RETURNS_LONGLONG = {"is_attn_colmean_probs_floats", "is_contrastive_scratch_floats", "is_contrastive_work_floats",
-                     "is_linear_dgrad_scratch_floats", "is_diff_attention_work_floats", "is_group_norm_work_floats"}
+                     "is_linear_dgrad_scratch_floats", "is_diff_attention_work_floats", "is_diff_attention_row_work_floats",
+                     "is_group_norm_work_floats"}
 SIGNATURES = {
     "is_version": [],
     "is_last_error_string": [],
@@ -97,6 +98,8 @@ SIGNATURES = {
     "is_rotary": [_P, _LL, _LL, _LL, _P, _I, _P, _LL, _LL, _LL, _P, _I, _P, _I, _LL, _LL, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P],
     "is_diff_attention_splits": [_I, _I, _I, _I],
     "is_diff_attention_work_floats": [_I, _I, _I, _I, _I],
+    "is_diff_attention_row_splits": [_I, _I, _I, _I, _I],
+    "is_diff_attention_row_work_floats": [_I, _I, _I, _I, _I, _I],
     "is_diff_attention_fwd": [_P, _P],
     "is_diff_attention_bwd": [_P, _P],
     "is_group_norm_work_floats": [_P, _I],
@@ -150,7 +153,8 @@ class DiffAttention(ctypes.Structure):
                                                "dv_out", "dlam")] + \
                [(n, ctypes.c_longlong) for n in ("q_b", "q_n", "q_h", "k_b", "k_n", "k_h", "v_b", "v_n", "v_h")] + \
                [(n, ctypes.c_int) for n in ("batch", "nq", "nk", "heads", "kv_heads", "d", "dv", "causal", "type", "lam_type", "splits",
-                                            "group", "vec")] + [("scale", ctypes.c_float)]
+                                            "row_splits", "rows", "group", "vec")] + \
+               [("group_magic", ctypes.c_uint), ("scale", ctypes.c_float)]
 
 
 class GroupNorm(ctypes.Structure):
@@ -232,6 +236,13 @@ def rows_ld(t):
 def last_contiguous(t):
     """the tensor itself, or a contiguous copy where its innermost dimension is not laid out element by element (a broadcast input)"""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def sequence_rows(t):
+    """the (B, n, heads, width) tensor itself, or a contiguous copy where the innermost dimension is not laid out element by element or the
+    rows of a tile lie too far apart for the attention kernels' 32-bit offsets"""
+    _, n, h, w = t.stride()
+    return t if w == 1 and n < 2 ** 23 and h * t.shape[2] < 2 ** 27 else t.contiguous()
 
 
 def same_device(first, *tensors):

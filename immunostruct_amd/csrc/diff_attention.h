@@ -44,45 +44,56 @@ __device__ __forceinline__ int first_query(const Args& a, int j, int len) {
   return i < 0 ? 0 : (i < a.nq ? i : a.nq);
 }
 
-template <typename T>
-__device__ __forceinline__ const T* q_row(const Args& a, int b, int hk, int r, int m) {
-  const int i = r / a.group, h = hk * a.group + r % a.group;
-  return reinterpret_cast<const T*>(a.q) + b * a.q_b + i * a.q_n + (2 * h + m) * a.q_h;
+// row r -> (query, head of the group): r / group by a 32-bit reciprocal (floor((2^32 - 1) / group)), at most one too small
+__device__ __forceinline__ int query_of(const Args& a, int r, int& g) {
+  int i = (int)__umulhi((unsigned)r, a.group_magic);
+  g = r - i * a.group;
+  if (g >= a.group) {
+    ++i;
+    g -= a.group;
+  }
+  return i;
 }
-template <typename T>
-__device__ __forceinline__ const T* k_row(const Args& a, int b, int hk, int j, int m) {
-  return reinterpret_cast<const T*>(a.k) + b * a.k_b + j * a.k_n + (2 * hk + m) * a.k_h;
+// element (b, query i, head h) of a contiguous (batch, nq, heads, dv) tensor
+__device__ __forceinline__ long long o_at(const Args& a, int b, int i, int h) { return (((long long)b * a.nq + i) * a.heads + h) * a.dv; }
+
+// byte offsets of a tile's key rows j0 + row_of(k), clamped to the last valid one, from row j0
+template <typename S>
+__device__ __forceinline__ void key_offsets(unsigned (&out)[S::PER], int tid, unsigned stride, int left) {
+#pragma unroll
+  for (int k = 0; k < S::PER; ++k) out[k] = (unsigned)min(S::row_of(tid, k), left) * stride;
 }
-template <typename T>
-__device__ __forceinline__ const T* v_row(const Args& a, int b, int hk, int j) {
-  return reinterpret_cast<const T*>(a.v) + b * a.v_b + j * a.v_n + hk * a.v_h;
-}
-// row r of a contiguous (batch, nq, heads, dv) tensor
-__device__ __forceinline__ long long o_at(const Args& a, int b, int hk, int r) {
-  return (((long long)b * a.nq + r / a.group) * a.heads + hk * a.group + r % a.group) * a.dv;
+// byte offsets of a tile's packed rows r0 + row_of(k), clamped to the last one, from query r0 / group and the group's first head
+template <typename S>
+__device__ __forceinline__ void row_offsets(const Args& a, unsigned (&out)[S::PER], int tid, int r0, int first, unsigned stride, unsigned head) {
+#pragma unroll
+  for (int k = 0; k < S::PER; ++k) {
+    int g;
+    const int i = query_of(a, min(r0 + S::row_of(tid, k), a.rows - 1), g);
+    out[k] = (unsigned)(i - first) * stride + (unsigned)g * head;
+  }
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
 // grid: (row tiles x splits x kv_heads x batch), NW waves of 32 rows.  splits > 1: every workgroup takes one range of the keys and leaves
 // unnormalised sums with their maxima in the workspace; join_kernel puts them together.
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kernel(const Args a) {
-  constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 64 * NW;
+  constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 64 * NW, SZ = sizeof(T);
   constexpr int KB = Tile<T, D>::bytes(KT), VB = Tile<T, DV>::bytes(KT), BUF = 2 * KB + VB;
   __shared__ __align__(16) char lds[2 * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, g = lane >> 5;
-  const int R = a.nq * a.group, tiles = (R + 32 * NW - 1) / (32 * NW);
-  int id = xcd_order(blockIdx.x, gridDim.x);
-  const int tile = tiles - 1 - id % tiles;      // the rows that see most keys first
-  id /= tiles;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int hk = id % a.kv_heads, b = id / a.kv_heads;
+  const int R = a.rows, tiles = (R + 32 * NW - 1) / (32 * NW);
+  int base, unit;
+  grid_order(blockIdx.x, a.batch * a.kv_heads, tiles * a.splits, base, unit);
+  const int split = unit % a.splits, tile = tiles - 1 - unit / a.splits;      // the rows that see most keys first
+  const int b = base / a.kv_heads, hk = base - b * a.kv_heads;
   const int len = length_of(a, b);
   const int row0 = tile * 32 * NW + wave * 32, r = row0 + qi, rr = r < R ? r : R - 1;
-  const int wg_last = min(tile * 32 * NW + 32 * NW, R) - 1;
-  const int wg_end = end_of(a, wg_last / a.group, len);
-  const int my_end = r < R ? end_of(a, rr / a.group, len) : 0;
+  int gi;
+  const int query = query_of(a, rr, gi), head = hk * a.group + gi;
+  const int wg_end = end_of(a, (min(tile * 32 * NW + 32 * NW, R) - 1) / a.group, len);
+  const int my_end = r < R ? end_of(a, query, len) : 0;
   const int wave_end = row0 < R ? end_of(a, min(row0 + 31, R - 1) / a.group, len) : 0;      // no row of the wave sees further
   const int wave_all = row0 + 31 < R ? end_of(a, row0 / a.group, len) : 0;                  // every row of the wave sees this far
   const int per = ((wg_end + a.splits - 1) / a.splits + KT - 1) / KT * KT;
@@ -90,22 +101,29 @@ __global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kern
   const float c = a.scale * 1.44269504088896340736f;
 
   u32x4_t q[2][NJ];
+  const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + 2 * head * a.q_h) * SZ;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const T* row = q_row<T>(a, b, hk, rr, m);
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) q[m][j] = load_chunk<T>(row, 2 * j + g, a.d, a.vec);
-  }
+    for (int j = 0; j < NJ; ++j) q[m][j] = load_chunk<T, VEC>(qp + m * a.q_h * SZ, 2 * j + g, a.d);
   f32x16 o[2][NT];
   zero_acc2(o);
   float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 
-  Stage<T, D, KT, NTH> sk0, sk1;
-  Stage<T, DV, KT, NTH> sv;
+  typedef Stage<T, D, KT, NTH, VEC> StageK;
+  typedef Stage<T, DV, KT, NTH, VEC> StageV;
+  StageK sk0, sk1;
+  StageV sv;
+  const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + 2 * hk * a.k_h) * SZ;
+  const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + hk * a.v_h) * SZ;
   auto fetch = [&](int j0) {
-    sk0.load(tid, [&](int i) { return k_row<T>(a, b, hk, min(j0 + i, len - 1), 0); }, a.d, a.vec);
-    sk1.load(tid, [&](int i) { return k_row<T>(a, b, hk, min(j0 + i, len - 1), 1); }, a.d, a.vec);
-    sv.load(tid, [&](int i) { return v_row<T>(a, b, hk, min(j0 + i, len - 1)); }, a.dv, a.vec);
+    unsigned ko[StageK::PER], vo[StageV::PER];
+    key_offsets<StageK>(ko, tid, (unsigned)a.k_n * SZ, len - 1 - j0);
+    key_offsets<StageV>(vo, tid, (unsigned)a.v_n * SZ, len - 1 - j0);
+    const char* k = kp + j0 * a.k_n * SZ;
+    sk0.load(tid, k, ko, a.d);
+    sk1.load(tid, k + a.k_h * SZ, ko, a.d);
+    sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
   auto place = [&](char* buf) {
     sk0.store(tid, buf);
@@ -179,9 +197,8 @@ __global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kern
 #pragma unroll
   for (int m = 0; m < 2; ++m) total[m] = sum[m] + other_half(sum[m]);
   if (r >= R) return;
-  const long long base = ((long long)b * a.kv_heads + hk);
   if (a.splits > 1) {
-    float* w = a.work + (base * a.splits + split) * (2 * (long long)R * (a.dv + 2));
+    float* w = a.work + ((long long)base * a.splits + split) * (2 * (long long)R * (a.dv + 2));
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       float* wm = w + (m * (long long)R + r) * (a.dv + 2);
@@ -193,19 +210,19 @@ __global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kern
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          store4(wm, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[m][t][4 * u], o[m][t][4 * u + 1], o[m][t][4 * u + 2], o[m][t][4 * u + 3]}, false);
+          store4<float, false>(wm, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[m][t][4 * u], o[m][t][4 * u + 1], o[m][t][4 * u + 2], o[m][t][4 * u + 3]});
     }
     return;
   }
-  const float lam = lam_at<T>(a, hk * a.group + rr % a.group);
+  const float lam = lam_at<T>(a, head);
   const float w0 = total[0] != 0.0f ? 1.0f / total[0] : 0.0f, w1 = total[1] != 0.0f ? 1.0f / total[1] : 0.0f;
   if (a.lse != nullptr && g == 0) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
-      a.lse[(base * 2 + m) * R + r] = total[m] != 0.0f ? __builtin_fmaf(top[m], c, __log2f(total[m])) : INFINITY;
+      a.lse[((long long)base * 2 + m) * R + r] = total[m] != 0.0f ? __builtin_fmaf(top[m], c, __log2f(total[m])) : INFINITY;
   }
-  T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, hk, r);
-  T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, hk, r);
+  T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, query, head);
+  T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, query, head);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -216,20 +233,21 @@ __global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kern
         y[e] = o[1][t][4 * u + e] * w1;
         x[e] = o[0][t][4 * u + e] * w0 - lam * y[e];
       }
-      store4(out, 32 * t + 8 * u + 4 * g, a.dv, x, a.vec);
-      if (a.o2 != nullptr) store4(out2, 32 * t + 8 * u + 4 * g, a.dv, y, a.vec);
+      store4<T, VEC>(out, 32 * t + 8 * u + 4 * g, a.dv, x);
+      if (a.o2 != nullptr) store4<T, VEC>(out2, 32 * t + 8 * u + 4 * g, a.dv, y);
     }
 }
 
 // the splits of one row put together: one wave per row, lane = column
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
-  const int R = a.nq * a.group, lane = threadIdx.x & 63;
+  const int R = a.rows, lane = threadIdx.x & 63;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (w >= (long long)a.batch * a.kv_heads * R) return;
-  const int r = (int)(w % R);
   const long long base = w / R;
-  const int hk = (int)(base % a.kv_heads), b = (int)(base / a.kv_heads);
+  const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
+  int gi;
+  const int query = query_of(a, r, gi), head = hk * a.group + gi;
   float inv[2], top[2], total[2];
   const long long step = 2 * (long long)R * (a.dv + 2);
   const float* from[2];
@@ -243,9 +261,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     inv[m] = total[m] != 0.0f ? 1.0f / total[m] : 0.0f;
     if (a.lse != nullptr && lane == 0) a.lse[(base * 2 + m) * R + r] = total[m] != 0.0f ? top[m] + __log2f(total[m]) : INFINITY;
   }
-  const float lam = lam_at<T>(a, hk * a.group + r % a.group);
-  T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, hk, r);
-  T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, hk, r);
+  const float lam = lam_at<T>(a, head);
+  T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, query, head);
+  T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, query, head);
   for (int col = lane; col < a.dv; col += 64) {
     float x[2];
     for (int m = 0; m < 2; ++m) {
@@ -263,13 +281,14 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // D_2 = dO . O_2 and D_1 = dO . O + lam D_2 of every row (one wave per row)
 template <typename T>
 __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
-  const int R = a.nq * a.group, lane = threadIdx.x & 63;
+  const int R = a.rows, lane = threadIdx.x & 63;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (w >= (long long)a.batch * a.kv_heads * R) return;
-  const int r = (int)(w % R);
   const long long base = w / R;
-  const int hk = (int)(base % a.kv_heads), b = (int)(base / a.kv_heads);
-  const long long at = o_at(a, b, hk, r);
+  const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
+  int gi;
+  const int query = query_of(a, r, gi), head = hk * a.group + gi;
+  const long long at = o_at(a, b, query, head);
   const T *o = reinterpret_cast<const T*>(a.o) + at, *o2 = reinterpret_cast<const T*>(a.o2) + at, *go = reinterpret_cast<const T*>(a.d_o) + at;
   float s = 0.0f, s2 = 0.0f;
   for (int col = lane; col < a.dv; col += 64) {
@@ -282,21 +301,21 @@ __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   s += other_half(s);
   s2 += other_half(s2);
   if (lane == 0) {
-    a.dots[(base * 2) * R + r] = s + lam_at<T>(a, hk * a.group + r % a.group) * s2;
+    a.dots[(base * 2) * R + r] = s + lam_at<T>(a, head) * s2;
     a.dots[(base * 2 + 1) * R + r] = s2;
   }
 }
 
-// dlam_h = - sum over samples and queries of D_2 (one workgroup per head, fixed order)
+// dlam_h = - sum over samples and queries of sum_j P_2 dP (dq_kernel's unrounded sums; one workgroup per head, fixed order)
 template <typename T>
 __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
   __shared__ float part[16];
-  const int h = blockIdx.x, hk = h / a.group, gi = h % a.group, R = a.nq * a.group;
+  const int h = blockIdx.x, hk = h / a.group, gi = h % a.group, R = a.rows;
   float s = 0.0f;
   for (long long x = threadIdx.x; x < (long long)a.batch * a.nq; x += 1024) {
     const long long b = x / a.nq;
     const int i = (int)(x - b * a.nq);
-    s += a.dots[((b * a.kv_heads + hk) * 2 + 1) * R + i * a.group + gi];
+    s += a.dots[(2LL * a.batch * a.kv_heads + b * a.kv_heads + hk) * R + i * a.group + gi];
   }
   s = sum_over_r(s);
   s += other_half(s);
@@ -310,50 +329,70 @@ __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
   }
 }
 
-// dK, dV of 32 keys per wave: grid (key tiles x kv_heads x batch)
-template <typename T, int D>
+// dK, dV of 32 keys per wave: grid (key tiles x row splits x kv_heads x batch).  row_splits > 1: the rows that see a key tile are cut into equal
+// parts, whose sums meet in the workspace (key_join_kernel): with a causal mask the first keys are seen by all rows and the last by few, and a
+// workgroup of 512-register waves is alone on its CU, so one workgroup per key tile would leave half the chip idle half the time.
+template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
-  constexpr int DV = 2 * D, RT = 32, NT = D / 32, NTV = DV / 32, NJ = D / (2 * Vec<T>::N), NJV = DV / (2 * Vec<T>::N);
+  constexpr int DV = 2 * D, RT = 32, NT = D / 32, NTV = DV / 32, NJ = D / (2 * Vec<T>::N), NJV = DV / (2 * Vec<T>::N), SZ = sizeof(T);
   constexpr int QB = Tile<T, D>::bytes(RT), OB = Tile<T, DV>::bytes(RT), BUF = 2 * QB + OB;
   __shared__ __align__(16) char lds[2 * BUF];
   __shared__ __align__(16) float stat[2][5][RT];      // lse1, lse2, D1, D2, lam of the tile's rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ki = lane & 31, g = lane >> 5;
-  const int R = a.nq * a.group, tiles = (a.nk + 127) / 128;
-  int id = xcd_order(blockIdx.x, gridDim.x);
-  const int tile = id % tiles;      // the keys that most rows see first
-  id /= tiles;
-  const int hk = id % a.kv_heads, b = id / a.kv_heads;
+  const int R = a.rows, tiles = (a.nk + 127) / 128;
+  int base, unit;
+  grid_order(blockIdx.x, a.batch * a.kv_heads, tiles * a.row_splits, base, unit);
+  const int split = unit % a.row_splits, tile = unit / a.row_splits;      // the keys that most rows see first
+  const int b = base / a.kv_heads, hk = base - b * a.kv_heads;
   const int len = length_of(a, b);
   const int wg_key = tile * 128, key0 = wg_key + wave * 32, key = key0 + ki;
-  const long long base = (long long)b * a.kv_heads + hk;
   const float c = a.scale * 1.44269504088896340736f;
   u32x4_t k[2][NJ], v[NJV];
   f32x16 dk0[1][NT], dk1[1][NT], dv[1][NTV];
   zero_acc2(dk0);
   zero_acc2(dk1);
   zero_acc2(dv);
-  const int r_first = wg_key < len ? first_query(a, wg_key, len) * a.group / RT * RT : R;
+  const int seen_from = wg_key < len ? first_query(a, wg_key, len) * a.group / RT * RT : R;
+  const int per = ((R - seen_from + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
+  const int r_first = seen_from + split * per, r_last = min(R, r_first + per);
   const int wave_first = key0 < len ? first_query(a, key0, len) * a.group : R;
   const int wave_all = key0 + 31 < len ? first_query(a, key0 + 31, len) * a.group : R;      // rows from here on see all 32 keys
   const int my_first = key < len ? first_query(a, key, len) * a.group : R;                   // rows from here on see this lane's key
-  if (r_first < R) {
+  if (r_first < r_last) {
     const int kk = min(key, len - 1);
+    const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + kk * a.k_n + 2 * hk * a.k_h) * SZ;
+    const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + kk * a.v_n + hk * a.v_h) * SZ;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) k[m][j] = load_chunk<T>(k_row<T>(a, b, hk, kk, m), 2 * j + g, a.d, a.vec);
+      for (int j = 0; j < NJ; ++j) k[m][j] = load_chunk<T, VEC>(kp + m * a.k_h * SZ, 2 * j + g, a.d);
 #pragma unroll
-    for (int j = 0; j < NJV; ++j) v[j] = load_chunk<T>(v_row<T>(a, b, hk, kk), 2 * j + g, a.dv, a.vec);
-    Stage<T, D, RT, 256> sq0, sq1;
-    Stage<T, DV, RT, 256> so;
+    for (int j = 0; j < NJV; ++j) v[j] = load_chunk<T, VEC>(vp, 2 * j + g, a.dv);
+    typedef Stage<T, D, RT, 256, VEC> StageQ;
+    typedef Stage<T, DV, RT, 256, VEC> StageO;
+    StageQ sq0, sq1;
+    StageO so;
     float st = 0.0f;
+    const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + 2 * hk * a.group * a.q_h) * SZ;
+    const char* op = reinterpret_cast<const char*>(a.d_o) + o_at(a, b, 0, hk * a.group) * SZ;
     auto fetch = [&](int r0) {
-      sq0.load(tid, [&](int i) { return q_row<T>(a, b, hk, min(r0 + i, R - 1), 0); }, a.d, a.vec);
-      sq1.load(tid, [&](int i) { return q_row<T>(a, b, hk, min(r0 + i, R - 1), 1); }, a.d, a.vec);
-      so.load(tid, [&](int i) { return reinterpret_cast<const T*>(a.d_o) + o_at(a, b, hk, min(r0 + i, R - 1)); }, a.dv, a.vec);
+      unsigned qo[StageQ::PER], oo[StageO::PER];
+      const int i0 = r0 / a.group;
+      row_offsets<StageQ>(a, qo, tid, r0, i0, (unsigned)a.q_n * SZ, 2u * (unsigned)a.q_h * SZ);
+      row_offsets<StageO>(a, oo, tid, r0, i0, (unsigned)(a.heads * a.dv) * SZ, (unsigned)a.dv * SZ);
+      const char* q = qp + i0 * a.q_n * SZ;
+      sq0.load(tid, q, qo, a.d);
+      sq1.load(tid, q + a.q_h * SZ, qo, a.d);
+      so.load(tid, op + (long long)i0 * a.heads * a.dv * SZ, oo, a.dv);
       if (tid < 5 * RT) {
         const int w = tid >> 5, rw = min(r0 + (tid & 31), R - 1);
-        st = w < 2 ? a.lse[(base * 2 + w) * R + rw] : w < 4 ? a.dots[(base * 2 + w - 2) * R + rw] : lam_at<T>(a, hk * a.group + rw % a.group);
+        if (w < 4) {
+          st = (w < 2 ? a.lse : a.dots)[((long long)base * 2 + (w & 1)) * R + rw];
+        } else {
+          int gi;
+          query_of(a, rw, gi);
+          st = lam_at<T>(a, hk * a.group + gi);
+        }
       }
     };
     auto place = [&](int buf) {
@@ -366,8 +405,8 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
     place(0);
     __syncthreads();
     int cur = 0;
-    for (int r0 = r_first; r0 < R; r0 += RT) {
-      const bool more = r0 + RT < R;
+    for (int r0 = r_first; r0 < r_last; r0 += RT) {
+      const bool more = r0 + RT < r_last;
       if (more) fetch(r0 + RT);
       if (r0 + RT > wave_first) {
         const char* buf = lds + cur * BUF;
@@ -388,10 +427,10 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = 4 * u + e;
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[0][t], c, -l1[e])), p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[1][t], c, -l2[e]));
-            w[0][t] = p1 - lm[e] * p2;
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[0][t], c, -l1[e])), p2 = lm[e] * __builtin_amdgcn_exp2f(__builtin_fmaf(p[1][t], c, -l2[e]));
+            w[0][t] = p1 - p2;
             p[0][t] = p1 * (dp[t] - d1[e]);
-            p[1][t] = -lm[e] * p2 * (dp[t] - d2[e]);
+            p[1][t] = p2 * (d2[e] - dp[t]);
             if (edge) {      // (the products are replaced, not the factors: nothing that stands in a hidden place gets through)
               const int row = r0 + tile_row(t, g);
               const bool seen = row >= my_first && row < R;
@@ -415,69 +454,112 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
     }
   }
   if (key >= a.nk) return;
-  T* dkp = reinterpret_cast<T*>(a.dk) + ((long long)b * a.nk + key) * (2 * a.kv_heads) * a.d + (2 * hk) * (long long)a.d;
-  T* dvp = reinterpret_cast<T*>(a.dv_out) + (((long long)b * a.nk + key) * a.kv_heads + hk) * a.dv;
   const bool live = key < len;      // (rows behind the length: the clamped key's sums are not theirs)
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        f32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = live ? (m == 0 ? dk0 : dk1)[0][t][4 * u + e] * a.scale : 0.0f;
-        store4(dkp + m * a.d, 32 * t + 8 * u + 4 * g, a.d, x, a.vec);
-      }
-#pragma unroll
-  for (int t = 0; t < NTV; ++t)
+  auto each = [&](auto put) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = live ? dv[0][t][4 * u + e] : 0.0f;
-      store4(dvp, 32 * t + 8 * u + 4 * g, a.dv, x, a.vec);
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = live ? (m == 0 ? dk0 : dk1)[0][t][4 * u + e] * a.scale : 0.0f;
+          put(m, 32 * t + 8 * u + 4 * g, x);
+        }
+#pragma unroll
+      for (int t = 0; t < NTV; ++t) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = live ? dv[0][t][4 * u + e] : 0.0f;
+        put(2, 32 * t + 8 * u + 4 * g, x);
+      }
     }
+  };
+  const long long at = ((long long)b * a.nk + key) * a.kv_heads + hk;
+  if (a.row_splits > 1) {      // [split][sample, key, head][dk1 | dk2 | dv]
+    const int w = 2 * a.d + a.dv;
+    float* part = a.work + ((long long)split * a.batch * a.nk * a.kv_heads + at) * w;
+    each([&](int m, int col, f32x4 x) { store4<float, VEC>(part + m * a.d, col, m < 2 ? a.d : a.dv, x); });
+  } else {
+    T* dkp = reinterpret_cast<T*>(a.dk) + at * 2 * a.d;
+    T* dvp = reinterpret_cast<T*>(a.dv_out) + at * a.dv;
+    each([&](int m, int col, f32x4 x) { store4<T, VEC>(m < 2 ? dkp + m * a.d : dvp, col, m < 2 ? a.d : a.dv, x); });
+  }
+}
+
+// dK, dV = the row splits' sums, in order; a thread per four elements (VEC) or one
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void key_join_kernel(const Args a) {
+  constexpr int N = VEC ? 4 : 1;
+  const int w = 2 * a.d + a.dv, items = w / N;
+  const long long all = (long long)a.batch * a.nk * a.kv_heads, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= all * items) return;
+  const long long at = i / items;
+  const int col = (int)(i - at * items) * N;
+  float x[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = 0.0f;
+  for (int s = 0; s < a.row_splits; ++s) {
+    const float* part = a.work + (s * all + at) * w + col;
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] += part[e];
+  }
+  T* out = col < 2 * a.d ? reinterpret_cast<T*>(a.dk) + at * 2 * a.d + col : reinterpret_cast<T*>(a.dv_out) + at * a.dv + (col - 2 * a.d);
+  if constexpr (VEC) store4<T, true>(out, 0, 4, f32x4{x[0], x[1], x[2], x[3]});
+  else *out = (T)x[0];
 }
 
 // dQ of 32 rows per wave: grid (row tiles x kv_heads x batch)
-template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void dq_kernel(const Args a) {
-  constexpr int DV = 2 * D, KT = 32, NT = D / 32, NJ = D / (2 * Vec<T>::N), NJV = DV / (2 * Vec<T>::N);
+template <typename T, int D, bool VEC>
+__global__ __launch_bounds__(256, (D <= 64 && sizeof(T) == 2) || D <= 32 ? 2 : 1) void dq_kernel(const Args a) {
+  constexpr int DV = 2 * D, KT = 32, NT = D / 32, NJ = D / (2 * Vec<T>::N), NJV = DV / (2 * Vec<T>::N), SZ = sizeof(T);
   constexpr int KB = Tile<T, D>::bytes(KT), VB = Tile<T, DV>::bytes(KT), BUF = 2 * KB + VB;
   __shared__ __align__(16) char lds[2 * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, g = lane >> 5;
-  const int R = a.nq * a.group, tiles = (R + 127) / 128;
-  int id = xcd_order(blockIdx.x, gridDim.x);
-  const int tile = tiles - 1 - id % tiles;
-  id /= tiles;
-  const int hk = id % a.kv_heads, b = id / a.kv_heads;
+  const int R = a.rows, tiles = (R + 127) / 128;
+  int base, unit;
+  grid_order(blockIdx.x, a.batch * a.kv_heads, tiles, base, unit);
+  const int tile = tiles - 1 - unit;
+  const int b = base / a.kv_heads, hk = base - b * a.kv_heads;
   const int len = length_of(a, b);
   const int row0 = tile * 128 + wave * 32, r = row0 + qi, rr = r < R ? r : R - 1;
+  int gi;
+  const int query = query_of(a, rr, gi), head = hk * a.group + gi;
   const int wg_end = end_of(a, (min(tile * 128 + 128, R) - 1) / a.group, len);
-  const int my_end = r < R ? end_of(a, rr / a.group, len) : 0;
+  const int my_end = r < R ? end_of(a, query, len) : 0;
   const int wave_end = row0 < R ? end_of(a, min(row0 + 31, R - 1) / a.group, len) : 0;
   const int wave_all = row0 + 31 < R ? end_of(a, row0 / a.group, len) : 0;
-  const long long base = (long long)b * a.kv_heads + hk;
   const float c = a.scale * 1.44269504088896340736f;
   u32x4_t q[2][NJ], go[NJV];
+  const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + 2 * head * a.q_h) * SZ;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) q[m][j] = load_chunk<T>(q_row<T>(a, b, hk, rr, m), 2 * j + g, a.d, a.vec);
+    for (int j = 0; j < NJ; ++j) q[m][j] = load_chunk<T, VEC>(qp + m * a.q_h * SZ, 2 * j + g, a.d);
+  const char* gp = reinterpret_cast<const char*>(a.d_o) + o_at(a, b, query, head) * SZ;
 #pragma unroll
-  for (int j = 0; j < NJV; ++j) go[j] = load_chunk<T>(reinterpret_cast<const T*>(a.d_o) + o_at(a, b, hk, rr), 2 * j + g, a.dv, a.vec);
-  const float l1 = a.lse[(base * 2) * R + rr], l2 = a.lse[(base * 2 + 1) * R + rr];
-  const float d1 = a.dots[(base * 2) * R + rr], d2 = a.dots[(base * 2 + 1) * R + rr], lam = lam_at<T>(a, hk * a.group + rr % a.group);
+  for (int j = 0; j < NJV; ++j) go[j] = load_chunk<T, VEC>(gp, 2 * j + g, a.dv);
+  const long long at = (long long)base * 2 * R + rr;
+  const float l1 = a.lse[at], l2 = a.lse[at + R], d1 = a.dots[at], d2 = a.dots[at + R], lam = lam_at<T>(a, head);
+  float sum2 = 0.0f;      // sum_j P_2 dP, for dlam
   f32x16 dq0[1][NT], dq1[1][NT];
   zero_acc2(dq0);
   zero_acc2(dq1);
-  Stage<T, D, KT, 256> sk0, sk1;
-  Stage<T, DV, KT, 256> sv;
+  typedef Stage<T, D, KT, 256, VEC> StageK;
+  typedef Stage<T, DV, KT, 256, VEC> StageV;
+  StageK sk0, sk1;
+  StageV sv;
+  const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + 2 * hk * a.k_h) * SZ;
+  const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + hk * a.v_h) * SZ;
   auto fetch = [&](int j0) {
-    sk0.load(tid, [&](int i) { return k_row<T>(a, b, hk, min(j0 + i, len - 1), 0); }, a.d, a.vec);
-    sk1.load(tid, [&](int i) { return k_row<T>(a, b, hk, min(j0 + i, len - 1), 1); }, a.d, a.vec);
-    sv.load(tid, [&](int i) { return v_row<T>(a, b, hk, min(j0 + i, len - 1)); }, a.dv, a.vec);
+    unsigned ko[StageK::PER], vo[StageV::PER];
+    key_offsets<StageK>(ko, tid, (unsigned)a.k_n * SZ, len - 1 - j0);
+    key_offsets<StageV>(vo, tid, (unsigned)a.v_n * SZ, len - 1 - j0);
+    const char* k = kp + j0 * a.k_n * SZ;
+    sk0.load(tid, k, ko, a.d);
+    sk1.load(tid, k + a.k_h * SZ, ko, a.d);
+    sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
   auto place = [&](char* buf) {
     sk0.store(tid, buf);
@@ -502,17 +584,22 @@ __global__ __launch_bounds__(256, 1) void dq_kernel(const Args a) {
         mm_tile<T, D>(p[1], buf + KB, 0, q[1], lane);
         mm_tile<T, DV>(dp, buf + 2 * KB, 0, go, lane);
         const bool edge = j0 + KT > wave_all;
+        float s = 0.0f;
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[0][t], c, -l1)), p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[1][t], c, -l2));
+          float both = p2 * dp[t];
           p[0][t] = p1 * (dp[t] - d1);
-          p[1][t] = -lam * p2 * (dp[t] - d2);
+          p[1][t] = p2 * (d2 - dp[t]) * lam;
           if (edge) {
             const bool seen = j0 + tile_row(t, g) < my_end;
             p[0][t] = seen ? p[0][t] : 0.0f;
             p[1][t] = seen ? p[1][t] : 0.0f;
+            both = seen ? both : 0.0f;
           }
+          s += both;
         }
+        sum2 += s;
         f32x16 one[1] = {p[0]};
         mm_transposed<T, D, NT, 1>(dq0, buf, 0, one, lane);
         one[0] = p[1];
@@ -525,9 +612,10 @@ __global__ __launch_bounds__(256, 1) void dq_kernel(const Args a) {
       }
     }
   }
+  sum2 += other_half(sum2);
   if (r >= R) return;
-  const int i = r / a.group, h = hk * a.group + r % a.group;
-  T* out = reinterpret_cast<T*>(a.dq) + (((long long)b * a.nq + i) * a.heads + h) * 2 * a.d;
+  if (g == 0) a.dots[(2LL * a.batch * a.kv_heads + base) * R + r] = sum2;
+  T* out = reinterpret_cast<T*>(a.dq) + (((long long)b * a.nq + query) * a.heads + head) * 2 * a.d;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -537,36 +625,45 @@ __global__ __launch_bounds__(256, 1) void dq_kernel(const Args a) {
         f32x4 x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = (m == 0 ? dq0 : dq1)[0][t][4 * u + e] * a.scale;
-        store4(out + m * a.d, 32 * t + 8 * u + 4 * g, a.d, x, a.vec);
+        store4<T, VEC>(out + m * a.d, 32 * t + 8 * u + 4 * g, a.d, x);
       }
 }
 
 // ---- launches: one compilation unit per element type ----------------------------------------------------------------------------------
-template <typename T, int D>
+template <typename T, int D, bool VEC>
 void launch_fwd(const Args& a, hipStream_t st) {
-  const int R = a.nq * a.group;
-  if (R <= 32) {      // a handful of rows: one wave per workgroup, the keys split over many of them
-    fwd_kernel<T, D, 1><<<a.splits * a.kv_heads * a.batch, 64, 0, st>>>(a);
+  const int heads = a.kv_heads * a.batch;
+  if (a.rows <= 32) {      // a handful of rows: one wave per workgroup, the keys split over many of them
+    fwd_kernel<T, D, 1, VEC><<<a.splits * heads, 64, 0, st>>>(a);
   } else {
-    fwd_kernel<T, D, 4><<<(R + 127) / 128 * a.splits * a.kv_heads * a.batch, 256, 0, st>>>(a);
+    fwd_kernel<T, D, 4, VEC><<<(a.rows + 127) / 128 * a.splits * heads, 256, 0, st>>>(a);
   }
-  if (a.splits > 1) join_kernel<T><<<(unsigned)(((long long)a.batch * a.kv_heads * R + 3) / 4), 256, 0, st>>>(a);
+  if (a.splits > 1) join_kernel<T><<<(unsigned)(((long long)heads * a.rows + 3) / 4), 256, 0, st>>>(a);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool VEC>
 void launch_bwd(const Args& a, hipStream_t st) {
-  const int R = a.nq * a.group;
-  rowdot_kernel<T><<<(unsigned)(((long long)a.batch * a.kv_heads * R + 3) / 4), 256, 0, st>>>(a);
+  const int heads = a.kv_heads * a.batch;
+  rowdot_kernel<T><<<(unsigned)(((long long)heads * a.rows + 3) / 4), 256, 0, st>>>(a);
+  dkv_kernel<T, D, VEC><<<(a.nk + 127) / 128 * a.row_splits * heads, 256, 0, st>>>(a);
+  if (a.row_splits > 1)
+    key_join_kernel<T, VEC><<<(unsigned)(((long long)heads * a.nk * (2 * a.d + a.dv) / (VEC ? 4 : 1) + 255) / 256), 256, 0, st>>>(a);
+  dq_kernel<T, D, VEC><<<(a.rows + 127) / 128 * heads, 256, 0, st>>>(a);
   dlam_kernel<T><<<a.heads, 1024, 0, st>>>(a);
-  dkv_kernel<T, D><<<(a.nk + 127) / 128 * a.kv_heads * a.batch, 256, 0, st>>>(a);
-  dq_kernel<T, D><<<(R + 127) / 128 * a.kv_heads * a.batch, 256, 0, st>>>(a);
 }
 
 // the built width a call runs at: heads of at most D elements, values of at most 2 D (shorter rows are padded with zeros on chip);
 // 0: wider than any.  32-bit inputs stop at 64 / 128: the resident operands of wider heads do not fit a wave's 512 registers.
+// Rows that cannot be read in 16-byte chunks (odd sizes, strides or pointers) run element by element at the widest.
 inline int class_of(const Args& a) {
-  const int need = a.d > (a.dv + 1) / 2 ? a.d : (a.dv + 1) / 2;
-  return need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 && a.type != TYPE_F32 ? 128 : 0;
+  const int need = a.d > (a.dv + 1) / 2 ? a.d : (a.dv + 1) / 2, most = a.type == TYPE_F32 ? 64 : 128;
+  return need > most ? 0 : !a.vec ? most : need <= 32 ? 32 : need <= 64 ? 64 : 128;
+}
+
+template <typename T, int D, bool VEC>
+void launch(const Args& a, bool backward, hipStream_t st) {
+  if (backward) launch_bwd<T, D, VEC>(a, st);
+  else launch_fwd<T, D, VEC>(a, st);
 }
 
 void run_f32(const Args& a, bool backward, hipStream_t st);

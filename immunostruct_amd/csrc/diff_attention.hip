@@ -12,17 +12,22 @@ int prepare(da::Args& a) {
   if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.lam == nullptr || a.o == nullptr) return -22;
   if (a.batch < 1 || a.nq < 1 || a.nk < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.d < 1 || a.dv < 1) return -22;
   if (a.type < TYPE_F32 || a.type > TYPE_F16 || (a.lam_type != TYPE_F32 && a.lam_type != a.type) || a.causal < 0 || a.causal > 2) return -22;
-  if (!(a.scale > 0.0f) || !(a.scale < INFINITY) || a.splits < 1) return -22;
+  if (!(a.scale > 0.0f) || !(a.scale < INFINITY) || a.splits < 1 || a.row_splits < 1) return -22;
   a.group = a.heads / a.kv_heads;
+  a.group_magic = 0xffffffffu / (unsigned)a.group;
   const long long rows = (long long)a.nq * a.group, big = 0x7fffff00LL;
+  const int n = a.type == TYPE_F32 ? 4 : 8, size = 16 / n;
   if (rows > big || a.nk > big || (rows / 32 + 1) * a.splits * a.kv_heads > big / a.batch || (rows + 3) * a.kv_heads > big / a.batch ||
-      (a.nk / 32 + 1LL) * a.kv_heads > big / a.batch) return -22;
-  if (da::class_of(a) == 0) return -38;
-  const int n = a.type == TYPE_F32 ? 4 : 8;
+      (a.nk / 128 + 1LL) * a.row_splits * a.kv_heads > big / a.batch || (a.nk * (2LL * a.d + a.dv) + 255) / 256 * a.kv_heads > big / a.batch) return -22;
+  a.rows = (int)rows;
+  // a tile's rows lie within 31 bits of its first
+  const long long near = 0x7fffffffLL / size;
+  if (a.q_n < 0 || a.q_h < 0 || a.k_n < 0 || a.v_n < 0 || a.q_n > near / 64 || a.k_n > near / 64 || a.v_n > near / 64 ||
+      a.q_h > near / 4 / a.group || (long long)a.heads * a.dv > near / 64) return -22;
   const long long strides = a.q_b | a.q_n | a.q_h | a.k_b | a.k_n | a.k_h | a.v_b | a.v_n | a.v_h;
   a.vec = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.o) && aligned16(a.o2) && aligned16(a.d_o) && aligned16(a.dq) &&
           aligned16(a.dk) && aligned16(a.dv_out) && strides % n == 0 && a.d % n == 0 && a.dv % n == 0;
-  return 0;
+  return da::class_of(a) == 0 ? -38 : 0;
 }
 
 int run(const da::Args& a, bool backward, const char* entry, void* stream) {
@@ -47,6 +52,20 @@ int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk) {
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
+// Row splits of the key gradients: workgroups of 128 keys are alone on their CU.  With a mask the first tiles have all the work, two parts of
+// each fill the gaps the last ones leave; few key tiles are split until 256 workgroups are there, at least 256 rows each, 16 parts at most.
+int is_diff_attention_row_splits(int batch, int kv_heads, int rows, int nk, int causal) {
+  if (batch < 1 || kv_heads < 1 || rows < 1 || nk < 1) return 1;
+  const long long groups = (nk + 127LL) / 128 * kv_heads * batch, most = (rows + 255LL) / 256;
+  long long s = groups <= 128 ? 256 / groups : causal != 0 && groups < 1024 ? 2 : 1;
+  s = s < most ? s : most;
+  return s < 1 ? 1 : s > 16 ? 16 : (int)s;
+}
+
+long long is_diff_attention_row_work_floats(int batch, int kv_heads, int nk, int d, int dv, int row_splits) {
+  return row_splits <= 1 ? 0 : (long long)row_splits * batch * kv_heads * nk * (2 * d + dv);
+}
+
 long long is_diff_attention_work_floats(int batch, int kv_heads, int rows, int dv, int splits) {
   return splits <= 1 ? 0 : 2LL * batch * kv_heads * splits * rows * (dv + 2);
 }
@@ -56,6 +75,7 @@ int is_diff_attention_fwd(const IsDiffAttention* args, void* stream) {
   da::Args a = *args;
   a.d_o = nullptr;
   a.dq = a.dk = a.dv_out = a.dlam = nullptr;
+  a.row_splits = 1;
   const int rc = prepare(a);
   if (rc != 0) return fail("is_diff_attention_fwd", rc);
   if ((a.lse == nullptr) != (a.o2 == nullptr) || (a.splits > 1 && a.work == nullptr)) return fail("is_diff_attention_fwd", -22);
@@ -69,7 +89,7 @@ int is_diff_attention_bwd(const IsDiffAttention* args, void* stream) {
   const int rc = prepare(a);
   if (rc != 0) return fail("is_diff_attention_bwd", rc);
   if (a.o2 == nullptr || a.lse == nullptr || a.d_o == nullptr || a.dots == nullptr || a.dq == nullptr || a.dk == nullptr ||
-      a.dv_out == nullptr || a.dlam == nullptr)
+      a.dv_out == nullptr || a.dlam == nullptr || (a.row_splits > 1 && a.work == nullptr))
     return fail("is_diff_attention_bwd", -22);
   return run(a, true, "is_diff_attention_bwd", stream);
 }

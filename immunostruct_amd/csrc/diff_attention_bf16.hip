@@ -6,9 +6,10 @@ namespace da {
 
 void run_bf16(const Args& a, bool backward, hipStream_t st) {
   const int width = class_of(a);
-  if (width == 32) backward ? launch_bwd<__bf16, 32>(a, st) : launch_fwd<__bf16, 32>(a, st);
-  else if (width == 64) backward ? launch_bwd<__bf16, 64>(a, st) : launch_fwd<__bf16, 64>(a, st);
-  else if (width == 128) backward ? launch_bwd<__bf16, 128>(a, st) : launch_fwd<__bf16, 128>(a, st);
+  if (!a.vec) launch<__bf16, 128, false>(a, backward, st);
+  else if (width == 32) launch<__bf16, 32, true>(a, backward, st);
+  else if (width == 64) launch<__bf16, 64, true>(a, backward, st);
+  else if (width == 128) launch<__bf16, 128, true>(a, backward, st);
 }
 
 }  // namespace da

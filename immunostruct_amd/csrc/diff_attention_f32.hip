@@ -6,8 +6,9 @@ namespace da {
 
 void run_f32(const Args& a, bool backward, hipStream_t st) {
   const int width = class_of(a);
-  if (width == 32) backward ? launch_bwd<float, 32>(a, st) : launch_fwd<float, 32>(a, st);
-  else if (width == 64) backward ? launch_bwd<float, 64>(a, st) : launch_fwd<float, 64>(a, st);
+  if (!a.vec) launch<float, 64, false>(a, backward, st);
+  else if (width == 32) launch<float, 32, true>(a, backward, st);
+  else if (width == 64) launch<float, 64, true>(a, backward, st);
 }
 
 }  // namespace da

@@ -46,18 +46,19 @@ template <typename T> struct Vec {
   }
 };
 
-// a chunk of a row in global memory: elements [c * N, c * N + N) of which the first `len` of the row exist (the rest are 0).
-// vec: rows are 16-byte aligned and `len` is a multiple of N, so a chunk is there whole or not at all.
-template <typename T>
-__device__ __forceinline__ u32x4_t load_chunk(const T* row, int c, int len, bool vec) {
+// chunk c of a row in global memory: elements [c N, c N + N) of which the first `len` of the row exist (the rest are 0).
+// VEC: rows are 16-byte aligned and `len` is a multiple of N, so a chunk is there whole or not at all.
+template <typename T, bool VEC>
+__device__ __forceinline__ u32x4_t load_chunk(const char* row, int c, int len) {
   constexpr int N = Vec<T>::N;
   u32x4_t out = {0u, 0u, 0u, 0u};
-  if (vec) {
-    if (c * N < len) out = *reinterpret_cast<const u32x4_t*>(row + c * N);
+  if constexpr (VEC) {
+    if (c * N < len) out = *reinterpret_cast<const u32x4_t*>(row + c * 16);
   } else {
+    const T* p = reinterpret_cast<const T*>(row);
     T x[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = c * N + i < len ? row[c * N + i] : (T)0.0f;
+    for (int i = 0; i < N; ++i) x[i] = c * N + i < len ? p[c * N + i] : (T)0.0f;
     __builtin_memcpy(&out, x, 16);
   }
   return out;
@@ -152,34 +153,31 @@ __device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NB][NT], const char*
   }
 }
 
-// ROWS rows of N elements, global -> registers -> LDS by NTHREADS threads; `row(i)` gives the address of tile row i
-template <typename T, int N, int ROWS, int NTHREADS>
+// ROWS rows of N elements, global -> registers -> LDS by NTHREADS threads.  Thread t handles rows row_of(k); their byte offsets from a base
+// that is uniform over the workgroup are 32-bit (one 64-bit scalar base per tile and one 32-bit lane offset per load).
+template <typename T, int N, int ROWS, int NTHREADS, bool VEC>
 struct Stage {
-  static constexpr int TOTAL = ROWS * Tile<T, N>::CHUNKS, PER = (TOTAL + NTHREADS - 1) / NTHREADS;
+  static constexpr int CH = Tile<T, N>::CHUNKS, TOTAL = ROWS * CH, PER = (TOTAL + NTHREADS - 1) / NTHREADS;
   u32x4_t v[PER];
-  template <typename RowF>
-  __device__ __forceinline__ void load(int tid, RowF row, int len, bool vec) {
+  static __device__ __forceinline__ int row_of(int tid, int k) { return (tid + k * NTHREADS) / CH; }
+  static __device__ __forceinline__ bool has(int tid, int k) { return TOTAL % NTHREADS == 0 || tid + k * NTHREADS < TOTAL; }
+  __device__ __forceinline__ void load(int tid, const char* base, const unsigned (&offset)[PER], int len) {
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int s = tid + k * NTHREADS;
-      if (TOTAL % NTHREADS == 0 || s < TOTAL) v[k] = load_chunk<T>(row(s / Tile<T, N>::CHUNKS), s % Tile<T, N>::CHUNKS, len, vec);
-    }
+    for (int k = 0; k < PER; ++k)
+      if (has(tid, k)) v[k] = load_chunk<T, VEC>(base + offset[k], (tid + k * NTHREADS) % CH, len);
   }
   __device__ __forceinline__ void store(int tid, char* tile) const {
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int s = tid + k * NTHREADS;
-      if (TOTAL % NTHREADS == 0 || s < TOTAL)
-        *reinterpret_cast<u32x4_t*>(tile + Tile<T, N>::offset(s / Tile<T, N>::CHUNKS, s % Tile<T, N>::CHUNKS)) = v[k];
-    }
+    for (int k = 0; k < PER; ++k)
+      if (has(tid, k)) *reinterpret_cast<u32x4_t*>(tile + Tile<T, N>::offset(row_of(tid, k), (tid + k * NTHREADS) % CH)) = v[k];
   }
 };
 
 // four consecutive elements of an output row (columns [col, col + 4) of which those below `len` exist)
-template <typename T>
-__device__ __forceinline__ void store4(T* row, int col, int len, f32x4 x, bool vec) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* row, int col, int len, f32x4 x) {
   typedef T V4 __attribute__((ext_vector_type(4)));
-  if (vec) {
+  if constexpr (VEC) {
     if (col < len) {
       V4 v;
 #pragma unroll
@@ -195,11 +193,29 @@ __device__ __forceinline__ void store4(T* row, int col, int len, f32x4 x, bool v
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
-// workgroup `id` of `total` -> position in the work list such that every XCD (id mod 8) gets one contiguous range of it: neighbours share
-// an XCD's L2
-__device__ __forceinline__ int xcd_order(int id, int total) {
-  const int x = id & 7, k = id >> 3, q = total >> 3, rem = total & 7;
-  return x * q + (x < rem ? x : rem) + k;
+// Order of a grid over `outer` independent problems of `units` workgroups each (units in the order they should start).  Consecutive workgroup
+// ids go to the 8 XCDs in turn; every XCD gets its own problems (neighbours share its L2).  With few problems per XCD the units of all of them
+// advance together, so that the heavy units of every problem start first; with many, problem after problem.
+__device__ __forceinline__ void grid_order(int id, int outer, int units, int& problem, int& unit) {
+  if (outer % 8 == 0) {
+    const int per = outer >> 3, x = id & 7, k = id >> 3;
+    if (per <= 4) {
+      unit = k / per;
+      problem = x * per + k - unit * per;
+    } else {
+      problem = k / units;
+      unit = k - problem * units;
+      problem += x * per;
+    }
+  } else if (outer <= 32) {
+    unit = id / outer;
+    problem = id - unit * outer;
+  } else {
+    const int total = outer * units, x = id & 7, k = id >> 3, q = total >> 3, rem = total & 7;
+    id = x * q + (x < rem ? x : rem) + k;
+    problem = id / units;
+    unit = id - problem * units;
+  }
 }
 
 }  // namespace is

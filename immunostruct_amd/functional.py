@@ -1898,7 +1898,7 @@ def _diff_forward(q, k, v, lam, lengths, causal, scale, need):
     work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     a = _lib.DiffAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(lengths), out.data_ptr(), _ptr(o2), _ptr(lse), _ptr(work),
                            None, None, None, None, None, None, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                           b, nq, nk, heads, hk, d, dv, causal, _lib.TYPES[q.dtype], _lib.TYPES[lam.dtype], splits, 0, 0, scale)
+                           b, nq, nk, heads, hk, d, dv, causal, _lib.TYPES[q.dtype], _lib.TYPES[lam.dtype], splits, 1, 0, 0, 0, 0, scale)
     _enqueue("is_diff_attention_fwd", lib.is_diff_attention_fwd, q.get_device(), ctypes.byref(a))
     return out, o2, lse, a
 
@@ -1908,7 +1908,7 @@ class DifferentialAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lam, lengths, causal, scale):
-        q, k, v, lam = (_lib.last_contiguous(t) for t in (q, k, v, lam))
+        q, k, v, lam = _lib.sequence_rows(q), _lib.sequence_rows(k), _lib.sequence_rows(v), lam.contiguous()
         out, o2, lse, ctx.args = _diff_forward(q, k, v, lam, lengths, causal, scale, True)
         ctx.save_for_backward(q, k, v, lam, lengths, out, o2, lse)
         return out
@@ -1922,10 +1922,14 @@ class DifferentialAttentionFn(torch.autograd.Function):
         if ctx.args is None:
             return dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), None, None, None
         g = g.contiguous()
-        dots = torch.empty_like(lse)
         a = _lib.DiffAttention.from_buffer_copy(ctx.args)      # (the forward's arguments with this call's buffers; its workspace is gone)
-        a.work, a.splits = None, 1
-        a.d_o, a.dots, a.dq, a.dk, a.dv_out, a.dlam = (t.data_ptr() for t in (g, dots, dq, dk, dv, dlam))
+        b, hk, _, rows = lse.shape
+        a.splits, a.row_splits = 1, lib.is_diff_attention_row_splits(b, hk, rows, a.nk, a.causal)
+        floats = lib.is_diff_attention_row_work_floats(b, hk, a.nk, a.d, a.dv, a.row_splits)
+        # (scratch for the rows' three dot products, behind the row splits' sums)
+        work = torch.empty(floats + 3 * b * hk * rows, dtype=torch.float32, device=q.device)
+        a.work, dots = work.data_ptr(), work.data_ptr() + 4 * floats
+        a.d_o, a.dots, a.dq, a.dk, a.dv_out, a.dlam = g.data_ptr(), dots, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr()
         _enqueue("is_diff_attention_bwd", lib.is_diff_attention_bwd, q.get_device(), ctypes.byref(a))
         return dq, dk, dv, dlam, None, None, None
 
@@ -1961,7 +1965,7 @@ def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
         raise NotImplementedError(f"differential_attention: heads of {d} / values of {dv} elements (the kernels: up to {limit} / {2 * limit} in {q.dtype})")
     _lib.same_device(q, k, v, lam, lengths)
     if not _needs_grad(q, k, v, lam):
-        return _diff_forward(*(_lib.last_contiguous(t) for t in (q, k, v, lam)), lengths, _CAUSAL[causal], scale, False)[0]
+        return _diff_forward(_lib.sequence_rows(q), _lib.sequence_rows(k), _lib.sequence_rows(v), lam.contiguous(), lengths, _CAUSAL[causal], scale, False)[0]
     return DifferentialAttentionFn.apply(q, k, v, lam, lengths, _CAUSAL[causal], scale)
 
 

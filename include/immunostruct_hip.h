@@ -449,8 +449,10 @@ int is_rotary(const void* q, long long q_b, long long q_n, long long q_h, void* 
  * is_diff_attention_fwd: reads q, k, v, lam, lengths; writes o (batch, nq, heads, dv); lse (batch, kv_heads, 2, nq heads / kv_heads; fp32) and
  *   o2 (like o: the second map's product) are what the backward needs, both or neither.  splits = is_diff_attention_splits(...) ranges of
  *   the keys per row (1: none); splits > 1 needs work[is_diff_attention_work_floats(...)] (rows = nq heads / kv_heads in both).
- * is_diff_attention_bwd: reads those and d_o (contiguous); writes dq, dk, dv_out (contiguous), dlam (lam's type); dots: scratch of lse's
- *   size.  group and vec are set by the library.  No atomics: bitwise reproducible.                                                  */
+ * is_diff_attention_bwd: reads those and d_o (contiguous); writes dq, dk, dv_out (contiguous), dlam (lam's type); dots: scratch of 1.5
+ *   times lse's size; row_splits = is_diff_attention_row_splits(...) parts of the rows per key tile (1: none), more than one need
+ *   work[is_diff_attention_row_work_floats(...)].  rows, group, vec and group_magic are set by the library.  Row strides below 2^31 / 64
+ *   bytes.  No atomics: bitwise reproducible.                                                                                         */
 typedef struct {
   const void *q, *k, *v, *lam;
   const int* lengths;
@@ -460,11 +462,14 @@ typedef struct {
   float* dots;
   void *dq, *dk, *dv_out, *dlam;
   long long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
-  int batch, nq, nk, heads, kv_heads, d, dv, causal, type, lam_type, splits, group, vec;
+  int batch, nq, nk, heads, kv_heads, d, dv, causal, type, lam_type, splits, row_splits, rows, group, vec;
+  unsigned group_magic;
   float scale;
 } IsDiffAttention;
 int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk);
 long long is_diff_attention_work_floats(int batch, int kv_heads, int rows, int dv, int splits);
+int is_diff_attention_row_splits(int batch, int kv_heads, int rows, int nk, int causal);
+long long is_diff_attention_row_work_floats(int batch, int kv_heads, int nk, int d, int dv, int row_splits);
 int is_diff_attention_fwd(const IsDiffAttention* args, void* stream);
 int is_diff_attention_bwd(const IsDiffAttention* args, void* stream);
 

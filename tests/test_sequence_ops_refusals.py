@@ -70,11 +70,12 @@ def test_entry_points_refuse_without_a_device():
     assert lib.is_diff_attention_fwd(None, None) == -22 and lib.is_diff_attention_bwd(None, None) == -22
     assert lib.is_group_norm_fwd(None, None) == -22 and lib.is_group_norm_bwd(None, None) == -22
     p = 4096      # (never dereferenced: every call below is refused)
-    good = dict(q=p, k=p, v=p, lam=p, o=p, batch=1, nq=1, nk=1, heads=2, kv_heads=1, d=8, dv=8, causal=0, type=0, lam_type=0, splits=1, scale=1.0)
+    good = dict(q=p, k=p, v=p, lam=p, o=p, batch=1, nq=1, nk=1, heads=2, kv_heads=1, d=8, dv=8, causal=0, type=0, lam_type=0, splits=1, row_splits=1, scale=1.0)
     for change, code in ((dict(q=None), -22), (dict(batch=0), -22), (dict(kv_heads=3), -22), (dict(type=3), -22), (dict(lam_type=1), -22),
                          (dict(causal=3), -22), (dict(scale=0.0), -22), (dict(splits=0), -22), (dict(splits=2), -22), (dict(lse=p), -22),
                          (dict(d=65), -38), (dict(dv=129), -38), (dict(type=1, lam_type=1, d=129), -38), (dict(nq=2 ** 31 - 1), -22),
-                         (dict(batch=2 ** 31 - 1, kv_heads=2), -22)):
+                         (dict(batch=2 ** 31 - 1, kv_heads=2), -22),
+                         (dict(k_n=2 ** 24), -22), (dict(q_n=-1), -22)):
         assert lib.is_diff_attention_fwd(ctypes.byref(_lib.DiffAttention(**dict(good, **change))), None) == code, change
     assert lib.is_diff_attention_bwd(ctypes.byref(_lib.DiffAttention(**good)), None) == -22      # nothing saved
     norm = dict(x=p, y=p, stats=p, batch=1, n=1, channels=8, groups=2, eps=1e-5)
@@ -96,6 +97,9 @@ def test_splits_cover_the_chip():
     assert lib.is_diff_attention_splits(1, 1, 1, 100) == 1 and lib.is_diff_attention_splits(1, 1, 1, 2 ** 20) == 64
     assert lib.is_diff_attention_work_floats(16, 4, 4, 128, 1) == 0
     assert lib.is_diff_attention_work_floats(16, 4, 4, 128, 16) == 2 * 16 * 4 * 16 * 4 * 130
+    assert lib.is_diff_attention_row_splits(2, 4, 16384, 4096, 1) == 2 and lib.is_diff_attention_row_splits(2, 4, 16384, 4096, 0) == 1
+    assert lib.is_diff_attention_row_splits(1, 1, 4096, 128, 0) == 16 and lib.is_diff_attention_row_splits(1, 1, 100, 128, 1) == 1
+    assert lib.is_diff_attention_row_work_floats(2, 4, 100, 64, 128, 2) == 2 * 2 * 4 * 100 * 256
 
 
 def test_rotary_frequencies():
