@@ -6,10 +6,16 @@
 //   visible   key j < end(i): end = len (no mask), min(len, i + 1) ("start") or len - nq + 1 + i ("end").  Keys at or behind len are never
 //             read (their rows are clamped to the last valid one and their scores replaced), so anything may stand there.
 //             A row that sees nothing gives 0, lse = +inf, and no gradient.
-//   forward   one pass over the keys: S^T = K Q^T (a lane owns one query), running maximum and sum per map in 32 bits, O^T += V^T P^T for
-//             both maps from ONE transposed read of V.  The maximum only moves when a score passes it by 2^8 (the weights stay <= 2^8, far
-//             inside every type), which makes the rescaling of the two accumulators rare.
-//   backward  dP = dO V^T is shared by the maps; D_m = dO . O_m; dS_1 = P1 (dP - D_1), dS_2 = -lam P2 (dP - D_2);
+//   waves     a wave works on 32 rows (or 32 keys) of ONE map; two neighbouring waves hold the two maps of the same rows and meet once at the end,
+//             lane to lane through LDS.  That halves a wave's registers (one accumulator set, one resident operand), so that two to four
+//             waves share a SIMD and hide each other's latencies.  The forward repeats nothing by it; the backward computes dP = dO V^T
+//             and the product with dO once per map (48 matrix instructions per 32 x 32 tile at d = 64 for 32) and is still far ahead:
+//             with both maps in one wave dK / dV took 849 us at (2, 4096, 16 / 4 heads, 64 / 128, bf16, causal), one wave per SIMD.
+//   forward   one pass over the keys: S^T = K Q^T (a lane owns one query), running maximum and sum in 32 bits, O^T += V^T P^T.
+//             The weights are formed with the old maximum first; only when a lane's 16 add up to more than 2^10 (far inside every type)
+//             the tile's maximum is looked for and the accumulators are rescaled: two thirds of the vector work of a tile is then
+//             the exponentials themselves, which bound the kernel beside the matrix instructions.
+//   backward  dP = dO V^T; D_m = dO . O_m; dS_1 = P1 (dP - D_1), dS_2 = -lam P2 (dP - D_2);
 //             dQ_m = scale dS_m K_m, dK_m = scale dS_m^T Q_m, dV = (P1 - lam P2)^T dO, dlam = -sum D_2.  Scores are recomputed from lse.
 //             dK / dV: a wave owns 32 keys and walks the rows; dQ: a wave owns 32 rows and walks the keys.
 // Scores, sums, lse, D and all accumulators are 32-bit; P and dS are rounded once to the inputs' type for the matrix instructions.
@@ -21,7 +27,25 @@ namespace is {
 namespace da {
 
 typedef IsDiffAttention Args;
-constexpr float SLACK = 8.0f;      // log2 of how far a weight may pass 1 before the running maximum follows
+constexpr float SLACK = 1024.0f;      // how far a lane's 16 weights may add up before the running maximum follows
+
+template <int V> struct Int { static constexpr int value = V; };
+// steps j0 = first, first + STEP ... below last, alternating between two buffers whose number is a compile-time constant
+// (LDS addresses then are loop-invariant registers plus immediates)
+template <int STEP, typename F>
+__device__ __forceinline__ void two_buffers(int first, int last, F step) {
+  for (int j0 = first; j0 < last; j0 += 2 * STEP) {
+    step(j0, Int<0>());
+    if (j0 + STEP < last) step(j0 + STEP, Int<1>());
+  }
+}
+
+// Row (key) groups of a workgroup: two waves each.  More groups share a staged tile, fewer let the workgroups of a CU drift apart, so that one
+// multiplies while another forms weights.  Measured at (2, 4096, 16 / 4 heads, 64 / 128, bf16, causal) for 2 / 4 groups: forward 284 / 317 us,
+// dK / dV 610 / 550, dQ 378 / 368; at (5, 517 x 1531, 6 / 2 heads, 128 / 256, fp16): forward 120 / 108, dQ 85 / 89, dK / dV two only (registers).
+template <typename T, int D> constexpr int fwd_groups() { return D * sizeof(T) <= 128 ? 2 : 4; }
+template <typename T, int D> constexpr int key_groups() { return D * sizeof(T) <= 128 ? 4 : 2; }
+template <typename T, int D> constexpr int dq_groups() { return D * sizeof(T) <= 128 ? 4 : 2; }
 
 template <typename T>
 __device__ __forceinline__ float lam_at(const Args& a, int head) {
@@ -57,42 +81,82 @@ __device__ __forceinline__ int query_of(const Args& a, int r, int& g) {
 // element (b, query i, head h) of a contiguous (batch, nq, heads, dv) tensor
 __device__ __forceinline__ long long o_at(const Args& a, int b, int i, int h) { return (((long long)b * a.nq + i) * a.heads + h) * a.dv; }
 
-// byte offsets of a tile's key rows j0 + row_of(k), clamped to the last valid one, from row j0
-template <typename S>
-__device__ __forceinline__ void key_offsets(unsigned (&out)[S::PER], int tid, unsigned stride, int left) {
-#pragma unroll
-  for (int k = 0; k < S::PER; ++k) out[k] = (unsigned)min(S::row_of(tid, k), left) * stride;
-}
-// byte offsets of a tile's packed rows r0 + row_of(k), clamped to the last one, from query r0 / group and the group's first head
-template <typename S>
-__device__ __forceinline__ void row_offsets(const Args& a, unsigned (&out)[S::PER], int tid, int r0, int first, unsigned stride, unsigned head) {
+// The two maps' rows of a tile lie behind each other: tile rows [0, n) are map 0's, [n, 2 n) map 1's (MAPS = 2; 1: values, one set).
+// byte offsets of a tile's key rows, clamped to the last valid one, from its first row
+template <typename S, int MAPS>
+__device__ __forceinline__ void key_offsets(unsigned (&out)[S::PER], int tid, unsigned stride, unsigned map, int left) {
+  constexpr int N = S::ROWS_ / MAPS;
 #pragma unroll
   for (int k = 0; k < S::PER; ++k) {
+    const int row = S::row_of(tid, k);
+    out[k] = (unsigned)min(row & (N - 1), left) * stride + (row >= N ? map : 0u);
+  }
+}
+// byte offsets of a tile's packed rows, clamped to the last one, from query r0 / group and the group's first head
+template <typename S, int MAPS>
+__device__ __forceinline__ void row_offsets(const Args& a, unsigned (&out)[S::PER], int tid, int r0, int first, unsigned stride, unsigned head, unsigned map) {
+  constexpr int N = S::ROWS_ / MAPS;
+#pragma unroll
+  for (int k = 0; k < S::PER; ++k) {
+    const int row = S::row_of(tid, k);
     int g;
-    const int i = query_of(a, min(r0 + S::row_of(tid, k), a.rows - 1), g);
-    out[k] = (unsigned)(i - first) * stride + (unsigned)g * head;
+    const int i = query_of(a, min(r0 + (row & (N - 1)), a.rows - 1), g);
+    out[k] = (unsigned)(i - first) * stride + (unsigned)g * head + (row >= N ? map : 0u);
+  }
+}
+// Hands the wave of map 1's accumulators to the wave of map 0 of the same rows: f(t, own, other) runs in map 0's lanes with both values of
+// 32-column block t (f32x16 each).  `lds`: BYTES of scratch; every wave of the workgroup takes part.
+template <int NT, int GROUPS, int BYTES, typename F>
+__device__ __forceinline__ void hand_over(const f32x16 (&acc)[NT], char* lds, int group, int map, int lane, F f) {
+  constexpr int FIT = BYTES / (GROUPS * 4096), STEP = FIT < NT ? FIT : NT;
+  static_assert(STEP >= 1, "one block of every group has to fit");
+  f32x4* mine = reinterpret_cast<f32x4*>(lds) + group * 256 + lane;
+#pragma unroll
+  for (int t0 = 0; t0 < NT; t0 += STEP) {
+    __syncthreads();
+    if (map == 1) {
+#pragma unroll
+      for (int t = t0; t < t0 + STEP && t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mine[(t - t0) * GROUPS * 256 + u * 64] = f32x4{acc[t][4 * u], acc[t][4 * u + 1], acc[t][4 * u + 2], acc[t][4 * u + 3]};
+    }
+    __syncthreads();
+    if (map == 0) {
+#pragma unroll
+      for (int t = t0; t < t0 + STEP && t < NT; ++t) {
+        f32x16 other;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f32x4 x = mine[(t - t0) * GROUPS * 256 + u * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) other[4 * u + e] = x[e];
+        }
+        f(t, acc[t], other);
+      }
+    }
   }
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
-// grid: (row tiles x splits x kv_heads x batch), NW waves of 32 rows.  splits > 1: every workgroup takes one range of the keys and leaves
-// unnormalised sums with their maxima in the workspace; join_kernel puts them together.
-template <typename T, int D, int NW, bool VEC>
-__global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kernel(const Args a) {
-  constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 64 * NW, SZ = sizeof(T);
+// grid: (row tiles x splits x kv_heads x batch), GROUPS x 2 waves of 32 rows and one map.  splits > 1: every workgroup takes one range of the
+// keys and leaves unnormalised sums with their maxima in the workspace; join_kernel puts them together.
+template <typename T, int D, int GROUPS, bool VEC>
+__global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2))) void fwd_kernel(const Args a) {
+  constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 128 * GROUPS, SZ = sizeof(T);
   constexpr int KB = Tile<T, D>::bytes(KT), VB = Tile<T, DV>::bytes(KT), BUF = 2 * KB + VB;
   __shared__ __align__(16) char lds[2 * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, g = lane >> 5;
-  const int R = a.rows, tiles = (R + 32 * NW - 1) / (32 * NW);
+  const int group = wave >> 1, map = wave & 1;
+  const int R = a.rows, tiles = (R + 32 * GROUPS - 1) / (32 * GROUPS);
   int base, unit;
   grid_order(blockIdx.x, a.batch * a.kv_heads, tiles * a.splits, base, unit);
   const int split = unit % a.splits, tile = tiles - 1 - unit / a.splits;      // the rows that see most keys first
   const int b = base / a.kv_heads, hk = base - b * a.kv_heads;
   const int len = length_of(a, b);
-  const int row0 = tile * 32 * NW + wave * 32, r = row0 + qi, rr = r < R ? r : R - 1;
+  const int row0 = (tile * GROUPS + group) * 32, r = row0 + qi, rr = r < R ? r : R - 1;
   int gi;
   const int query = query_of(a, rr, gi), head = hk * a.group + gi;
-  const int wg_end = end_of(a, (min(tile * 32 * NW + 32 * NW, R) - 1) / a.group, len);
+  const int wg_end = end_of(a, (min((tile + 1) * GROUPS * 32, R) - 1) / a.group, len);
   const int my_end = r < R ? end_of(a, query, len) : 0;
   const int wave_end = row0 < R ? end_of(a, min(row0 + 31, R - 1) / a.group, len) : 0;      // no row of the wave sees further
   const int wave_all = row0 + 31 < R ? end_of(a, row0 / a.group, len) : 0;                  // every row of the wave sees this far
@@ -100,145 +164,141 @@ __global__ __launch_bounds__(64 * NW, (D <= 64 && NW > 1 ? 2 : 1)) void fwd_kern
   const int first = split * per, last = min(wg_end, first + per);
   const float c = a.scale * 1.44269504088896340736f;
 
-  u32x4_t q[2][NJ];
-  const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + 2 * head * a.q_h) * SZ;
+  u32x4_t q[NJ];
+  const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + (2 * head + map) * a.q_h) * SZ;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) q[m][j] = load_chunk<T, VEC>(qp + m * a.q_h * SZ, 2 * j + g, a.d);
-  f32x16 o[2][NT];
-  zero_acc2(o);
-  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  for (int j = 0; j < NJ; ++j) q[j] = load_chunk<T, VEC>(qp, 2 * j + g, a.d);
+  const int k_at = map * KB + Tile<T, D>::rows_at(lane), v_at = 2 * KB + Tile<T, DV>::columns_at(lane);
+  f32x16 o[NT];
+  zero_acc(o);
+  float top = -INFINITY, ref = 0.0f, sum = 0.0f;      // ref: what the exponents are taken against (-top c; 0 before the first key)
 
-  typedef Stage<T, D, KT, NTH, VEC> StageK;
+  typedef Stage<T, D, 2 * KT, NTH, VEC> StageK;
   typedef Stage<T, DV, KT, NTH, VEC> StageV;
-  StageK sk0, sk1;
+  StageK sk;
   StageV sv;
   const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + 2 * hk * a.k_h) * SZ;
   const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + hk * a.v_h) * SZ;
   auto fetch = [&](int j0) {
     unsigned ko[StageK::PER], vo[StageV::PER];
-    key_offsets<StageK>(ko, tid, (unsigned)a.k_n * SZ, len - 1 - j0);
-    key_offsets<StageV>(vo, tid, (unsigned)a.v_n * SZ, len - 1 - j0);
-    const char* k = kp + j0 * a.k_n * SZ;
-    sk0.load(tid, k, ko, a.d);
-    sk1.load(tid, k + a.k_h * SZ, ko, a.d);
+    key_offsets<StageK, 2>(ko, tid, (unsigned)a.k_n * SZ, (unsigned)a.k_h * SZ, len - 1 - j0);
+    key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, len - 1 - j0);
+    sk.load(tid, kp + j0 * a.k_n * SZ, ko, a.d);
     sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
   auto place = [&](char* buf) {
-    sk0.store(tid, buf);
-    sk1.store(tid, buf + KB);
+    sk.store(tid, buf);
     sv.store(tid, buf + 2 * KB);
   };
   if (first < last) {      // (uniform over the workgroup, as is every barrier below)
     fetch(first);
     place(lds);
     __syncthreads();
-    int cur = 0;
-    for (int j0 = first; j0 < last; j0 += KT) {
+    two_buffers<KT>(first, last, [&](int j0, auto which) {
+      constexpr int CUR = decltype(which)::value;
+      const char* buf = lds + CUR * BUF;
       const bool more = j0 + KT < last;
       if (more) fetch(j0 + KT);
       if (j0 < wave_end) {
-        const char* buf = lds + cur * BUF;
-        f32x16 p[2];
-        zero_acc(p);
-        mm_tile<T, D>(p[0], buf, 0, q[0], lane);
-        mm_tile<T, D>(p[1], buf + KB, 0, q[1], lane);
-        if (j0 + KT > wave_all) {
+        f32x16 p = mm_tile<T, D>(buf + k_at, q);
+        auto hide = [&]() {
+          if (j0 + KT > wave_all) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) p[t] = j0 + tile_row(t, g) >= my_end ? -INFINITY : p[t];
+          }
+        };
+        float add;
+        auto weights = [&]() {
+          add = 0.0f;
 #pragma unroll
           for (int t = 0; t < 16; ++t) {
-            const bool hidden = j0 + tile_row(t, g) >= my_end;
-            p[0][t] = hidden ? -INFINITY : p[0][t];
-            p[1][t] = hidden ? -INFINITY : p[1][t];
+            p[t] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t], c, ref));
+            add += p[t];
           }
+        };
+        hide();
+        weights();
+        if (__any(add > SLACK || top == -INFINITY)) {      // (rare: the scores are formed again rather than kept)
+          p = mm_tile<T, D>(buf + k_at, q);
+          hide();
+          float high = p[0];
+#pragma unroll
+          for (int t = 1; t < 16; ++t) high = fmaxf(high, p[t]);
+          const float now = fmaxf(top, fmaxf(high, other_half(high)));
+          const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - now) * c);
+          top = now;
+          ref = now == -INFINITY ? 0.0f : -now * c;
+          sum *= shrink;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[t][e] *= shrink;
+          weights();
         }
-        float high[2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          float x = p[m][0];
-#pragma unroll
-          for (int t = 1; t < 16; ++t) x = fmaxf(x, p[m][t]);
-          high[m] = fmaxf(x, other_half(x));
-        }
-        if (__any((high[0] - top[0]) * c > SLACK || (high[1] - top[1]) * c > SLACK)) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const float now = fmaxf(top[m], high[m]), ref = now == -INFINITY ? 0.0f : now;
-            const float shrink = __builtin_amdgcn_exp2f((top[m] - ref) * c);
-            top[m] = now;
-            sum[m] *= shrink;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[m][t][e] *= shrink;
-          }
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const float ref = top[m] == -INFINITY ? 0.0f : -top[m] * c;
-          float s = 0.0f;
-#pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            p[m][t] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[m][t], c, ref));
-            s += p[m][t];
-          }
-          sum[m] += s;
-        }
-        mm_transposed<T, DV, NT, 2>(o, buf + 2 * KB, 0, p, lane);
+        sum += add;
+        mm_transposed<T, DV, NT>(o, buf + v_at, p);
       }
       if (more) {
-        place(lds + (cur ^ 1) * BUF);
+        place(lds + (CUR ^ 1) * BUF);
         __syncthreads();
-        cur ^= 1;
       }
-    }
+    });
   }
-  float total[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) total[m] = sum[m] + other_half(sum[m]);
-  if (r >= R) return;
+  const float total = sum + other_half(sum);
+  const bool live = r < R;
   if (a.splits > 1) {
-    float* w = a.work + ((long long)base * a.splits + split) * (2 * (long long)R * (a.dv + 2));
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      float* wm = w + (m * (long long)R + r) * (a.dv + 2);
-      if (g == 0) {
-        wm[a.dv] = top[m] == -INFINITY ? -INFINITY : top[m] * c;
-        wm[a.dv + 1] = total[m];
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          store4<float, false>(wm, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[m][t][4 * u], o[m][t][4 * u + 1], o[m][t][4 * u + 2], o[m][t][4 * u + 3]});
+    if (!live) return;
+    float* w = a.work + (((long long)base * a.splits + split) * 2 + map) * ((long long)R * (a.dv + 2)) + (long long)r * (a.dv + 2);
+    if (g == 0) {
+      w[a.dv] = top == -INFINITY ? -INFINITY : top * c;
+      w[a.dv + 1] = total;
     }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        store4<float, false>(w, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[t][4 * u], o[t][4 * u + 1], o[t][4 * u + 2], o[t][4 * u + 3]});
     return;
   }
-  const float lam = lam_at<T>(a, head);
-  const float w0 = total[0] != 0.0f ? 1.0f / total[0] : 0.0f, w1 = total[1] != 0.0f ? 1.0f / total[1] : 0.0f;
-  if (a.lse != nullptr && g == 0) {
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-      a.lse[((long long)base * 2 + m) * R + r] = total[m] != 0.0f ? __builtin_fmaf(top[m], c, __log2f(total[m])) : INFINITY;
-  }
-  T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, query, head);
-  T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, query, head);
+  const float inv = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      f32x4 x, y;
+    for (int e = 0; e < 16; ++e) o[t][e] *= inv;
+  if (a.lse != nullptr && live && g == 0) a.lse[((long long)base * 2 + map) * R + r] = total != 0.0f ? __builtin_fmaf(top, c, __log2f(total)) : INFINITY;
+  const long long at = o_at(a, b, query, head);
+  if (a.o2 != nullptr && live && map == 1) {
+    T* out2 = reinterpret_cast<T*>(a.o2) + at;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = o[1][t][4 * u + e] * w1;
-        x[e] = o[0][t][4 * u + e] * w0 - lam * y[e];
-      }
-      store4<T, VEC>(out, 32 * t + 8 * u + 4 * g, a.dv, x);
-      if (a.o2 != nullptr) store4<T, VEC>(out2, 32 * t + 8 * u + 4 * g, a.dv, y);
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        store4<T, VEC>(out2, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[t][4 * u], o[t][4 * u + 1], o[t][4 * u + 2], o[t][4 * u + 3]});
+  }
+  const float lam = lam_at<T>(a, head);
+  T* out = reinterpret_cast<T*>(a.o) + at;
+  hand_over<NT, GROUPS, 2 * BUF>(o, lds, group, map, lane, [&](int t, const f32x16& x, const f32x16& y) {
+    if (!live) return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f32x4 z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = x[4 * u + e] - lam * y[4 * u + e];
+      store4<T, VEC>(out, 32 * t + 8 * u + 4 * g, a.dv, z);
     }
+  });
 }
 
-// the splits of one row put together: one wave per row, lane = column
+__device__ __forceinline__ float wave_max(float v) {
+  v = max_over_r(v);
+  return fmaxf(v, other_half(v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = sum_over_r(v);
+  return v + other_half(v);
+}
+
+// the splits of one row put together: one wave per row; lane = split for the maxima and sums (at most 64 splits), then lane = column
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const int R = a.rows, lane = threadIdx.x & 63;
@@ -248,58 +308,69 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
   int gi;
   const int query = query_of(a, r, gi), head = hk * a.group + gi;
-  float inv[2], top[2], total[2];
   const long long step = 2 * (long long)R * (a.dv + 2);
   const float* from[2];
+  float weight[2];
+#pragma unroll
   for (int m = 0; m < 2; ++m) {
     from[m] = a.work + base * a.splits * step + (m * (long long)R + r) * (a.dv + 2);
-    top[m] = -INFINITY;
-    total[m] = 0.0f;
-    for (int s = 0; s < a.splits; ++s) top[m] = fmaxf(top[m], from[m][s * step + a.dv]);
-    const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-    for (int s = 0; s < a.splits; ++s) total[m] += from[m][s * step + a.dv + 1] * __builtin_amdgcn_exp2f(from[m][s * step + a.dv] - ref);
-    inv[m] = total[m] != 0.0f ? 1.0f / total[m] : 0.0f;
-    if (a.lse != nullptr && lane == 0) a.lse[(base * 2 + m) * R + r] = total[m] != 0.0f ? top[m] + __log2f(total[m]) : INFINITY;
+    float top = -INFINITY, sum = 0.0f;
+    if (lane < a.splits) {
+      top = from[m][lane * step + a.dv];
+      sum = from[m][lane * step + a.dv + 1];
+    }
+    const float high = wave_max(top), ref = high == -INFINITY ? 0.0f : high;
+    weight[m] = __builtin_amdgcn_exp2f(top - ref);
+    const float total = wave_sum(sum * weight[m]);
+    weight[m] *= total != 0.0f ? 1.0f / total : 0.0f;
+    if (a.lse != nullptr && lane == 0) a.lse[(base * 2 + m) * R + r] = total != 0.0f ? high + __log2f(total) : INFINITY;
   }
   const float lam = lam_at<T>(a, head);
   T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, query, head);
   T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, query, head);
-  for (int col = lane; col < a.dv; col += 64) {
-    float x[2];
-    for (int m = 0; m < 2; ++m) {
-      const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-      float acc = 0.0f;
-      for (int s = 0; s < a.splits; ++s) acc += from[m][s * step + col] * __builtin_amdgcn_exp2f(from[m][s * step + a.dv] - ref);
-      x[m] = acc * inv[m];
+  for (int c0 = 0; c0 < a.dv; c0 += 64) {      // (uniform: the weights travel between lanes)
+    const int col = min(c0 + lane, a.dv - 1);
+    float x = 0.0f, y = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) {
+      x += from[0][s * step + col] * __shfl(weight[0], s);
+      y += from[1][s * step + col] * __shfl(weight[1], s);
     }
-    out[col] = (T)(x[0] - lam * x[1]);
-    if (a.o2 != nullptr) out2[col] = (T)x[1];
+    if (c0 + lane < a.dv) {
+      out[col] = (T)(x - lam * y);
+      if (a.o2 != nullptr) out2[col] = (T)y;
+    }
   }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
-// D_2 = dO . O_2 and D_1 = dO . O + lam D_2 of every row (one wave per row)
-template <typename T>
+// D_2 = dO . O_2 and D_1 = dO . O + lam D_2 of every row (16 lanes per row)
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
-  const int R = a.rows, lane = threadIdx.x & 63;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int N = Vec<T>::N;
+  const int R = a.rows, lane = threadIdx.x & 15;
+  const long long w = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
   if (w >= (long long)a.batch * a.kv_heads * R) return;
   const long long base = w / R;
   const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
   int gi;
   const int query = query_of(a, r, gi), head = hk * a.group + gi;
-  const long long at = o_at(a, b, query, head);
-  const T *o = reinterpret_cast<const T*>(a.o) + at, *o2 = reinterpret_cast<const T*>(a.o2) + at, *go = reinterpret_cast<const T*>(a.d_o) + at;
+  const long long at = o_at(a, b, query, head) * sizeof(T);
+  const char *o = reinterpret_cast<const char*>(a.o) + at, *o2 = reinterpret_cast<const char*>(a.o2) + at, *go = reinterpret_cast<const char*>(a.d_o) + at;
   float s = 0.0f, s2 = 0.0f;
-  for (int col = lane; col < a.dv; col += 64) {
-    const float x = (float)go[col];
-    s += x * (float)o[col];
-    s2 += x * (float)o2[col];
+  for (int c = lane; c * N < a.dv; c += 16) {
+    float x[N], y[N], y2[N];
+    Vec<T>::unpack(load_chunk<T, VEC>(go, c, a.dv), x);
+    Vec<T>::unpack(load_chunk<T, VEC>(o, c, a.dv), y);
+    Vec<T>::unpack(load_chunk<T, VEC>(o2, c, a.dv), y2);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      s += x[e] * y[e];
+      s2 += x[e] * y2[e];
+    }
   }
-  s = sum_over_r(s);
-  s2 = sum_over_r(s2);
-  s += other_half(s);
-  s2 += other_half(s2);
+  s = sum_over_r16(s);
+  s2 = sum_over_r16(s2);
   if (lane == 0) {
     a.dots[(base * 2) * R + r] = s + lam_at<T>(a, head) * s2;
     a.dots[(base * 2 + 1) * R + r] = s2;
@@ -329,29 +400,34 @@ __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
   }
 }
 
-// dK, dV of 32 keys per wave: grid (key tiles x row splits x kv_heads x batch).  row_splits > 1: the rows that see a key tile are cut into equal
-// parts, whose sums meet in the workspace (key_join_kernel): with a causal mask the first keys are seen by all rows and the last by few, and a
-// workgroup of 512-register waves is alone on its CU, so one workgroup per key tile would leave half the chip idle half the time.
+// dK, dV of 32 keys per wave: grid (key tiles x row splits x kv_heads x batch), GROUPS x 2 waves.  row_splits > 1: the rows that see a key tile
+// are cut into equal parts, whose sums meet in the workspace (key_join_kernel): with a causal mask the first keys are seen by all rows and
+// the last by few, and one workgroup per key tile would leave half the chip idle half the time.
+// Map m's weight with its sign: P_1, -lam P_2; both waves run the same code on (lse, D, coefficient).
 template <typename T, int D, bool VEC>
-__global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
-  constexpr int DV = 2 * D, RT = 32, NT = D / 32, NTV = DV / 32, NJ = D / (2 * Vec<T>::N), NJV = DV / (2 * Vec<T>::N), SZ = sizeof(T);
+__global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) <= 128 ? 2 : 1))) void dkv_kernel(const Args a) {
+  constexpr int GROUPS = key_groups<T, D>(), NTH = 128 * GROUPS, KEYS = 32 * GROUPS;
+  constexpr int DV = 2 * D, RT = 32, NT = D / 32, NTV = DV / 32, NJ = D / (2 * Vec<T>::N), SZ = sizeof(T);
   constexpr int QB = Tile<T, D>::bytes(RT), OB = Tile<T, DV>::bytes(RT), BUF = 2 * QB + OB;
-  __shared__ __align__(16) char lds[2 * BUF];
-  __shared__ __align__(16) float stat[2][5][RT];      // lse1, lse2, D1, D2, lam of the tile's rows
+  __shared__ __align__(16) char lds[2 * BUF], vt[Tile<T, DV>::bytes(KEYS)];      // row tiles; the workgroup's own values
+  __shared__ __align__(16) float stat[2][2][3][RT];      // [buffer][map][lse, D, coefficient] of the tile's rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ki = lane & 31, g = lane >> 5;
-  const int R = a.rows, tiles = (a.nk + 127) / 128;
+  const int group = wave >> 1, map = wave & 1;
+  const int R = a.rows, tiles = (a.nk + KEYS - 1) / KEYS;
   int base, unit;
   grid_order(blockIdx.x, a.batch * a.kv_heads, tiles * a.row_splits, base, unit);
   const int split = unit % a.row_splits, tile = unit / a.row_splits;      // the keys that most rows see first
   const int b = base / a.kv_heads, hk = base - b * a.kv_heads;
   const int len = length_of(a, b);
-  const int wg_key = tile * 128, key0 = wg_key + wave * 32, key = key0 + ki;
+  const int wg_key = tile * KEYS, key0 = wg_key + group * 32, key = key0 + ki;
   const float c = a.scale * 1.44269504088896340736f;
-  u32x4_t k[2][NJ], v[NJV];
-  f32x16 dk0[1][NT], dk1[1][NT], dv[1][NTV];
-  zero_acc2(dk0);
-  zero_acc2(dk1);
-  zero_acc2(dv);
+  u32x4_t k[NJ];
+  const int q_at = map * QB + Tile<T, D>::rows_at(lane), g_at = 2 * QB + Tile<T, DV>::rows_at(lane);
+  const int qt_at = map * QB + Tile<T, D>::columns_at(lane), gt_at = 2 * QB + Tile<T, DV>::columns_at(lane);
+  const char* own = vt + Tile<T, DV>::bytes(32) * group + Tile<T, DV>::rows_at(lane);
+  f32x16 dk[NT], dv[NTV];
+  zero_acc(dk);
+  zero_acc(dv);
   const int seen_from = wg_key < len ? first_query(a, wg_key, len) * a.group / RT * RT : R;
   const int per = ((R - seen_from + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
   const int r_first = seen_from + split * per, r_last = min(R, r_first + per);
@@ -359,18 +435,20 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
   const int wave_all = key0 + 31 < len ? first_query(a, key0 + 31, len) * a.group : R;      // rows from here on see all 32 keys
   const int my_first = key < len ? first_query(a, key, len) * a.group : R;                   // rows from here on see this lane's key
   if (r_first < r_last) {
-    const int kk = min(key, len - 1);
-    const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + kk * a.k_n + 2 * hk * a.k_h) * SZ;
-    const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + kk * a.v_n + hk * a.v_h) * SZ;
+    const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + min(key, len - 1) * a.k_n + (2 * hk + map) * a.k_h) * SZ;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) k[m][j] = load_chunk<T, VEC>(kp + m * a.k_h * SZ, 2 * j + g, a.d);
-#pragma unroll
-    for (int j = 0; j < NJV; ++j) v[j] = load_chunk<T, VEC>(vp, 2 * j + g, a.dv);
-    typedef Stage<T, D, RT, 256, VEC> StageQ;
-    typedef Stage<T, DV, RT, 256, VEC> StageO;
-    StageQ sq0, sq1;
+    for (int j = 0; j < NJ; ++j) k[j] = load_chunk<T, VEC>(kp, 2 * j + g, a.d);
+    {
+      typedef Stage<T, DV, KEYS, NTH, VEC, true> StageV;
+      StageV sv;
+      unsigned vo[StageV::PER];
+      key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, len - 1 - wg_key);
+      sv.load(tid, reinterpret_cast<const char*>(a.v) + (b * a.v_b + wg_key * a.v_n + hk * a.v_h) * SZ, vo, a.dv);
+      sv.store(tid, vt);
+    }
+    typedef Stage<T, D, 2 * RT, NTH, VEC> StageQ;
+    typedef Stage<T, DV, RT, NTH, VEC> StageO;
+    StageQ sq;
     StageO so;
     float st = 0.0f;
     const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + 2 * hk * a.group * a.q_h) * SZ;
@@ -378,114 +456,94 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(const Args a) {
     auto fetch = [&](int r0) {
       unsigned qo[StageQ::PER], oo[StageO::PER];
       const int i0 = r0 / a.group;
-      row_offsets<StageQ>(a, qo, tid, r0, i0, (unsigned)a.q_n * SZ, 2u * (unsigned)a.q_h * SZ);
-      row_offsets<StageO>(a, oo, tid, r0, i0, (unsigned)(a.heads * a.dv) * SZ, (unsigned)a.dv * SZ);
-      const char* q = qp + i0 * a.q_n * SZ;
-      sq0.load(tid, q, qo, a.d);
-      sq1.load(tid, q + a.q_h * SZ, qo, a.d);
+      row_offsets<StageQ, 2>(a, qo, tid, r0, i0, (unsigned)a.q_n * SZ, 2u * (unsigned)a.q_h * SZ, (unsigned)a.q_h * SZ);
+      row_offsets<StageO, 1>(a, oo, tid, r0, i0, (unsigned)(a.heads * a.dv) * SZ, (unsigned)a.dv * SZ, 0);
+      sq.load(tid, qp + i0 * a.q_n * SZ, qo, a.d);
       so.load(tid, op + (long long)i0 * a.heads * a.dv * SZ, oo, a.dv);
-      if (tid < 5 * RT) {
-        const int w = tid >> 5, rw = min(r0 + (tid & 31), R - 1);
-        if (w < 4) {
-          st = (w < 2 ? a.lse : a.dots)[((long long)base * 2 + (w & 1)) * R + rw];
+      if (tid < 6 * RT) {
+        const int w = tid >> 5, m = w >= 3 ? 1 : 0, rw = min(r0 + (tid & 31), R - 1);
+        if (w - 3 * m < 2) {
+          st = (w == 3 * m ? a.lse : a.dots)[((long long)base * 2 + m) * R + rw];
         } else {
           int gi;
           query_of(a, rw, gi);
-          st = lam_at<T>(a, hk * a.group + gi);
+          st = m == 0 ? 1.0f : -lam_at<T>(a, hk * a.group + gi);
         }
       }
     };
     auto place = [&](int buf) {
-      sq0.store(tid, lds + buf * BUF);
-      sq1.store(tid, lds + buf * BUF + QB);
+      sq.store(tid, lds + buf * BUF);
       so.store(tid, lds + buf * BUF + 2 * QB);
-      if (tid < 5 * RT) stat[buf][tid >> 5][tid & 31] = st;
+      if (tid < 6 * RT) (&stat[buf][0][0][0])[tid] = st;
     };
     fetch(r_first);
     place(0);
     __syncthreads();
-    int cur = 0;
-    for (int r0 = r_first; r0 < r_last; r0 += RT) {
+    two_buffers<RT>(r_first, r_last, [&](int r0, auto which) {
+      constexpr int CUR = decltype(which)::value;
+      const char* buf = lds + CUR * BUF;
       const bool more = r0 + RT < r_last;
       if (more) fetch(r0 + RT);
       if (r0 + RT > wave_first) {
-        const char* buf = lds + cur * BUF;
-        f32x16 p[2], dp;
-        zero_acc(p);
-#pragma unroll
-        for (int t = 0; t < 16; ++t) dp[t] = 0.0f;
-        mm_tile<T, D>(p[0], buf, 0, k[0], lane);
-        mm_tile<T, D>(p[1], buf + QB, 0, k[1], lane);
-        mm_tile<T, DV>(dp, buf + 2 * QB, 0, v, lane);
-        const bool edge = r0 < wave_all || r0 + RT > R;
-        f32x16 w[1];
+        f32x16 w = mm_tile<T, D>(buf + q_at, k), ds = mm_tiles<T, DV>(buf + g_at, own);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const f32x4 l1 = *reinterpret_cast<const f32x4*>(&stat[cur][0][8 * u + 4 * g]), l2 = *reinterpret_cast<const f32x4*>(&stat[cur][1][8 * u + 4 * g]);
-          const f32x4 d1 = *reinterpret_cast<const f32x4*>(&stat[cur][2][8 * u + 4 * g]), d2 = *reinterpret_cast<const f32x4*>(&stat[cur][3][8 * u + 4 * g]);
-          const f32x4 lm = *reinterpret_cast<const f32x4*>(&stat[cur][4][8 * u + 4 * g]);
+          const f32x4 l = *reinterpret_cast<const f32x4*>(&stat[CUR][map][0][8 * u + 4 * g]);
+          const f32x4 dd = *reinterpret_cast<const f32x4*>(&stat[CUR][map][1][8 * u + 4 * g]);
+          const f32x4 cf = *reinterpret_cast<const f32x4*>(&stat[CUR][map][2][8 * u + 4 * g]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = 4 * u + e;
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[0][t], c, -l1[e])), p2 = lm[e] * __builtin_amdgcn_exp2f(__builtin_fmaf(p[1][t], c, -l2[e]));
-            w[0][t] = p1 - p2;
-            p[0][t] = p1 * (dp[t] - d1[e]);
-            p[1][t] = p2 * (d2[e] - dp[t]);
-            if (edge) {      // (the products are replaced, not the factors: nothing that stands in a hidden place gets through)
-              const int row = r0 + tile_row(t, g);
-              const bool seen = row >= my_first && row < R;
-              w[0][t] = seen ? w[0][t] : 0.0f;
-              p[0][t] = seen ? p[0][t] : 0.0f;
-              p[1][t] = seen ? p[1][t] : 0.0f;
-            }
+            w[t] = cf[e] * __builtin_amdgcn_exp2f(__builtin_fmaf(w[t], c, -l[e]));
+            ds[t] = w[t] * (ds[t] - dd[e]);
           }
         }
-        mm_transposed<T, DV, NTV, 1>(dv, buf + 2 * QB, 0, w, lane);
-        f32x16 one[1] = {p[0]};
-        mm_transposed<T, D, NT, 1>(dk0, buf, 0, one, lane);
-        one[0] = p[1];
-        mm_transposed<T, D, NT, 1>(dk1, buf + QB, 0, one, lane);
+        if (r0 < wave_all || r0 + RT > R) {      // (the products are replaced, not the factors: nothing that stands in a hidden place gets through)
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            const int row = r0 + tile_row(t, g);
+            const bool seen = row >= my_first && row < R;
+            w[t] = seen ? w[t] : 0.0f;
+            ds[t] = seen ? ds[t] : 0.0f;
+          }
+        }
+        mm_transposed<T, DV, NTV>(dv, buf + gt_at, w);
+        mm_transposed<T, D, NT>(dk, buf + qt_at, ds);
       }
       if (more) {
-        place(cur ^ 1);
+        place(CUR ^ 1);
         __syncthreads();
-        cur ^= 1;
       }
-    }
+    });
   }
-  if (key >= a.nk) return;
-  const bool live = key < len;      // (rows behind the length: the clamped key's sums are not theirs)
-  auto each = [&](auto put) {
+  const bool live = key < len, there = key < a.nk;      // (rows behind the length: the clamped key's sums are not theirs)
+  const long long at = ((long long)b * a.nk + key) * a.kv_heads + hk;
+  const int width = 2 * a.d + a.dv;
+  float* part = a.work + ((long long)split * a.batch * a.nk * a.kv_heads + at) * width;      // [split][sample, key, head][dk1 | dk2 | dv]
+  auto put = [&](int which, int col, f32x4 x) {
+    if (!there) return;
+    if (!live) x = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (a.row_splits > 1) store4<float, VEC>(part + which * a.d, col, which < 2 ? a.d : a.dv, x);
+    else store4<T, VEC>(which < 2 ? reinterpret_cast<T*>(a.dk) + (at * 2 + which) * a.d : reinterpret_cast<T*>(a.dv_out) + at * a.dv, col, which < 2 ? a.d : a.dv, x);
+  };
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      f32x4 x;
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          f32x4 x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = live ? (m == 0 ? dk0 : dk1)[0][t][4 * u + e] * a.scale : 0.0f;
-          put(m, 32 * t + 8 * u + 4 * g, x);
-        }
-#pragma unroll
-      for (int t = 0; t < NTV; ++t) {
-        f32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = live ? dv[0][t][4 * u + e] : 0.0f;
-        put(2, 32 * t + 8 * u + 4 * g, x);
-      }
+      for (int e = 0; e < 4; ++e) x[e] = dk[t][4 * u + e] * a.scale;
+      put(map, 32 * t + 8 * u + 4 * g, x);
     }
-  };
-  const long long at = ((long long)b * a.nk + key) * a.kv_heads + hk;
-  if (a.row_splits > 1) {      // [split][sample, key, head][dk1 | dk2 | dv]
-    const int w = 2 * a.d + a.dv;
-    float* part = a.work + ((long long)split * a.batch * a.nk * a.kv_heads + at) * w;
-    each([&](int m, int col, f32x4 x) { store4<float, VEC>(part + m * a.d, col, m < 2 ? a.d : a.dv, x); });
-  } else {
-    T* dkp = reinterpret_cast<T*>(a.dk) + at * 2 * a.d;
-    T* dvp = reinterpret_cast<T*>(a.dv_out) + at * a.dv;
-    each([&](int m, int col, f32x4 x) { store4<T, VEC>(m < 2 ? dkp + m * a.d : dvp, col, m < 2 ? a.d : a.dv, x); });
-  }
+  hand_over<NTV, GROUPS, 2 * BUF>(dv, lds, group, map, lane, [&](int t, const f32x16& x, const f32x16& y) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f32x4 z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = x[4 * u + e] + y[4 * u + e];
+      put(2, 32 * t + 8 * u + 4 * g, z);
+    }
+  });
 }
 
 // dK, dV = the row splits' sums, in order; a thread per four elements (VEC) or one
@@ -510,133 +568,132 @@ __global__ __launch_bounds__(256) void key_join_kernel(const Args a) {
   else *out = (T)x[0];
 }
 
-// dQ of 32 rows per wave: grid (row tiles x kv_heads x batch)
+// dQ of 32 rows per wave: grid (row tiles x kv_heads x batch), GROUPS x 2 waves; dO of the workgroup's rows stays in LDS (registers)
 template <typename T, int D, bool VEC>
-__global__ __launch_bounds__(256, (D <= 64 && sizeof(T) == 2) || D <= 32 ? 2 : 1) void dq_kernel(const Args a) {
-  constexpr int DV = 2 * D, KT = 32, NT = D / 32, NJ = D / (2 * Vec<T>::N), NJV = DV / (2 * Vec<T>::N), SZ = sizeof(T);
+__global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(2))) void dq_kernel(const Args a) {
+  constexpr int GROUPS = dq_groups<T, D>(), NTH = 128 * GROUPS, ROWS = 32 * GROUPS;
+  constexpr int DV = 2 * D, KT = 32, NT = D / 32, NJ = D / (2 * Vec<T>::N), SZ = sizeof(T);
   constexpr int KB = Tile<T, D>::bytes(KT), VB = Tile<T, DV>::bytes(KT), BUF = 2 * KB + VB;
-  __shared__ __align__(16) char lds[2 * BUF];
+  __shared__ __align__(16) char lds[2 * BUF], gt[Tile<T, DV>::bytes(ROWS)];      // key tiles; dO of the workgroup's own rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, g = lane >> 5;
-  const int R = a.rows, tiles = (R + 127) / 128;
+  const int group = wave >> 1, map = wave & 1;
+  const int R = a.rows, tiles = (R + ROWS - 1) / ROWS;
   int base, unit;
   grid_order(blockIdx.x, a.batch * a.kv_heads, tiles, base, unit);
   const int tile = tiles - 1 - unit;
   const int b = base / a.kv_heads, hk = base - b * a.kv_heads;
   const int len = length_of(a, b);
-  const int row0 = tile * 128 + wave * 32, r = row0 + qi, rr = r < R ? r : R - 1;
+  const int row0 = tile * ROWS + group * 32, r = row0 + qi, rr = r < R ? r : R - 1;
   int gi;
   const int query = query_of(a, rr, gi), head = hk * a.group + gi;
-  const int wg_end = end_of(a, (min(tile * 128 + 128, R) - 1) / a.group, len);
+  const int wg_end = end_of(a, (min((tile + 1) * ROWS, R) - 1) / a.group, len);
   const int my_end = r < R ? end_of(a, query, len) : 0;
   const int wave_end = row0 < R ? end_of(a, min(row0 + 31, R - 1) / a.group, len) : 0;
   const int wave_all = row0 + 31 < R ? end_of(a, row0 / a.group, len) : 0;
   const float c = a.scale * 1.44269504088896340736f;
-  u32x4_t q[2][NJ], go[NJV];
-  const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + 2 * head * a.q_h) * SZ;
+  u32x4_t q[NJ];
+  const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + (2 * head + map) * a.q_h) * SZ;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) q[m][j] = load_chunk<T, VEC>(qp + m * a.q_h * SZ, 2 * j + g, a.d);
-  const char* gp = reinterpret_cast<const char*>(a.d_o) + o_at(a, b, query, head) * SZ;
-#pragma unroll
-  for (int j = 0; j < NJV; ++j) go[j] = load_chunk<T, VEC>(gp, 2 * j + g, a.dv);
-  const long long at = (long long)base * 2 * R + rr;
-  const float l1 = a.lse[at], l2 = a.lse[at + R], d1 = a.dots[at], d2 = a.dots[at + R], lam = lam_at<T>(a, head);
-  float sum2 = 0.0f;      // sum_j P_2 dP, for dlam
-  f32x16 dq0[1][NT], dq1[1][NT];
-  zero_acc2(dq0);
-  zero_acc2(dq1);
-  typedef Stage<T, D, KT, 256, VEC> StageK;
-  typedef Stage<T, DV, KT, 256, VEC> StageV;
-  StageK sk0, sk1;
+  for (int j = 0; j < NJ; ++j) q[j] = load_chunk<T, VEC>(qp, 2 * j + g, a.d);
+  {
+    typedef Stage<T, DV, ROWS, NTH, VEC, true> StageG;
+    StageG sg;
+    unsigned offset[StageG::PER];
+    const int r0 = tile * ROWS, i0 = r0 / a.group;
+    row_offsets<StageG, 1>(a, offset, tid, r0, i0, (unsigned)(a.heads * a.dv) * SZ, (unsigned)a.dv * SZ, 0);
+    sg.load(tid, reinterpret_cast<const char*>(a.d_o) + o_at(a, b, i0, hk * a.group) * SZ, offset, a.dv);
+    sg.store(tid, gt);      // (read behind the barrier that follows the first key tile)
+  }
+  const long long at = ((long long)base * 2 + map) * R + rr;
+  const float l = a.lse[at], dd = a.dots[at], cf = map == 0 ? 1.0f : -lam_at<T>(a, head);
+  float dot = 0.0f;      // sum_j P dP: map 1's is what dlam is made of
+  const int k_at = map * KB + Tile<T, D>::rows_at(lane), kt_at = map * KB + Tile<T, D>::columns_at(lane), v_at = 2 * KB + Tile<T, DV>::rows_at(lane);
+  const char* own = gt + Tile<T, DV>::bytes(32) * group + Tile<T, DV>::rows_at(lane);
+  f32x16 dq[NT];
+  zero_acc(dq);
+  typedef Stage<T, D, 2 * KT, NTH, VEC> StageK;
+  typedef Stage<T, DV, KT, NTH, VEC> StageV;
+  StageK sk;
   StageV sv;
   const char* kp = reinterpret_cast<const char*>(a.k) + (b * a.k_b + 2 * hk * a.k_h) * SZ;
   const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + hk * a.v_h) * SZ;
   auto fetch = [&](int j0) {
     unsigned ko[StageK::PER], vo[StageV::PER];
-    key_offsets<StageK>(ko, tid, (unsigned)a.k_n * SZ, len - 1 - j0);
-    key_offsets<StageV>(vo, tid, (unsigned)a.v_n * SZ, len - 1 - j0);
-    const char* k = kp + j0 * a.k_n * SZ;
-    sk0.load(tid, k, ko, a.d);
-    sk1.load(tid, k + a.k_h * SZ, ko, a.d);
+    key_offsets<StageK, 2>(ko, tid, (unsigned)a.k_n * SZ, (unsigned)a.k_h * SZ, len - 1 - j0);
+    key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, len - 1 - j0);
+    sk.load(tid, kp + j0 * a.k_n * SZ, ko, a.d);
     sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
   auto place = [&](char* buf) {
-    sk0.store(tid, buf);
-    sk1.store(tid, buf + KB);
+    sk.store(tid, buf);
     sv.store(tid, buf + 2 * KB);
   };
   if (wg_end > 0) {
     fetch(0);
     place(lds);
     __syncthreads();
-    int cur = 0;
-    for (int j0 = 0; j0 < wg_end; j0 += KT) {
+    two_buffers<KT>(0, wg_end, [&](int j0, auto which) {
+      constexpr int CUR = decltype(which)::value;
+      const char* buf = lds + CUR * BUF;
       const bool more = j0 + KT < wg_end;
       if (more) fetch(j0 + KT);
       if (j0 < wave_end) {
-        const char* buf = lds + cur * BUF;
-        f32x16 p[2], dp;
-        zero_acc(p);
+        f32x16 w = mm_tile<T, D>(buf + k_at, q), ds = mm_tiles<T, DV>(buf + v_at, own);
 #pragma unroll
-        for (int t = 0; t < 16; ++t) dp[t] = 0.0f;
-        mm_tile<T, D>(p[0], buf, 0, q[0], lane);
-        mm_tile<T, D>(p[1], buf + KB, 0, q[1], lane);
-        mm_tile<T, DV>(dp, buf + 2 * KB, 0, go, lane);
-        const bool edge = j0 + KT > wave_all;
-        float s = 0.0f;
+        for (int t = 0; t < 16; ++t) w[t] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[t], c, -l));
+        if (j0 + KT > wave_all) {
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[0][t], c, -l1)), p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[1][t], c, -l2));
-          float both = p2 * dp[t];
-          p[0][t] = p1 * (dp[t] - d1);
-          p[1][t] = p2 * (d2 - dp[t]) * lam;
-          if (edge) {
+          for (int t = 0; t < 16; ++t) {
             const bool seen = j0 + tile_row(t, g) < my_end;
-            p[0][t] = seen ? p[0][t] : 0.0f;
-            p[1][t] = seen ? p[1][t] : 0.0f;
-            both = seen ? both : 0.0f;
+            w[t] = seen ? w[t] : 0.0f;
+            ds[t] = seen ? ds[t] : 0.0f;
           }
-          s += both;
         }
-        sum2 += s;
-        f32x16 one[1] = {p[0]};
-        mm_transposed<T, D, NT, 1>(dq0, buf, 0, one, lane);
-        one[0] = p[1];
-        mm_transposed<T, D, NT, 1>(dq1, buf + KB, 0, one, lane);
+        if (map == 1) {
+          float s = 0.0f;
+#pragma unroll
+          for (int t = 0; t < 16; ++t) s = __builtin_fmaf(w[t], ds[t], s);
+          dot += s;
+        }
+#pragma unroll
+        for (int t = 0; t < 16; ++t) ds[t] = w[t] * (ds[t] - dd);
+        if (j0 + KT > wave_all) {      // (dd may be no number where the row sees nothing)
+#pragma unroll
+          for (int t = 0; t < 16; ++t) ds[t] = j0 + tile_row(t, g) < my_end ? ds[t] : 0.0f;
+        }
+        mm_transposed<T, D, NT>(dq, buf + kt_at, ds);
       }
       if (more) {
-        place(lds + (cur ^ 1) * BUF);
+        place(lds + (CUR ^ 1) * BUF);
         __syncthreads();
-        cur ^= 1;
       }
-    }
+    });
   }
-  sum2 += other_half(sum2);
+  dot += other_half(dot);
   if (r >= R) return;
-  if (g == 0) a.dots[(2LL * a.batch * a.kv_heads + base) * R + r] = sum2;
-  T* out = reinterpret_cast<T*>(a.dq) + (((long long)b * a.nq + query) * a.heads + head) * 2 * a.d;
+  if (map == 1 && g == 0) a.dots[(2LL * a.batch * a.kv_heads + base) * R + r] = dot;
+  T* out = reinterpret_cast<T*>(a.dq) + ((((long long)b * a.nq + query) * a.heads + head) * 2 + map) * a.d;
+  const float f = a.scale * cf;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int u = 0; u < 4; ++u) {
+      f32x4 x;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        f32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = (m == 0 ? dq0 : dq1)[0][t][4 * u + e] * a.scale;
-        store4<T, VEC>(out + m * a.d, 32 * t + 8 * u + 4 * g, a.d, x);
-      }
+      for (int e = 0; e < 4; ++e) x[e] = dq[t][4 * u + e] * f;
+      store4<T, VEC>(out, 32 * t + 8 * u + 4 * g, a.d, x);
+    }
 }
 
 // ---- launches: one compilation unit per element type ----------------------------------------------------------------------------------
 template <typename T, int D, bool VEC>
 void launch_fwd(const Args& a, hipStream_t st) {
   const int heads = a.kv_heads * a.batch;
-  if (a.rows <= 32) {      // a handful of rows: one wave per workgroup, the keys split over many of them
-    fwd_kernel<T, D, 1, VEC><<<a.splits * heads, 64, 0, st>>>(a);
+  if (a.rows <= 32) {      // a handful of rows: one pair of waves per workgroup, the keys split over many of them
+    fwd_kernel<T, D, 1, VEC><<<a.splits * heads, 128, 0, st>>>(a);
   } else {
-    fwd_kernel<T, D, 4, VEC><<<(a.rows + 127) / 128 * a.splits * heads, 256, 0, st>>>(a);
+    constexpr int GROUPS = fwd_groups<T, D>(), ROWS = 32 * GROUPS;
+    fwd_kernel<T, D, GROUPS, VEC><<<(a.rows + ROWS - 1) / ROWS * a.splits * heads, 4 * ROWS, 0, st>>>(a);
   }
   if (a.splits > 1) join_kernel<T><<<(unsigned)(((long long)heads * a.rows + 3) / 4), 256, 0, st>>>(a);
 }
@@ -644,11 +701,12 @@ void launch_fwd(const Args& a, hipStream_t st) {
 template <typename T, int D, bool VEC>
 void launch_bwd(const Args& a, hipStream_t st) {
   const int heads = a.kv_heads * a.batch;
-  rowdot_kernel<T><<<(unsigned)(((long long)heads * a.rows + 3) / 4), 256, 0, st>>>(a);
-  dkv_kernel<T, D, VEC><<<(a.nk + 127) / 128 * a.row_splits * heads, 256, 0, st>>>(a);
+  constexpr int KEYS = 32 * key_groups<T, D>(), ROWS = 32 * dq_groups<T, D>();
+  rowdot_kernel<T, VEC><<<(unsigned)(((long long)heads * a.rows + 15) / 16), 256, 0, st>>>(a);
+  dkv_kernel<T, D, VEC><<<(a.nk + KEYS - 1) / KEYS * a.row_splits * heads, 4 * KEYS, 0, st>>>(a);
   if (a.row_splits > 1)
     key_join_kernel<T, VEC><<<(unsigned)(((long long)heads * a.nk * (2 * a.d + a.dv) / (VEC ? 4 : 1) + 255) / 256), 256, 0, st>>>(a);
-  dq_kernel<T, D, VEC><<<(a.rows + 127) / 128 * heads, 256, 0, st>>>(a);
+  dq_kernel<T, D, VEC><<<(a.rows + ROWS - 1) / ROWS * heads, 4 * ROWS, 0, st>>>(a);
   dlam_kernel<T><<<a.heads, 1024, 0, st>>>(a);
 }
 

@@ -18,7 +18,7 @@ int prepare(da::Args& a) {
   const long long rows = (long long)a.nq * a.group, big = 0x7fffff00LL;
   const int n = a.type == TYPE_F32 ? 4 : 8, size = 16 / n;
   if (rows > big || a.nk > big || (rows / 32 + 1) * a.splits * a.kv_heads > big / a.batch || (rows + 3) * a.kv_heads > big / a.batch ||
-      (a.nk / 128 + 1LL) * a.row_splits * a.kv_heads > big / a.batch || (a.nk * (2LL * a.d + a.dv) + 255) / 256 * a.kv_heads > big / a.batch) return -22;
+      (a.nk / 64 + 1LL) * a.row_splits * a.kv_heads > big / a.batch || (a.nk * (2LL * a.d + a.dv) + 255) / 256 * a.kv_heads > big / a.batch) return -22;
   a.rows = (int)rows;
   // a tile's rows lie within 31 bits of its first
   const long long near = 0x7fffffffLL / size;
@@ -47,7 +47,7 @@ extern "C" {
 int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk) {
   if (batch < 1 || kv_heads < 1 || rows < 1 || nk < 1) return 1;
   const long long groups = (rows <= 32 ? 1LL : (rows + 127LL) / 128) * kv_heads * batch;
-  const long long want = (rows <= 32 ? 1024 : 512) / groups, most = (nk + 127LL) / 128;
+  const long long want = rows <= 32 ? 1024 / groups : groups < 192 ? 512 / groups : 1, most = (nk + 127LL) / 128;
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }

@@ -78,98 +78,105 @@ __device__ __forceinline__ f32x16 mfma_chunk(u32x4_t a, u32x4_t b, f32x16 c) {
   }
 }
 
-// Row-major LDS tile of N-element rows, addressed in 16-byte chunks.
-//   16-bit types: rows are a power of two >= 64 bytes, no padding; chunk c of a row sits at slot c ^ swizzle(row), chosen so that both the
-//   row-per-lane b128 reads (16 rows, one chunk) and the transposed reads (4 rows x 64 bytes per 32 lanes) touch all 64 banks once.
-//   float: one chunk of padding per row (b128 rows conflict-free; the b32 transposed reads are 2-way, hidden behind the 64-cycle MFMAs).
+// Row-major LDS tile of N-element rows, each padded so that one lane address and compile-time offsets reach everything (a swizzle would cost a
+// register or an instruction per read, and these kernels have neither to spare).  In 4-byte words, rows are W + pad apart with (W + pad) / 4
+// odd: 16 rows of one chunk fall on 64 different banks.  The transposed reads take 4 rows x 64 bytes at a time: the pads of the 16-bit types keep
+// those (nearly) apart as well; 32-bit transposed reads are at most 2-way, hidden behind their 64-cycle matrix instructions.
 template <typename T, int N>
 struct Tile {
-  static constexpr int CHUNKS = N * (int)sizeof(T) / 16;
-  static constexpr int STRIDE = N * (int)sizeof(T) + (sizeof(T) == 4 ? 16 : 0);
+  static constexpr int WORDS = N * (int)sizeof(T) / 4, CHUNKS = WORDS / 4;
+  static constexpr int STRIDE = 4 * (WORDS + (sizeof(T) == 4 || WORDS <= 32 ? 4 : 20));
   static constexpr int bytes(int rows) { return rows * STRIDE; }
-  static __device__ __forceinline__ int swizzle(int row) {
-    if constexpr (sizeof(T) == 4) return 0;
-    else if constexpr (CHUNKS >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
-    else if constexpr (CHUNKS == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
-    else return (row >> 2) & 3;
-  }
-  static __device__ __forceinline__ int offset(int row, int chunk) { return row * STRIDE + ((chunk ^ swizzle(row)) << 4); }
-  // lane (r, g)'s share of step j of the rows [row0, row0 + 32)
-  static __device__ __forceinline__ u32x4_t rows(const char* tile, int row0, int j, int lane) {
-    return *reinterpret_cast<const u32x4_t*>(tile + offset(row0 + (lane & 31), 2 * j + (lane >> 5)));
+  static __device__ __forceinline__ int offset(int row, int chunk) { return row * STRIDE + chunk * 16; }
+  // lane (r, g)'s place in rows [0, 32): chunk g of row r (step j: + 32 j)
+  static __device__ __forceinline__ int rows_at(int lane) { return (lane & 31) * STRIDE + (lane >> 5) * 16; }
+  // lane's place for the transposed reads of rows [0, 4) + 4 g, columns [0, 32): see mm_transposed
+  static __device__ __forceinline__ int columns_at(int lane) {
+    if constexpr (sizeof(T) == 4) return 4 * (lane >> 5) * STRIDE + (lane & 31) * 4;
+    else return (4 * (lane >> 5) + ((lane >> 2) & 3)) * STRIDE + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
   }
 };
 
-// acc (32 x 32) += tile rows [row0, row0 + 32) . b, b = the register-resident other operand (N / (2 Vec::N) steps)
+// (32 x 32) = tile rows . b: `at` = tile + rows_at(lane) of its first row, b = the register-resident other operand (N / (2 Vec::N) steps)
 template <typename T, int N>
-__device__ __forceinline__ void mm_tile(f32x16& acc, const char* tile, int row0, const u32x4_t (&b)[N / (2 * Vec<T>::N)], int lane) {
+__device__ __forceinline__ f32x16 mm_tile(const char* at, const u32x4_t (&b)[N / (2 * Vec<T>::N)]) {
+  f32x16 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < N / (2 * Vec<T>::N); ++j) acc = mfma_chunk<T>(Tile<T, N>::rows(tile, row0, j, lane), b[j], acc);
+  for (int j = 0; j < N / (2 * Vec<T>::N); ++j) acc = mfma_chunk<T>(*reinterpret_cast<const u32x4_t*>(at + 32 * j), b[j], acc);
+  return acc;
+}
+// the same with both operands in LDS
+template <typename T, int N>
+__device__ __forceinline__ f32x16 mm_tiles(const char* at, const char* other) {
+  f32x16 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < N / (2 * Vec<T>::N); ++j)
+    acc = mfma_chunk<T>(*reinterpret_cast<const u32x4_t*>(at + 32 * j), *reinterpret_cast<const u32x4_t*>(other + 32 * j), acc);
+  return acc;
 }
 
-// acc[m][t] (32 x 32: rows = columns 32 t .. of the tile, columns = p's columns) += (tile rows [row0, row0 + 32))^T . p[m]
-template <typename T, int N, int NT, int NB>
-__device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NB][NT], const char* tile, int row0, const f32x16 (&p)[NB], int lane) {
-  const int g = lane >> 5;
+// acc[t] (32 x 32: rows = columns 32 t .. of the tile, columns = p's columns) += (32 tile rows)^T . p;  `at` = tile + columns_at(lane) of the first row
+template <typename T, int N, int NT>
+__device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NT], const char* at, const f32x16& p) {
   if constexpr (sizeof(T) == 4) {
-    const char* base = tile + (row0 + 4 * g) * Tile<T, N>::STRIDE + (lane & 31) * 4;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float a = *reinterpret_cast<const float*>(base + (8 * u + e) * Tile<T, N>::STRIDE + t * 128);
-#pragma unroll
-          for (int m = 0; m < NB; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[m][4 * u + e], acc[m][t], 0, 0, 0);
-        }
+        for (int t = 0; t < NT; ++t)
+          acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(at + (8 * u + e) * Tile<T, N>::STRIDE + t * 128), p[4 * u + e], acc[t], 0, 0, 0);
   } else {
     typedef T V __attribute__((ext_vector_type(8)));
-    const int i = lane & 15, row = 4 * g + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    // 16 lanes read 4 rows x 16 columns (lane i: row i / 4, columns 4 (i mod 4) ..) and receive column i of the 4 rows
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4_t b[NB];
+      V v;
 #pragma unroll
-      for (int m = 0; m < NB; ++m) {
-        V v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (T)p[m][8 * h + e];      // one rounding to the inputs' type: what the matrix instruction takes
-        b[m] = __builtin_bit_cast(u32x4_t, v);
-      }
+      for (int e = 0; e < 8; ++e) v[e] = (T)p[8 * h + e];      // one rounding to the inputs' type: what the matrix instruction takes
+      const u32x4_t b = __builtin_bit_cast(u32x4_t, v);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         u32x2 half[2];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int rr = row0 + 8 * (2 * h + w) + row;
-          const char* at = tile + Tile<T, N>::offset(rr, 4 * t + c) + (i & 1) * 8;
-          half[w] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
-        }
-        const u32x4_t a = {half[0][0], half[0][1], half[1][0], half[1][1]};
-#pragma unroll
-        for (int m = 0; m < NB; ++m) acc[m][t] = mfma_chunk<T>(a, b[m], acc[m][t]);
+        for (int w = 0; w < 2; ++w)
+          half[w] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(at + 8 * (2 * h + w) * Tile<T, N>::STRIDE + t * 64)));
+        acc[t] = mfma_chunk<T>(u32x4_t{half[0][0], half[0][1], half[1][0], half[1][1]}, b, acc[t]);
       }
     }
   }
 }
 
-// ROWS rows of N elements, global -> registers -> LDS by NTHREADS threads.  Thread t handles rows row_of(k); their byte offsets from a base
-// that is uniform over the workgroup are 32-bit (one 64-bit scalar base per tile and one 32-bit lane offset per load).
-template <typename T, int N, int ROWS, int NTHREADS, bool VEC>
+// ROWS rows of N elements, global -> registers -> LDS by NTHREADS threads.  Thread t handles chunk t mod CH of the rows row_of(k); their byte
+// offsets from a base that is uniform over the workgroup are 32-bit (one 64-bit scalar base per tile and one 32-bit lane offset per load).
+// Rows of fewer than N elements: EXACT fills the rest with zeros, the other form repeats the row's last chunk there (no test per load):
+// the other operand of every product over that dimension is zero there, or the columns are never stored.
+template <typename T, int N, int ROWS, int NTHREADS, bool VEC, bool EXACT = false>
 struct Stage {
-  static constexpr int CH = Tile<T, N>::CHUNKS, TOTAL = ROWS * CH, PER = (TOTAL + NTHREADS - 1) / NTHREADS;
+  static constexpr int ROWS_ = ROWS, CH = Tile<T, N>::CHUNKS, TOTAL = ROWS * CH, PER = (TOTAL + NTHREADS - 1) / NTHREADS;
   u32x4_t v[PER];
   static __device__ __forceinline__ int row_of(int tid, int k) { return (tid + k * NTHREADS) / CH; }
   static __device__ __forceinline__ bool has(int tid, int k) { return TOTAL % NTHREADS == 0 || tid + k * NTHREADS < TOTAL; }
   __device__ __forceinline__ void load(int tid, const char* base, const unsigned (&offset)[PER], int len) {
+    int c = tid % CH;
+    if constexpr (VEC && !EXACT) {
+      const int most = len / Vec<T>::N - 1;
+      c = c < most ? c : most;
+    }
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-      if (has(tid, k)) v[k] = load_chunk<T, VEC>(base + offset[k], (tid + k * NTHREADS) % CH, len);
+      if (has(tid, k)) {
+        if constexpr (VEC && !EXACT) v[k] = *reinterpret_cast<const u32x4_t*>(base + (offset[k] + (unsigned)c * 16u));
+        else v[k] = load_chunk<T, VEC>(base + offset[k], c, len);
+      }
   }
   __device__ __forceinline__ void store(int tid, char* tile) const {
+    static_assert(NTHREADS % CH == 0, "a thread's chunks lie whole rows apart");
+    char* at = tile + Tile<T, N>::offset(tid / CH, tid % CH);
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-      if (has(tid, k)) *reinterpret_cast<u32x4_t*>(tile + Tile<T, N>::offset(row_of(tid, k), (tid + k * NTHREADS) % CH)) = v[k];
+      if (has(tid, k)) *reinterpret_cast<u32x4_t*>(at + k * (NTHREADS / CH) * Tile<T, N>::STRIDE) = v[k];
   }
 };
 

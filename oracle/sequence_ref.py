@@ -162,9 +162,11 @@ def differential_attention(q, k, v, lam, lengths, causal, scale, do=None):
             g = DO[i, :, head]
             ga = g.abs()
             w = p[0] - lm * p[1]
+            # (each map's weights are rounded on their own and multiplied with dO on their own: |d(P1 - lam P2)| <= u P1 + u |lam| P2)
+            wa = p[0] + lm.abs() * p[1]
             dw = f[0] * p[0] + lm.abs() * f[1] * p[1]
             out["dv"][0][i, :n, kv] += w.t() @ g
-            out["dv"][1][i, :n, kv] += (dw + u * w.abs() + sub + 64 * E32 * w.abs()).t() @ ga
+            out["dv"][1][i, :n, kv] += (dw + u * wa + 2 * sub + 64 * E32 * wa).t() @ ga
             dp, dpa = g @ val.t(), (dv + 4) * E32 * (ga @ val.abs().t())
             d2 = (g * o[1]).sum(1, keepdim=True)
             e2 = (ga * (do_[1] + ot * o[1].abs() + tiny + dv * E32 * o[1].abs())).sum(1, keepdim=True)
