@@ -8,7 +8,8 @@
 //         a workgroup walks many samples and keeps its channels' dw / db sums in registers.
 //   slab  a workgroup holds all rows of one sample's slice of whole groups in registers (up to 16 chunks a thread): one read, exact two-step
 //         variance, one write.  Slices are as narrow as 64-byte row segments allow, so that small batches still fill the chip.
-//   long  a sample does not fit: row blocks leave (mean, M2) / (sum t, sum t xhat) of every group, a second launch joins a sample's blocks and
+//   long  a sample does not fit: row blocks leave (mean, M2) / (sum t, sum t xhat) of every group, a small launch joins a sample's blocks (one
+//         wave per sample and group; done by every workgroup of the next pass it cost 50 us at (2, 65536, 512), 32 groups), a third
 //         writes.  Block sums are taken about each thread's own first value, so a large mean costs no precision.
 //   any   groups of more than 256 chunks: one workgroup per (sample, group), re-reading.
 // Chunks are 16 bytes where pointers, strides and the group width allow, single elements otherwise (a chunk never straddles two groups).
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int s
 }
 
 // ---- long: row blocks ---------------------------------------------------------------------------------------------------------------------
-// workspace: pairs[sample][block][group][2], behind it the dw / db records.  Workgroup = (sample, block, slice)
+// workspace: pairs[sample][group][block][2], joined[sample][group][2], then the dw / db records.  Workgroup = (sample, block, slice)
 struct Block {
   int b, block, c0, first, last, len;
   __device__ __forceinline__ Block(const Args& a, const Plan& p) {
@@ -394,6 +395,29 @@ struct Block {
     first = block * p.rows;
     last = min(first + p.rows, len);
   }
+};
+
+__device__ __forceinline__ float* pair_at(const Args& a, const Plan& plan, const Block& k, int group) {
+  return a.work + 2 * (((long long)k.b * a.groups + group) * plan.blocks + k.block);
+}
+
+// rows first, first + step ... below end, four at a time: all loads of a batch are in flight before its first use
+constexpr int BATCH = 4;
+template <typename H, typename LoadF, typename UseF>
+__device__ __forceinline__ void batches(int first, int end, int step, LoadF load, UseF use) {
+  for (int row = first; row < end; row += BATCH * step) {
+    H h[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (row + u * step < end) load(row + u * step, h[u]);
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (row + u * step < end) use(row + u * step, h[u]);
+  }
+}
+template <typename T, int VE>
+struct Pair {
+  Held<T, VE> x, d;
 };
 
 template <typename T, int VE>
@@ -417,8 +441,8 @@ __global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan
       for (int e = 0; e < VE; ++e) base[e] = v.x[e];
       ++count;
     }
-    for (row += p.lanes; row < k.last; row += p.lanes) {
-      v.load(x + row * a.x_n);
+    batches<Held<T, VE>>(row + p.lanes, k.last, p.lanes, [&](int r, Held<T, VE>& h) { h.load(x + r * a.x_n); }, [&](int, const Held<T, VE>& h) {
+      h.get(v.x);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         const float t = v.x[e] - base[e];
@@ -426,7 +450,7 @@ __global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan
         q[e] += t * t;
       }
       ++count;
-    }
+    });
   }
   const float rows = (float)(k.last > k.first ? k.last - k.first : 0), total = rows * (float)cg;
   float sum = 0.0f;
@@ -444,55 +468,55 @@ __global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan
   }
   m2 = group_sum(m2, p, cpg, all, out);
   if (p.on && p.rl == 0 && p.col % cpg == 0) {
-    float* at = a.work + 2 * (((long long)k.b * plan.blocks + k.block) * a.groups + c / cg);
+    float* at = pair_at(a, plan, k, c / cg);
     at[0] = mean;
     at[1] = m2;
   }
 }
 
-// the two sums over a sample's blocks of pairs[..][group][2], for the slice's groups; `weigh` turns a block's pair into its two summands
-template <typename F>
-__device__ __forceinline__ void join_blocks(const Args& a, const Plan& plan, const Block& k, int cg, float (*out)[256], F weigh) {
-  // out[.][i] for the slice's group i: a wave per group
-  const int groups = plan.slice / cg, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int i = wave; i < groups; i += 4) {
-    float s0 = 0.0f, s1 = 0.0f;
-    for (int n = lane; n < plan.blocks; n += 64) {
-      const float* at = a.work + 2 * (((long long)k.b * plan.blocks + n) * a.groups + k.c0 / cg + i);
-      const int r0 = n * plan.rows, rows = min(r0 + plan.rows, k.len) - r0;
-      if (rows > 0) weigh(at[0], at[1], (float)rows, i, s0, s1);
-    }
-    s0 = wave_sum(s0);
-    s1 = wave_sum(s1);
-    if (lane == 0) {
-      out[0][i] = s0;
-      out[1][i] = s1;
+// one wave per (sample, group): forward -> mean and rstd; backward -> the means of t and t xhat
+template <bool BACK>
+__global__ __launch_bounds__(256) void long_join_kernel(const Args a, const Plan plan) {
+  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (long long)a.batch * a.groups) return;
+  const int lane = threadIdx.x & 63, len = length_of(a, (int)(i / a.groups)), cg = a.channels / a.groups;
+  const float2* at = reinterpret_cast<const float2*>(a.work) + i * plan.blocks;
+  const float total = (float)(len > 0 ? len : 1);
+  auto rows = [&](int n) { return (float)max(min((n + 1) * plan.rows, len) - n * plan.rows, 0); };
+  float s0 = 0.0f, s1 = 0.0f;
+  for (int n = lane; n < plan.blocks; n += 64) {
+    const float2 x = at[n];
+    if constexpr (BACK) {
+      s0 += x.x;
+      s1 += x.y;
+    } else {
+      s0 += x.x * (rows(n) / total);
     }
   }
-  __syncthreads();
+  s0 = wave_sum(s0);
+  if constexpr (BACK) {
+    s1 = wave_sum(s1);
+    if (lane == 0) reinterpret_cast<float2*>(a.work)[(long long)a.batch * a.groups * plan.blocks + i] = make_float2(s0 / (total * cg), s1 / (total * cg));
+  } else {
+    for (int n = lane; n < plan.blocks; n += 64) {
+      const float2 x = at[n];
+      const float off = x.x - s0;
+      s1 += x.y + rows(n) * (float)cg * off * off;
+    }
+    s1 = wave_sum(s1);
+    if (lane == 0) reinterpret_cast<float2*>(a.stats)[i] = make_float2(s0, 1.0f / sqrtf(s1 / (total * cg) + a.eps));
+  }
 }
 
 template <typename T, int VE>
 __global__ __launch_bounds__(256) void long_apply_kernel(const Args a, const Plan plan) {
-  __shared__ float join[2][2][256];
   const Block k(a, plan);
-  const int cg = a.channels / a.groups, cpg = cg / VE;
-  const float total = (float)(k.len > 0 ? k.len : 1);
-  // mean of the sample, then M2 about it
-  join_blocks(a, plan, k, cg, join[0], [&](float mean, float, float rows, int, float& s0, float&) { s0 += mean * (rows / total); });
-  join_blocks(a, plan, k, cg, join[1], [&](float mean, float m2, float rows, int i, float& s0, float&) {
-    const float off = mean - join[0][0][i];
-    s0 += m2 + rows * (float)cg * off * off;
-  });
+  const int cg = a.channels / a.groups;
   const Place p(plan.slice, VE);
   if (!p.on) return;
   const int c = k.c0 + p.col * VE;
-  const float mean = join[0][0][p.col / cpg], rstd = 1.0f / sqrtf(join[1][0][p.col / cpg] / (total * (float)cg) + a.eps);
-  if (k.block == 0 && p.rl == 0 && p.col % cpg == 0) {
-    float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
-    st[0] = mean;
-    st[1] = rstd;
-  }
+  const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
+  const float mean = st[0], rstd = st[1];
   float w[VE], o[VE];
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
@@ -502,17 +526,16 @@ __global__ __launch_bounds__(256) void long_apply_kernel(const Args a, const Pla
   const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
   T* y = reinterpret_cast<T*>(a.y) + (long long)k.b * a.n * a.channels + c;
   const int end = min(k.first + plan.rows, a.n);
-  for (int row = k.first + p.rl; row < end; row += p.lanes) {
+  batches<Held<T, VE>>(k.first + p.rl, end, p.lanes, [&](int row, Held<T, VE>& h) {
+    h.zero();
+    if (row < k.len) h.load(x + row * a.x_n);
+  }, [&](int row, const Held<T, VE>& h) {
     Chunk<T, VE> v;
+    h.get(v.x);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) v.x[e] = 0.0f;
-    if (row < k.len) {
-      v.load(x + row * a.x_n);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) v.x[e] = act((v.x[e] - mean) * rstd * w[e] + o[e], a.activation);
-    }
+    for (int e = 0; e < VE; ++e) v.x[e] = row < k.len ? act((v.x[e] - mean) * rstd * w[e] + o[e], a.activation) : 0.0f;
     v.store(y + (long long)row * a.channels);
-  }
+  });
 }
 
 template <typename T, int VE>
@@ -534,17 +557,20 @@ __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan 
     const float mean = st[0], rstd = st[1];
     const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
     const T* dy = reinterpret_cast<const T*>(a.dy) + (long long)k.b * a.n * a.channels + c;
-    for (int row = k.first + p.rl; row < k.last; row += p.lanes) {
-      Chunk<T, VE> v, d;
-      v.load(x + row * a.x_n);
-      d.load(dy + (long long)row * a.channels);
+    batches<Pair<T, VE>>(k.first + p.rl, k.last, p.lanes, [&](int row, Pair<T, VE>& h) {
+      h.x.load(x + row * a.x_n);
+      h.d.load(dy + (long long)row * a.channels);
+    }, [&](int, const Pair<T, VE>& h) {
+      float v[VE], d[VE];
+      h.x.get(v);
+      h.d.get(d);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float hat = (v.x[e] - mean) * rstd, dz = d.x[e] * act_slope(hat * w[e] + o[e], a.activation);
+        const float hat = (v[e] - mean) * rstd, dz = d[e] * act_slope(hat * w[e] + o[e], a.activation);
         sw[e] += dz * hat;
         sb[e] += dz;
       }
-    }
+    });
   }
   float t1 = 0.0f, t2 = 0.0f;
 #pragma unroll
@@ -554,9 +580,9 @@ __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan 
   }
   t1 = group_sum(t1, p, cpg, all, out);
   t2 = group_sum(t2, p, cpg, all, out);
-  const long long pairs = 2LL * a.batch * plan.blocks * a.groups, index = (long long)k.b * plan.blocks + k.block;
+  const long long pairs = 2LL * a.batch * (plan.blocks + 1) * a.groups, index = (long long)k.b * plan.blocks + k.block;
   if (p.on && p.rl == 0 && p.col % cpg == 0) {
-    float* at = a.work + 2 * (index * a.groups + c / cg);
+    float* at = pair_at(a, plan, k, c / cg);
     at[0] = t1;
     at[1] = t2;
   }
@@ -565,17 +591,13 @@ __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan 
 
 template <typename T, int VE>
 __global__ __launch_bounds__(256) void long_dx_kernel(const Args a, const Plan plan) {
-  __shared__ float join[2][256];
   const Block k(a, plan);
-  const int cg = a.channels / a.groups, cpg = cg / VE;
-  join_blocks(a, plan, k, cg, join, [](float t1, float t2, float, int, float& s0, float& s1) {
-    s0 += t1;
-    s1 += t2;
-  });
+  const int cg = a.channels / a.groups;
   const Place p(plan.slice, VE);
   if (!p.on) return;
   const int c = k.c0 + p.col * VE;
-  const float inv = 1.0f / ((float)(k.len > 0 ? k.len : 1) * (float)cg), t1 = join[0][p.col / cpg] * inv, t2 = join[1][p.col / cpg] * inv;
+  const float* joined = a.work + 2LL * a.batch * a.groups * plan.blocks + 2 * ((long long)k.b * a.groups + c / cg);
+  const float t1 = joined[0], t2 = joined[1];
   const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
   const float mean = st[0], rstd = st[1];
   float w[VE], o[VE];
@@ -589,21 +611,25 @@ __global__ __launch_bounds__(256) void long_dx_kernel(const Args a, const Plan p
   const T* dy = reinterpret_cast<const T*>(a.dy) + at;
   T* dx = reinterpret_cast<T*>(a.dx) + at;
   const int end = min(k.first + plan.rows, a.n);
-  for (int row = k.first + p.rl; row < end; row += p.lanes) {
-    Chunk<T, VE> v, d;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) d.x[e] = 0.0f;
+  batches<Pair<T, VE>>(k.first + p.rl, end, p.lanes, [&](int row, Pair<T, VE>& h) {
+    h.x.zero();
+    h.d.zero();
     if (row < k.len) {
-      v.load(x + row * a.x_n);
-      d.load(dy + (long long)row * a.channels);
+      h.x.load(x + row * a.x_n);
+      h.d.load(dy + (long long)row * a.channels);
+    }
+  }, [&](int row, const Pair<T, VE>& h) {
+    float v[VE];
+    Chunk<T, VE> d;
+    h.x.get(v);
+    h.d.get(d.x);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float hat = (v.x[e] - mean) * rstd, dz = d.x[e] * act_slope(hat * w[e] + o[e], a.activation);
-        d.x[e] = rstd * (dz * w[e] - t1 - hat * t2);
-      }
+    for (int e = 0; e < VE; ++e) {
+      const float hat = (v[e] - mean) * rstd, dz = d.x[e] * act_slope(hat * w[e] + o[e], a.activation);
+      d.x[e] = row < k.len ? rstd * (dz * w[e] - t1 - hat * t2) : 0.0f;
     }
     d.store(dx + (long long)row * a.channels);
-  }
+  });
 }
 
 // ---- any: one workgroup per (sample, group), re-reading -----------------------------------------------------------------------------------
@@ -773,7 +799,7 @@ Plan plan(const Args& a) {
 }
 
 long long work_floats(const Args& a, const Plan& p, bool backward) {
-  const long long pairs = p.form == LONG ? 2LL * a.batch * p.blocks * a.groups : 0;
+  const long long pairs = p.form == LONG ? 2LL * a.batch * (p.blocks + 1) * a.groups : 0;
   return pairs + (backward && a.weight != nullptr ? 2LL * p.records * a.channels : 0);
 }
 
@@ -793,12 +819,14 @@ void launch_slab(const Args& a, const Plan& p, bool backward, hipStream_t st) {
 
 template <typename T, int VE>
 void launch_long(const Args& a, const Plan& p, bool backward, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)a.batch * p.blocks * p.slices);
+  const unsigned grid = (unsigned)((long long)a.batch * p.blocks * p.slices), join = (unsigned)(((long long)a.batch * a.groups + 3) / 4);
   if (backward) {
     long_sum_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
+    long_join_kernel<true><<<join, 256, 0, st>>>(a, p);
     long_dx_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
   } else {
     long_stat_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
+    long_join_kernel<false><<<join, 256, 0, st>>>(a, p);
     long_apply_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
   }
 }
@@ -831,7 +859,7 @@ void launch(const Args& a, const Plan& p, bool backward, hipStream_t st) {
 int run(const Args* args, bool backward, const char* entry, void* stream) {
   if (args == nullptr || !sizes_ok(*args)) return fail(entry, -22);
   const Args& a = *args;
-  if (a.x == nullptr || a.stats == nullptr || a.activation < 0 || a.activation > 3 || (a.weight == nullptr) != (a.bias == nullptr) ||
+  if (a.x == nullptr || a.stats == nullptr || (reinterpret_cast<uintptr_t>(a.stats) | reinterpret_cast<uintptr_t>(a.work)) % 8 != 0 || a.activation < 0 || a.activation > 3 || (a.weight == nullptr) != (a.bias == nullptr) ||
       (a.weight_type != TYPE_F32 && a.weight_type != a.type) || !(a.eps >= 0.0f))
     return fail(entry, -22);
   if (!backward && a.y == nullptr) return fail(entry, -22);

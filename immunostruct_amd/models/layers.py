@@ -8,6 +8,9 @@
   ever passed on this path (reference ``models/layers.py:51-106``).
 
 Both evaluate through one shared routine (:func:`attend`).
+
+* ``DifferentialAttention(feature_dim, n_head, ...)`` -- not in the reference: the difference of two softmax maps with learned weights, for
+  residue sequences and padded graphs (positions, lengths, causal order, grouped keys), every step a HIP kernel.
 """
 from __future__ import annotations
 
@@ -134,3 +137,71 @@ class MultiHeadAttention(nn.Module):
             return out.mean(dim=1), w
         return attend_pooled_mean(x, self.w_q.weight, self.w_q.bias, self.w_k.weight, self.w_k.bias,
                                   self.w_v.weight, self.w_v.bias, self.n_head, need_weights, qk=qk, out_proj=self.w_concat)
+
+
+class DifferentialAttention(nn.Module):
+    """Differential attention block over (B, n, input_dim): per head ``(softmax(q1 k1^T / sqrt(d)) - lam softmax(q2 k2^T / sqrt(d))) v``, each
+    position's head outputs normalised on their own, then the output projection.
+
+    Head width d = ``feature_dim / (2 n_head)``, values 2 d wide; ``kv_heads`` < n_head: query heads share keys and values.  ``lam`` of a head is
+    ``exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) + lambda_init``, learned.  ``rotary``: an ``nn.RotaryEmbedding`` applied to q and k.
+    The norm's weight starts at ``1 - lambda_init``, which keeps the block's scale that of plain attention.
+
+    ``forward(x, positions=None, lengths=None, causal=None) -> (B, n, feature_dim)``: see ``functional.differential_attention``; rows at or behind
+    ``lengths`` come back as zeros.  ``attend_cached`` is the same for new tokens over a cache of keys and values."""
+
+    def __init__(self, feature_dim, n_head, kv_heads=None, input_dim=None, lambda_init=0.8, rotary=None):
+        super().__init__()
+        kv_heads = kv_heads or n_head
+        if feature_dim % (2 * n_head) != 0 or n_head % kv_heads != 0:
+            raise ValueError("feature_dim must be divisible by 2 n_head, n_head by kv_heads")
+        from ..nn import GroupNorm
+        input_dim = input_dim or feature_dim
+        self.n_head, self.kv_heads, self.lambda_init, self.rotary = n_head, kv_heads, lambda_init, rotary
+        self.head_dim = d = feature_dim // (2 * n_head)
+        if rotary is not None and rotary.dims > d:
+            raise ValueError(f"the rotary embedding turns {rotary.dims} elements of heads of {d}")
+        self.w_q = nn.Linear(input_dim, feature_dim)
+        self.w_k = nn.Linear(input_dim, 2 * kv_heads * d)
+        self.w_v = nn.Linear(input_dim, 2 * kv_heads * d)
+        self.w_concat = nn.Linear(feature_dim, feature_dim)
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            self.register_parameter(name, nn.Parameter(0.1 * torch.randn(n_head, d)))
+        self.norm = GroupNorm(n_head, feature_dim)
+        nn.init.constant_(self.norm.weight, 1.0 - lambda_init)
+
+    def lam(self):
+        """(n_head,) weights of the second map, fp32"""
+        first = (self.lambda_q1.float() * self.lambda_k1.float()).sum(dim=1).exp()
+        return first - (self.lambda_q2.float() * self.lambda_k2.float()).sum(dim=1).exp() + self.lambda_init
+
+    def project(self, x, positions=None):
+        """(q, k, v) of the positions of x, turned: what a cache keeps of them is k (B, n, 2 kv_heads, d) and v (B, n, kv_heads, 2 d)"""
+        b, n, _ = x.shape
+        q = self.w_q(x).view(b, n, 2 * self.n_head, self.head_dim)
+        k = self.w_k(x).view(b, n, 2 * self.kv_heads, self.head_dim)
+        v = self.w_v(x).view(b, n, self.kv_heads, 2 * self.head_dim)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, positions)
+        return q, k, v
+
+    def attend_cached(self, q, k, v, lengths=None, causal=None):
+        """the block's output for projected queries over projected keys and values (the rows a cache holds): (B, nq, feature_dim)"""
+        from .. import functional as HF
+        b, n = q.shape[:2]
+        y = HF.differential_attention(q, k, v, self.lam(), lengths, causal)
+        return self.w_concat(self.norm(y.view(b * n, -1)).view(b, n, -1))
+
+    def forward(self, x, positions=None, lengths=None, causal=None):
+        out = self.attend_cached(*self.project(x, positions), lengths, causal)
+        if lengths is not None:
+            there = torch.arange(x.shape[1], device=x.device) < lengths[:, None]
+            out = out.masked_fill(~there[:, :, None], 0.0)
+        return out
+
+    def pooled_mean(self, x, positions=None, lengths=None):
+        """mean of the block's output over each sample's rows (an empty sample: zeros)"""
+        out = self.forward(x, positions, lengths)
+        if lengths is None:
+            return out.mean(dim=1)
+        return out.sum(dim=1) / lengths.clamp(min=1)[:, None].to(out.dtype)

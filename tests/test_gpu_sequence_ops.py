@@ -347,3 +347,89 @@ def test_token_equals_the_last_row_of_the_prompt(cuda_device):
         token = HF.differential_attention(q[:, -1:], k, v, lam, None, "end")
         _within(token, (whole[0][:, -1:], whole[1][:, -1:]), "token")
         _within(HF.differential_attention(q, k, v, lam, None, "start"), whole, "prompt")
+
+
+def _plain_block(m, x, positions, lengths, causal):
+    """models.layers.DifferentialAttention in float64 on the CPU, from elementary operations"""
+    p = {k: v.detach().cpu().double().requires_grad_(True) for k, v in m.named_parameters()}
+    x = x.detach().cpu().double().requires_grad_(True)
+    b, n, _ = x.shape
+    h, hk, d = m.n_head, m.kv_heads, m.head_dim
+    lin = lambda name, t: t @ p[name + ".weight"].t() + p[name + ".bias"]
+    q, k, v = lin("w_q", x).view(b, n, 2 * h, d), lin("w_k", x).view(b, n, 2 * hk, d), lin("w_v", x).view(b, n, hk, 2 * d)
+    if m.rotary is not None:
+        t = positions.cpu().double().expand(b, n)[:, :, None, None] * m.rotary.freq
+        half = m.rotary.freq.numel()
+        turn = lambda z: torch.cat([z[..., :half] * t.cos() - z[..., half:2 * half] * t.sin(), z[..., :half] * t.sin() + z[..., half:2 * half] * t.cos(),
+                                    z[..., 2 * half:]], dim=-1)
+        q, k = turn(q), turn(k)
+    lam = (p["lambda_q1"] * p["lambda_k1"]).sum(1).exp() - (p["lambda_q2"] * p["lambda_k2"]).sum(1).exp() + m.lambda_init
+    at, length = torch.arange(n), torch.full((b,), n) if lengths is None else lengths.cpu().long()
+    seen = (at < length[:, None, None]).expand(b, n, n)
+    if causal is not None:
+        seen = seen & (at[None, None, :] <= at[None, :, None] + ((length - n)[:, None, None] if causal == "end" else 0))
+    maps = []
+    for j in range(2):
+        s = torch.einsum("bihd,bjhd->bhij", q[:, :, j::2], k[:, :, j::2].repeat_interleave(h // hk, dim=2)) / d ** 0.5
+        s = s.masked_fill(~seen[:, None], -1e300)
+        maps.append(torch.softmax(s, -1).masked_fill(~seen[:, None], 0.0))
+    y = torch.einsum("bhij,bjhd->bihd", maps[0] - lam[:, None, None] * maps[1], v.repeat_interleave(h // hk, dim=2))
+    y = (y - y.mean(-1, keepdim=True)) / torch.sqrt(y.var(-1, correction=0, keepdim=True) + m.norm.eps)
+    y = lin("w_concat", y.reshape(b, n, -1) * p["norm.weight"] + p["norm.bias"])
+    return y.masked_fill((at >= length[:, None])[:, :, None], 0.0), x, p
+
+
+@pytest.mark.parametrize("heads,kv,dims,causal,ragged", [(1, 1, 0, None, True), (4, 2, 8, "start", False), (2, 1, 16, "end", True)])
+def test_differential_attention_module(cuda_device, heads, kv, dims, causal, ragged):
+    """the whole block in fp32, values and every gradient against float64: relative to each tensor's largest entry within 2e-4 (a chain of three
+    products of up to 64 terms, a softmax and a norm whose rstd of up to ~10 multiplies all of their errors: 10 * 3 * (64 + 72) * 2^-24 = 2.4e-4
+    if every rounding had its worst sign)"""
+    from immunostruct_amd.models.layers import DifferentialAttention
+    torch.manual_seed(5)
+    rope = HN.RotaryEmbedding(dims) if dims else None
+    m = DifferentialAttention(64, heads, kv_heads=kv, input_dim=20, rotary=rope).cuda()
+    with torch.no_grad():
+        m.norm.bias.normal_()
+    x = _randn(3, 83, 20, dtype=torch.float32, seed=71).requires_grad_(True)
+    pos = torch.arange(83, device="cuda") + 5
+    lens = torch.tensor([83, 40, 11], dtype=torch.int32, device="cuda") if ragged else None
+    want, xd, p = _plain_block(m, x, pos, lens, causal)
+    got = m(x, pos, lens, causal)
+    dy = torch.randn(want.shape, generator=torch.Generator().manual_seed(9))
+    want.backward(dy.double())
+    got.backward(dy.cuda())
+
+    def close(a, b, what, top=None):
+        top = float(b.detach().abs().max()) if top is None else top
+        off = float((a.detach().cpu().double() - b.detach()).abs().max())
+        assert off <= 2e-4 * top, f"{what}: {off / top:.2e}"
+
+    close(got, want, "out")
+    close(x.grad, xd.grad, "dx")
+    for name, par in m.named_parameters():
+        # a bias' gradient is a sum of the terms its layer's weight gradient multiplies with x (of order 1): that is what its rounding is relative
+        # to (w_k.bias without positions: it adds the same to a row's scores, the terms cancel and the gradient is 0)
+        weight = p[name.replace("bias", "weight")]
+        close(par.grad, p[name].grad, name, float(max(weight.grad.abs().max(), p[name].grad.abs().max())))
+    if causal is None:
+        mean = m.pooled_mean(x, pos, lens)
+        n = torch.tensor([83.0, 40.0, 11.0]) if ragged else torch.full((3,), 83.0)
+        close(mean, want.sum(1) / n[:, None].double(), "mean")
+
+
+def test_module_token_by_token(cuda_device):
+    """serving: projecting one position at a time into a cache and attending over it gives the whole causal pass"""
+    from immunostruct_amd.models.layers import DifferentialAttention
+    torch.manual_seed(6)
+    m = DifferentialAttention(64, 4, kv_heads=2, rotary=HN.RotaryEmbedding(8)).cuda().to(torch.bfloat16)
+    x = _randn(2, 9, 64, dtype=torch.bfloat16, seed=72)
+    with torch.no_grad():
+        whole = m(x, torch.arange(9, device="cuda"), None, "start")
+        k, v = torch.full((2, 16, 4, 8), float("nan"), dtype=torch.bfloat16, device="cuda"), torch.full((2, 16, 2, 16), float("nan"), dtype=torch.bfloat16, device="cuda")
+        for t in range(9):
+            q, kt, vt = m.project(x[:, t:t + 1], torch.tensor([t], device="cuda"))
+            k[:, t:t + 1], v[:, t:t + 1] = kt, vt
+            one = m.attend_cached(q, k, v, torch.full((2,), t + 1, dtype=torch.int32, device="cuda"), "end")
+            # two summation orders ahead of roundings to bf16 (2^-8 each) of the block's steps: attention, norm (whose rstd of up to ~10
+            # multiplies the attention's), projection
+            assert float((one[:, 0] - whole[:, t]).abs().max()) <= 12 * 2.0 ** -8 * float(whole.abs().max())
