@@ -194,6 +194,27 @@ def load():
     return lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The sequence operators' autograd functions (``csrc/torch_ops.cpp``, built beside the library), bound to this process' library."""
+    global _torch_ops
+    if _torch_ops is None:
+        path = os.path.join(_HERE, "csrc", "immunostruct_torch.so")
+        if not os.path.isfile(path):
+            raise HipExtensionError(f"{path} not found: build it with `make -C immunostruct_amd/csrc`. There is no fallback.")
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("immunostruct_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        lib = load()
+        names = ["is_last_error_string"] + [n for n in SIGNATURES if n.startswith(("is_rotary", "is_diff_attention", "is_group_norm"))]
+        module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, HipExtensionError)
+        _torch_ops = module
+    return _torch_ops
+
+
 def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
@@ -231,18 +252,6 @@ def rows_ld(t):
     if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
     return t, int(t.stride(0))
-
-
-def last_contiguous(t):
-    """the tensor itself, or a contiguous copy where its innermost dimension is not laid out element by element (a broadcast input)"""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def sequence_rows(t):
-    """the (B, n, heads, width) tensor itself, or a contiguous copy where the innermost dimension is not laid out element by element or the
-    rows of a tile lie too far apart for the attention kernels' 32-bit offsets"""
-    _, n, h, w = t.stride()
-    return t if w == 1 and n < 2 ** 23 and h * t.shape[2] < 2 ** 27 else t.contiguous()
 
 
 def same_device(first, *tensors):

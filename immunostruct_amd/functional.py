@@ -8,7 +8,6 @@ stream.  There is no fallback path: CPU tensors raise ``HipExtensionError``.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -1759,39 +1758,17 @@ def vae_loss(recon, x, mu, logvar, logit, y, mode, pos_weight, c_pred, c_mse, c_
 
 
 # ---- operators of attention blocks over sequences (csrc/rotary.hip, diff_attention*.hip, group_norm.hip) ----------------------------------
-# fp32, bf16 and fp16; they run on the tensors' own device and its current stream, also where that device is not the current one.
-
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-
-
-def _enqueue(name, entry, index, *args):
-    """one call of a C entry point on device ``index`` and that device's current stream (the arguments end with the stream)"""
-    if KernelTimer.enabled or index != _current_device():
-        with torch.cuda.device(index), KernelTimer.span(name):
-            code = entry(*args, _raw_stream(index))
-    else:      # (the common case spends nothing on contexts: small launches are bound by what the host does per call)
-        code = entry(*args, _raw_stream(index))
-    if code:
-        _lib.check(code, name)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _aligned(t):
-    """contiguous and 16-byte aligned (an incoming gradient may be any view)"""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
+# fp32, bf16 and fp16; they run on the tensors' own device and its current stream, also where that device is not the current one.  Arguments are
+# checked here, the autograd functions are C++ (csrc/torch_ops.cpp): small calls are bound by the host.
 
 def _sequence_type(name, *tensors):
     """raises unless the operator's tensors have one element type that the kernels are built for"""
     t = tensors[0].dtype
     if t not in _lib.TYPES:
         raise ValueError(f"{name}: expected float32, bfloat16 or float16 tensors, got {t}")
-    if any(u is not None and u.dtype != t for u in tensors):
-        raise ValueError(f"{name}: tensors of different types {[u.dtype for u in tensors if u is not None]}")
+    for u in tensors:
+        if u is not None and u.dtype != t:
+            raise ValueError(f"{name}: tensors of different types {t} and {u.dtype}")
 
 
 def _check_lengths(name, lengths, batch):
@@ -1800,56 +1777,6 @@ def _check_lengths(name, lengths, batch):
     if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch:
         raise ValueError(f"{name}: lengths has to be an int32 tensor of ({batch},)")
     return lengths.contiguous()
-
-
-def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _rotary_launch(q, k, freq, positions, layout, amplitude, inverse):
-    lib = _lib.load()
-    b, n, _, width = q.shape
-    args, outs = [], [None, None]
-    for i, t in enumerate((q, k)):
-        if t is None:
-            args += (None, 0, 0, 0, None, 0)
-        else:
-            # (a copy, where one is made, is freed behind the launch in the order of its stream)
-            t = _lib.last_contiguous(t)
-            outs[i] = torch.empty_like(t, memory_format=torch.contiguous_format)
-            args += (t.data_ptr(), *t.stride()[:3], outs[i].data_ptr(), t.shape[2])
-    if b == 0 or n == 0:
-        return outs
-    pos = (None, 0, 0, 0)
-    if positions is not None:
-        pos = (positions.data_ptr(), positions.dtype == torch.int64, positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1))
-    _enqueue("is_rotary", lib.is_rotary, q.get_device(), *args, *pos, freq.data_ptr(), b, n, width, 2 * freq.numel(), layout == "interleaved",
-             inverse, amplitude, _lib.TYPES[q.dtype])
-    return outs
-
-
-class RotaryFn(torch.autograd.Function):
-    """q (B, n, heads, width) and k (B, n, kv_heads, width) turned by their positions in one launch (``csrc/rotary.hip``); the backward is
-    the opposite turn."""
-
-    @staticmethod
-    def forward(ctx, q, k, freq, positions, layout, amplitude):
-        ctx.set_materialize_grads(False)
-        ctx.cfg = (freq, layout, amplitude)
-        ctx.save_for_backward(positions)
-        q_out, k_out = _rotary_launch(q, k, freq, positions, layout, amplitude, False)
-        return q_out if k is None else (q_out, k_out)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk=None):
-        (positions,) = ctx.saved_tensors
-        freq, layout, amplitude = ctx.cfg
-        if gq is not None:
-            gq, gk = _rotary_launch(gq, gk, freq, positions, layout, amplitude, True)
-        elif gk is not None:
-            gk, _ = _rotary_launch(gk, None, freq, positions, layout, amplitude, True)
-        return gq, gk, None, None, None, None
 
 
 def rotary(q, k, freq, positions=None, layout="half", amplitude=1.0):
@@ -1871,67 +1798,10 @@ def rotary(q, k, freq, positions=None, layout="half", amplitude=1.0):
                                   or tuple(positions.shape) not in ((q.shape[1],), (q.shape[0], q.shape[1]))):
         raise ValueError("rotary: positions has to be an int32 / int64 tensor of (n,) or (B, n)")
     _lib.same_device(q, k, positions)
-    freq, amplitude = freq.contiguous(), float(amplitude)
-    if not _needs_grad(q, k):
-        return tuple(_rotary_launch(q, k, freq, positions, layout, amplitude, False))
-    out = RotaryFn.apply(q, k, freq, positions, layout, amplitude)
-    return out if k is not None else (out, None)
+    return _lib.torch_ops().rotary(q, k, freq.contiguous(), positions, layout == "interleaved", float(amplitude))
 
 
 _CAUSAL = {None: 0, "start": 1, "end": 2}
-
-
-def _diff_forward(q, k, v, lam, lengths, causal, scale, need):
-    """launches of the forward pass -> (out, o2, lse, arguments); o2 and lse (what the backward needs) are None unless ``need``"""
-    lib = _lib.load()
-    b, nq, h2, d = q.shape
-    nk, hk, dv = v.shape[1:]
-    heads = h2 // 2
-    rows = nq * heads // hk
-    out = torch.empty(b, nq, heads, dv, dtype=q.dtype, device=q.device)
-    o2 = torch.empty_like(out) if need else None
-    lse = torch.empty(b, hk, 2, rows, dtype=torch.float32, device=q.device) if need else None
-    if out.numel() == 0 or nk == 0:      # nobody asks, or there is nothing to see
-        return out.zero_(), o2, lse, None
-    splits = lib.is_diff_attention_splits(b, hk, rows, nk)
-    floats = lib.is_diff_attention_work_floats(b, hk, rows, dv, splits)
-    work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    a = _lib.DiffAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(lengths), out.data_ptr(), _ptr(o2), _ptr(lse), _ptr(work),
-                           None, None, None, None, None, None, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                           b, nq, nk, heads, hk, d, dv, causal, _lib.TYPES[q.dtype], _lib.TYPES[lam.dtype], splits, 1, 0, 0, 0, 0, scale)
-    _enqueue("is_diff_attention_fwd", lib.is_diff_attention_fwd, q.get_device(), ctypes.byref(a))
-    return out, o2, lse, a
-
-
-class DifferentialAttentionFn(torch.autograd.Function):
-    """The difference of two softmax maps over shared values (``csrc/diff_attention.h``); see :func:`differential_attention`."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, lam, lengths, causal, scale):
-        q, k, v, lam = _lib.sequence_rows(q), _lib.sequence_rows(k), _lib.sequence_rows(v), lam.contiguous()
-        out, o2, lse, ctx.args = _diff_forward(q, k, v, lam, lengths, causal, scale, True)
-        ctx.save_for_backward(q, k, v, lam, lengths, out, o2, lse)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        lib = _lib.load()
-        q, k, v, lam, lengths, out, o2, lse = ctx.saved_tensors
-        dq, dk, dv, dlam = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, lam))
-        if ctx.args is None:
-            return dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), None, None, None
-        g = g.contiguous()
-        a = _lib.DiffAttention.from_buffer_copy(ctx.args)      # (the forward's arguments with this call's buffers; its workspace is gone)
-        b, hk, _, rows = lse.shape
-        a.splits, a.row_splits = 1, lib.is_diff_attention_row_splits(b, hk, rows, a.nk, a.causal)
-        floats = lib.is_diff_attention_row_work_floats(b, hk, a.nk, a.d, a.dv, a.row_splits)
-        # (scratch for the rows' three dot products, behind the row splits' sums)
-        work = torch.empty(floats + 3 * b * hk * rows, dtype=torch.float32, device=q.device)
-        a.work, dots = work.data_ptr(), work.data_ptr() + 4 * floats
-        a.d_o, a.dots, a.dq, a.dk, a.dv_out, a.dlam = g.data_ptr(), dots, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr()
-        _enqueue("is_diff_attention_bwd", lib.is_diff_attention_bwd, q.get_device(), ctypes.byref(a))
-        return dq, dk, dv, dlam, None, None, None
 
 
 def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
@@ -1964,58 +1834,10 @@ def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
     if d > limit or dv > 2 * limit:
         raise NotImplementedError(f"differential_attention: heads of {d} / values of {dv} elements (the kernels: up to {limit} / {2 * limit} in {q.dtype})")
     _lib.same_device(q, k, v, lam, lengths)
-    if not _needs_grad(q, k, v, lam):
-        return _diff_forward(_lib.sequence_rows(q), _lib.sequence_rows(k), _lib.sequence_rows(v), lam.contiguous(), lengths, _CAUSAL[causal], scale, False)[0]
-    return DifferentialAttentionFn.apply(q, k, v, lam, lengths, _CAUSAL[causal], scale)
+    return _lib.torch_ops().differential_attention(q, k, v, lam, lengths, _CAUSAL[causal], scale)
 
 
 _ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "relu": 3}
-
-
-def _group_norm_launch(x, weight, bias, lengths, groups, eps, activation):
-    """-> (y, stats, arguments); x (B, n, channels) with a unit innermost stride"""
-    lib = _lib.load()
-    b, n, c = x.shape
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    if y.numel() == 0:
-        return y, None, None
-    stats = torch.empty(b, groups, 2, dtype=torch.float32, device=x.device)
-    a = _lib.GroupNorm(x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(lengths), y.data_ptr(), stats.data_ptr(), None, None, None, None, None,
-                       x.stride(0), x.stride(1), b, n, c, groups, activation, _lib.TYPES[x.dtype],
-                       0 if weight is None else _lib.TYPES[weight.dtype], 0, eps)
-    floats = lib.is_group_norm_work_floats(ctypes.byref(a), 0)
-    work = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-    a.work = _ptr(work)
-    _enqueue("is_group_norm_fwd", lib.is_group_norm_fwd, x.get_device(), ctypes.byref(a))
-    return y, stats, a
-
-
-class GroupNormFn(torch.autograd.Function):
-    """Group norm with an activation, channels last (``csrc/group_norm.hip``); see :func:`group_norm`.  x (B, n, channels)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, lengths, groups, eps, activation):
-        x = _lib.last_contiguous(x)
-        y, stats, ctx.args = _group_norm_launch(x, weight, bias, lengths, groups, eps, activation)
-        ctx.save_for_backward(x, weight, bias, lengths, stats)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        lib = _lib.load()
-        x, weight, bias, lengths, stats = ctx.saved_tensors
-        dx, dw, db = (None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, weight, bias))
-        if ctx.args is None:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None, None, None
-        a = _lib.GroupNorm.from_buffer_copy(ctx.args)
-        g = _aligned(g)
-        floats = lib.is_group_norm_work_floats(ctypes.byref(a), 1)
-        work = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-        a.y, a.dy, a.dx = None, g.data_ptr(), dx.data_ptr()
-        a.dweight, a.dbias, a.work = _ptr(dw), _ptr(db), _ptr(work)
-        _enqueue("is_group_norm_bwd", lib.is_group_norm_bwd, x.get_device(), ctypes.byref(a))
-        return dx, dw, db, None, None, None, None
 
 
 def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lengths=None):
@@ -2045,8 +1867,5 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, len
         raise ValueError("group_norm: eps has to be a number >= 0")
     _lib.same_device(x, weight, bias, lengths)
     x3 = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
-    if _needs_grad(x, weight, bias):
-        y = GroupNormFn.apply(x3, weight, bias, lengths, int(groups), eps, _ACTIVATIONS[activation])
-    else:
-        y = _group_norm_launch(_lib.last_contiguous(x3), weight, bias, lengths, int(groups), eps, _ACTIVATIONS[activation])[0]
-    return y.view(x.shape)
+    y = _lib.torch_ops().group_norm(x3, weight, bias, lengths, groups, eps, _ACTIVATIONS[activation])
+    return y if x3 is x else y.view(x.shape)

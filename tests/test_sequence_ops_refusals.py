@@ -125,3 +125,9 @@ def test_group_norm_module_refuses():
     with pytest.raises(ValueError):
         GroupNorm(3, 8)
     assert [tuple(p.shape) for p in GroupNorm(2, 8).parameters()] == [(8,), (8,)] and not list(GroupNorm(2, 8, affine=False).parameters())
+
+
+def test_autograd_functions_load_and_raise_the_package_error():
+    """the C++ side loads against this torch and is bound to the library; host tensors never reach it through the package"""
+    ops = _lib.torch_ops()
+    assert ops is _lib.torch_ops() and all(callable(getattr(ops, n)) for n in ("rotary", "differential_attention", "group_norm"))
