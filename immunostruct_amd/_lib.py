@@ -96,7 +96,7 @@ SIGNATURES = {
     "is_recon_mse": [_P, _P, _P, _LL, _F, _P, _P],
     "is_vae_loss": [_P, _P, _P, _LL, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _F, _F, _F, _F, _P, _P, _P, _P],
     "is_rotary": [_P, _LL, _LL, _LL, _P, _I, _P, _LL, _LL, _LL, _P, _I, _P, _I, _LL, _LL, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P],
-    "is_diff_attention_splits": [_I, _I, _I, _I],
+    "is_diff_attention_splits": [_I, _I, _I, _I, _I],
     "is_diff_attention_work_floats": [_I, _I, _I, _I, _I],
     "is_diff_attention_row_splits": [_I, _I, _I, _I, _I],
     "is_diff_attention_row_work_floats": [_I, _I, _I, _I, _I, _I],

@@ -12,9 +12,8 @@
 //             and the product with dO once per map (48 matrix instructions per 32 x 32 tile at d = 64 for 32) and is still far ahead:
 //             with both maps in one wave dK / dV took 849 us at (2, 4096, 16 / 4 heads, 64 / 128, bf16, causal), one wave per SIMD.
 //   forward   one pass over the keys: S^T = K Q^T (a lane owns one query), running maximum and sum in 32 bits, O^T += V^T P^T.
-//             The weights are formed with the old maximum first; only when a lane's 16 add up to more than 2^10 (far inside every type)
-//             the tile's maximum is looked for and the accumulators are rescaled: two thirds of the vector work of a tile is then
-//             the exponentials themselves, which bound the kernel beside the matrix instructions.
+//             The maximum only moves when a score passes it by 2^8 (the weights stay <= 2^8, far inside every type), which makes
+//             the rescaling of the accumulators rare.
 //   backward  dP = dO V^T; D_m = dO . O_m; dS_1 = P1 (dP - D_1), dS_2 = -lam P2 (dP - D_2);
 //             dQ_m = scale dS_m K_m, dK_m = scale dS_m^T Q_m, dV = (P1 - lam P2)^T dO, dlam = -sum D_2.  Scores are recomputed from lse.
 //             dK / dV: a wave owns 32 keys and walks the rows; dQ: a wave owns 32 rows and walks the keys.
@@ -27,7 +26,7 @@ namespace is {
 namespace da {
 
 typedef IsDiffAttention Args;
-constexpr float SLACK = 1024.0f;      // how far a lane's 16 weights may add up before the running maximum follows
+constexpr float SLACK = 8.0f;      // log2 of how far a weight may pass 1 before the running maximum follows
 
 template <int V> struct Int { static constexpr int value = V; };
 // steps j0 = first, first + STEP ... below last, alternating between two buffers whose number is a compile-time constant
@@ -201,29 +200,14 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
       if (more) fetch(j0 + KT);
       if (j0 < wave_end) {
         f32x16 p = mm_tile<T, D>(buf + k_at, q);
-        auto hide = [&]() {
-          if (j0 + KT > wave_all) {
+        if (j0 + KT > wave_all) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t) p[t] = j0 + tile_row(t, g) >= my_end ? -INFINITY : p[t];
-          }
-        };
-        float add;
-        auto weights = [&]() {
-          add = 0.0f;
+          for (int t = 0; t < 16; ++t) p[t] = j0 + tile_row(t, g) >= my_end ? -INFINITY : p[t];
+        }
+        float high = p[0];
 #pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            p[t] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t], c, ref));
-            add += p[t];
-          }
-        };
-        hide();
-        weights();
-        if (__any(add > SLACK || top == -INFINITY)) {      // (rare: the scores are formed again rather than kept)
-          p = mm_tile<T, D>(buf + k_at, q);
-          hide();
-          float high = p[0];
-#pragma unroll
-          for (int t = 1; t < 16; ++t) high = fmaxf(high, p[t]);
+        for (int t = 1; t < 16; ++t) high = fmaxf(high, p[t]);
+        if (__any((high - top) * c > SLACK)) {
           const float now = fmaxf(top, fmaxf(high, other_half(high)));
           const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - now) * c);
           top = now;
@@ -233,7 +217,12 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[t][e] *= shrink;
-          weights();
+        }
+        float add = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          p[t] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t], c, ref));
+          add += p[t];
         }
         sum += add;
         mm_transposed<T, DV, NT>(o, buf + v_at, p);
@@ -383,10 +372,15 @@ __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
   __shared__ float part[16];
   const int h = blockIdx.x, hk = h / a.group, gi = h % a.group, R = a.rows;
   float s = 0.0f;
-  for (long long x = threadIdx.x; x < (long long)a.batch * a.nq; x += 1024) {
-    const long long b = x / a.nq;
-    const int i = (int)(x - b * a.nq);
-    s += a.dots[(2LL * a.batch * a.kv_heads + b * a.kv_heads + hk) * R + i * a.group + gi];
+  const unsigned total = (unsigned)a.batch * (unsigned)a.nq;      // (below 2^31, as the rows of all heads are)
+  for (unsigned x0 = threadIdx.x; x0 < total; x0 += 4096) {
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned x = x0 + u * 1024, b = x / (unsigned)a.nq, i = x - b * (unsigned)a.nq;
+      v[u] = x < total ? a.dots[(2LL * a.batch * a.kv_heads + b * a.kv_heads + hk) * R + i * a.group + gi] : 0.0f;
+    }
+    s += (v[0] + v[1]) + (v[2] + v[3]);
   }
   s = sum_over_r(s);
   s += other_half(s);

@@ -42,13 +42,16 @@ int run(const da::Args& a, bool backward, const char* entry, void* stream) {
 
 extern "C" {
 
-// Splits of the keys: enough workgroups for 256 CUs where the rows alone do not give them (a wave works on 32 rows; up to 32 rows are one
-// wave per workgroup, four of which fill a CU), at least 128 keys each.
-int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk) {
+// Splits of the keys, where the rows alone do not fill the chip.  Up to 32 rows (single tokens) a workgroup is one pair of waves and the call is
+// bound by the cache's bytes: 1024 workgroups, at least 128 keys each.  More rows: 256 workgroups in all, and only while a split has work enough to
+// pay for leaving its sums in memory: 512 keys in the 16-bit types, 128 in the 8 to 16 times slower 32-bit one.  Measured (us) for at
+// least 128 / 512 / 1024 keys: (1, 512 over 4096, 8 / 2 heads, 64) bf16 81 / 53 / 46, (2, 300 over 300, 8, 64) bf16 28 / 14 / 14, (1, 128 over 2048,
+// 4 / 1, 64) bf16 29 / 25 / 33, (1, 2048 over 2048, 2, 64) fp32 98 / 120 / 207; with 256 workgroups instead of 512 the last takes 76.
+int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk, int type) {
   if (batch < 1 || kv_heads < 1 || rows < 1 || nk < 1) return 1;
   const long long groups = (rows <= 32 ? 1LL : (rows + 127LL) / 128) * kv_heads * batch;
-  const long long want = rows <= 32 ? 1024 / groups : groups < 192 ? 512 / groups : 1, most = (nk + 127LL) / 128;
-  const long long s = want < most ? want : most;
+  const long long want = rows <= 32 ? 1024 / groups : groups < 128 ? 256 / groups : 1, least = rows <= 32 || type == TYPE_F32 ? 128 : 512;
+  const long long most = (nk + least - 1) / least, s = want < most ? want : most;
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 

@@ -147,7 +147,7 @@ Attended diff_forward(const Tensor& q, const Tensor& k, const Tensor& v, const T
     r.out.zero_();
     return r;
   }
-  a.splits = entry.splits(a.batch, a.kv_heads, rows, a.nk);
+  a.splits = entry.splits(a.batch, a.kv_heads, rows, a.nk, a.type);
   const long long need_floats = entry.work_floats(a.batch, a.kv_heads, rows, a.dv, a.splits);
   Tensor work;
   if (need_floats > 0) work = floats(q, {(int64_t)need_floats});

@@ -466,7 +466,7 @@ typedef struct {
   unsigned group_magic;
   float scale;
 } IsDiffAttention;
-int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk);
+int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk, int type);
 long long is_diff_attention_work_floats(int batch, int kv_heads, int rows, int dv, int splits);
 int is_diff_attention_row_splits(int batch, int kv_heads, int rows, int nk, int causal);
 long long is_diff_attention_row_work_floats(int batch, int kv_heads, int nk, int d, int dv, int row_splits);

@@ -150,7 +150,8 @@ def test_attention_strides_scale_and_types(cuda_device):
     for t in (q, k, v):
         o = torch.zeros(*t.shape[:3], t.shape[3] + 1, dtype=dtype, device="cuda")[..., 1:]
         odd.append(o.copy_(t))
-    assert torch.equal(HF.differential_attention(*odd, lam), base)
+    # (those run element by element in tiles of another width, another order of the same sums: within the bound, not bit for bit)
+    _within(HF.differential_attention(*odd, lam), SR.differential_attention(q, k, v, lam, None, None, 32 ** -0.5)["o"], "unaligned")
     column = [t.transpose(2, 3).contiguous().transpose(2, 3) for t in (q, k, v)]      # an innermost stride that is not 1: copied
     assert torch.equal(HF.differential_attention(*column, lam), base)
     want = SR.differential_attention(q, k, v, lam.float(), None, None, 0.3, base)

@@ -91,10 +91,10 @@ def test_entry_points_refuse_without_a_device():
 
 def test_splits_cover_the_chip():
     lib = _lib.load()
-    assert lib.is_diff_attention_splits(16, 4, 4, 16384) == 16      # single tokens: 64 workgroups alone
-    assert lib.is_diff_attention_splits(128, 1, 190, 190) <= 2
-    assert lib.is_diff_attention_splits(2, 4, 16384, 4096) == 1
-    assert lib.is_diff_attention_splits(1, 1, 1, 100) == 1 and lib.is_diff_attention_splits(1, 1, 1, 2 ** 20) == 64
+    assert lib.is_diff_attention_splits(16, 4, 4, 16384, 1) == 16      # single tokens: 64 workgroups alone
+    assert lib.is_diff_attention_splits(128, 1, 190, 190, 0) == 1 and lib.is_diff_attention_splits(2, 4, 16384, 4096, 1) == 1
+    assert lib.is_diff_attention_splits(1, 1, 1, 100, 2) == 1 and lib.is_diff_attention_splits(1, 1, 1, 2 ** 20, 0) == 64
+    assert lib.is_diff_attention_splits(1, 1, 256, 2048, 1) == 4 and lib.is_diff_attention_splits(1, 1, 256, 2048, 0) == 16
     assert lib.is_diff_attention_work_floats(16, 4, 4, 128, 1) == 0
     assert lib.is_diff_attention_work_floats(16, 4, 4, 128, 16) == 2 * 16 * 4 * 16 * 4 * 130
     assert lib.is_diff_attention_row_splits(2, 4, 16384, 4096, 1) == 2 and lib.is_diff_attention_row_splits(2, 4, 16384, 4096, 0) == 1
