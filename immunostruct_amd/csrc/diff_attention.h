@@ -397,14 +397,15 @@ __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
 // dK, dV of 32 keys per wave: grid (key tiles x row splits x kv_heads x batch), GROUPS x 2 waves.  row_splits > 1: the rows that see a key tile
 // are cut into equal parts, whose sums meet in the workspace (key_join_kernel): with a causal mask the first keys are seen by all rows and
 // the last by few, and one workgroup per key tile would leave half the chip idle half the time.
-// Map m's weight with its sign: P_1, -lam P_2; both waves run the same code on (lse, D, coefficient).
+// Both waves run the same code on (lse, D): map 1's weight is taken as +|lam| P_2 with |lam| folded into lse, and its results are negated when they
+// leave the wave.  Only where a lam of the group is negative do its rows' signs have to be put back (flip).
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) <= 128 ? 2 : 1))) void dkv_kernel(const Args a) {
   constexpr int GROUPS = key_groups<T, D>(), NTH = 128 * GROUPS, KEYS = 32 * GROUPS;
   constexpr int DV = 2 * D, RT = 32, NT = D / 32, NTV = DV / 32, NJ = D / (2 * Vec<T>::N), SZ = sizeof(T);
   constexpr int QB = Tile<T, D>::bytes(RT), OB = Tile<T, DV>::bytes(RT), BUF = 2 * QB + OB;
   __shared__ __align__(16) char lds[2 * BUF], vt[Tile<T, DV>::bytes(KEYS)];      // row tiles; the workgroup's own values
-  __shared__ __align__(16) float stat[2][2][3][RT];      // [buffer][map][lse, D, coefficient] of the tile's rows
+  __shared__ __align__(16) float stat[2][2][3][RT];      // [buffer][map][lse - log2 |coefficient|, D, its sign] of the tile's rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ki = lane & 31, g = lane >> 5;
   const int group = wave >> 1, map = wave & 1;
   const int R = a.rows, tiles = (a.nk + KEYS - 1) / KEYS;
@@ -422,6 +423,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
   f32x16 dk[NT], dv[NTV];
   zero_acc(dk);
   zero_acc(dv);
+  bool flip = false;
   const int seen_from = wg_key < len ? first_query(a, wg_key, len) * a.group / RT * RT : R;
   const int per = ((R - seen_from + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
   const int r_first = seen_from + split * per, r_last = min(R, r_first + per);
@@ -447,28 +449,36 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
     float st = 0.0f;
     const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + 2 * hk * a.group * a.q_h) * SZ;
     const char* op = reinterpret_cast<const char*>(a.d_o) + o_at(a, b, 0, hk * a.group) * SZ;
-    auto fetch = [&](int r0) {
-      unsigned qo[StageQ::PER], oo[StageO::PER];
-      const int i0 = r0 / a.group;
+    for (int gi = 0; gi < a.group; ++gi) flip = flip || lam_at<T>(a, hk * a.group + gi) < 0.0f;
+    static_assert(NTH >= 6 * RT, "a thread stages one statistic");
+    const int sw = tid >> 5, sm = sw >= 3 ? 1 : 0, sk = sw - 3 * sm;      // which statistic of which map
+    // a tile of 32 rows holds whole queries where the group divides 32: its rows' offsets then are the same in every tile
+    const bool whole = RT % a.group == 0;
+    unsigned qo[StageQ::PER], oo[StageO::PER];
+    float extra = 0.0f;      // what this thread's statistic takes of lam: -log2 |coefficient| or its sign
+    auto offsets = [&](int r0, int i0) {
       row_offsets<StageQ, 2>(a, qo, tid, r0, i0, (unsigned)a.q_n * SZ, 2u * (unsigned)a.q_h * SZ, (unsigned)a.q_h * SZ);
       row_offsets<StageO, 1>(a, oo, tid, r0, i0, (unsigned)(a.heads * a.dv) * SZ, (unsigned)a.dv * SZ, 0);
+      int gi;
+      query_of(a, min(r0 + (tid & 31), R - 1), gi);
+      const float lam = sm == 0 ? 1.0f : lam_at<T>(a, hk * a.group + gi);
+      extra = sk == 0 ? -__log2f(fabsf(lam)) : sk == 1 ? 0.0f : lam < 0.0f ? -1.0f : 1.0f;
+    };
+    offsets(r_first, r_first / a.group);
+    auto fetch = [&](int r0) {
+      const int i0 = r0 / a.group;
+      if (!whole || r0 + RT > R) offsets(r0, i0);
       sq.load(tid, qp + i0 * a.q_n * SZ, qo, a.d);
       so.load(tid, op + (long long)i0 * a.heads * a.dv * SZ, oo, a.dv);
       if (tid < 6 * RT) {
-        const int w = tid >> 5, m = w >= 3 ? 1 : 0, rw = min(r0 + (tid & 31), R - 1);
-        if (w - 3 * m < 2) {
-          st = (w == 3 * m ? a.lse : a.dots)[((long long)base * 2 + m) * R + rw];
-        } else {
-          int gi;
-          query_of(a, rw, gi);
-          st = m == 0 ? 1.0f : -lam_at<T>(a, hk * a.group + gi);
-        }
+        const int rw = min(r0 + (tid & 31), R - 1);
+        if (sk < 2) st = (sk == 0 ? a.lse : a.dots)[((long long)base * 2 + sm) * R + rw];
       }
     };
     auto place = [&](int buf) {
       sq.store(tid, lds + buf * BUF);
       so.store(tid, lds + buf * BUF + 2 * QB);
-      if (tid < 6 * RT) (&stat[buf][0][0][0])[tid] = st;
+      if (tid < 6 * RT) (&stat[buf][0][0][0])[tid] = st + extra;
     };
     fetch(r_first);
     place(0);
@@ -484,12 +494,19 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
         for (int u = 0; u < 4; ++u) {
           const f32x4 l = *reinterpret_cast<const f32x4*>(&stat[CUR][map][0][8 * u + 4 * g]);
           const f32x4 dd = *reinterpret_cast<const f32x4*>(&stat[CUR][map][1][8 * u + 4 * g]);
-          const f32x4 cf = *reinterpret_cast<const f32x4*>(&stat[CUR][map][2][8 * u + 4 * g]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = 4 * u + e;
-            w[t] = cf[e] * __builtin_amdgcn_exp2f(__builtin_fmaf(w[t], c, -l[e]));
+            w[t] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[t], c, -l[e]));
             ds[t] = w[t] * (ds[t] - dd[e]);
+          }
+        }
+        if (flip) {
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            const float f = stat[CUR][map][2][tile_row(t, g)];
+            w[t] *= f;
+            ds[t] *= f;
           }
         }
         if (r0 < wave_all || r0 + RT > R) {      // (the products are replaced, not the factors: nothing that stands in a hidden place gets through)
@@ -526,7 +543,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
     for (int u = 0; u < 4; ++u) {
       f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dk[t][4 * u + e] * a.scale;
+      for (int e = 0; e < 4; ++e) x[e] = dk[t][4 * u + e] * (map == 0 ? a.scale : -a.scale);
       put(map, 32 * t + 8 * u + 4 * g, x);
     }
   hand_over<NTV, GROUPS, 2 * BUF>(dv, lds, group, map, lane, [&](int t, const f32x16& x, const f32x16& y) {
@@ -534,7 +551,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
     for (int u = 0; u < 4; ++u) {
       f32x4 z;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = x[4 * u + e] + y[4 * u + e];
+      for (int e = 0; e < 4; ++e) z[e] = x[4 * u + e] - y[4 * u + e];
       put(2, 32 * t + 8 * u + 4 * g, z);
     }
   });
