@@ -186,8 +186,8 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
     sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
   auto place = [&](char* buf) {
-    sk.store(tid, buf);
-    sv.store(tid, buf + 2 * KB);
+    sk.store(tid, buf, a.d);
+    sv.store(tid, buf + 2 * KB, a.dv);
   };
   if (first < last) {      // (uniform over the workgroup, as is every barrier below)
     fetch(first);
@@ -435,12 +435,12 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
 #pragma unroll
     for (int j = 0; j < NJ; ++j) k[j] = load_chunk<T, VEC>(kp, 2 * j + g, a.d);
     {
-      typedef Stage<T, DV, KEYS, NTH, VEC, true> StageV;
+      typedef Stage<T, DV, KEYS, NTH, VEC> StageV;
       StageV sv;
       unsigned vo[StageV::PER];
       key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, len - 1 - wg_key);
       sv.load(tid, reinterpret_cast<const char*>(a.v) + (b * a.v_b + wg_key * a.v_n + hk * a.v_h) * SZ, vo, a.dv);
-      sv.store(tid, vt);
+      sv.store(tid, vt, a.dv);
     }
     typedef Stage<T, D, 2 * RT, NTH, VEC> StageQ;
     typedef Stage<T, DV, RT, NTH, VEC> StageO;
@@ -476,8 +476,8 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
       }
     };
     auto place = [&](int buf) {
-      sq.store(tid, lds + buf * BUF);
-      so.store(tid, lds + buf * BUF + 2 * QB);
+      sq.store(tid, lds + buf * BUF, a.d);
+      so.store(tid, lds + buf * BUF + 2 * QB, a.dv);
       if (tid < 6 * RT) (&stat[buf][0][0][0])[tid] = st + extra;
     };
     fetch(r_first);
@@ -607,13 +607,13 @@ __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_wa
 #pragma unroll
   for (int j = 0; j < NJ; ++j) q[j] = load_chunk<T, VEC>(qp, 2 * j + g, a.d);
   {
-    typedef Stage<T, DV, ROWS, NTH, VEC, true> StageG;
+    typedef Stage<T, DV, ROWS, NTH, VEC> StageG;
     StageG sg;
     unsigned offset[StageG::PER];
     const int r0 = tile * ROWS, i0 = r0 / a.group;
     row_offsets<StageG, 1>(a, offset, tid, r0, i0, (unsigned)(a.heads * a.dv) * SZ, (unsigned)a.dv * SZ, 0);
     sg.load(tid, reinterpret_cast<const char*>(a.d_o) + o_at(a, b, i0, hk * a.group) * SZ, offset, a.dv);
-    sg.store(tid, gt);      // (read behind the barrier that follows the first key tile)
+    sg.store(tid, gt, a.dv);      // (read behind the barrier that follows the first key tile)
   }
   const long long at = ((long long)base * 2 + map) * R + rr;
   const float l = a.lse[at], dd = a.dots[at], cf = map == 0 ? 1.0f : -lam_at<T>(a, head);
@@ -636,8 +636,8 @@ __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_wa
     sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
   auto place = [&](char* buf) {
-    sk.store(tid, buf);
-    sv.store(tid, buf + 2 * KB);
+    sk.store(tid, buf, a.d);
+    sv.store(tid, buf + 2 * KB, a.dv);
   };
   if (wg_end > 0) {
     fetch(0);

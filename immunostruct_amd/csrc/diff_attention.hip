@@ -12,7 +12,7 @@ int prepare(da::Args& a) {
   if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.lam == nullptr || a.o == nullptr) return -22;
   if (a.batch < 1 || a.nq < 1 || a.nk < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.d < 1 || a.dv < 1) return -22;
   if (a.type < TYPE_F32 || a.type > TYPE_F16 || (a.lam_type != TYPE_F32 && a.lam_type != a.type) || a.causal < 0 || a.causal > 2) return -22;
-  if (!(a.scale > 0.0f) || !(a.scale < INFINITY) || a.splits < 1 || a.row_splits < 1) return -22;
+  if (!(a.scale > 0.0f) || !(a.scale < 2e38f) || a.splits < 1 || a.splits > 64 || a.row_splits < 1) return -22;
   a.group = a.heads / a.kv_heads;
   a.group_magic = 0xffffffffu / (unsigned)a.group;
   const long long rows = (long long)a.nq * a.group, big = 0x7fffff00LL;
@@ -22,7 +22,7 @@ int prepare(da::Args& a) {
   a.rows = (int)rows;
   // a tile's rows lie within 31 bits of its first
   const long long near = 0x7fffffffLL / size;
-  if (a.q_n < 0 || a.q_h < 0 || a.k_n < 0 || a.v_n < 0 || a.q_n > near / 64 || a.k_n > near / 64 || a.v_n > near / 64 ||
+  if (a.q_n < 0 || a.q_h < 0 || a.k_n < 0 || a.k_h < 0 || a.v_n < 0 || a.k_h > near / 4 || a.q_n > near / 64 || a.k_n > near / 64 || a.v_n > near / 64 ||
       a.q_h > near / 4 / a.group || (long long)a.heads * a.dv > near / 64) return -22;
   const long long strides = a.q_b | a.q_n | a.q_h | a.k_b | a.k_n | a.k_h | a.v_b | a.v_n | a.v_h;
   a.vec = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.o) && aligned16(a.o2) && aligned16(a.d_o) && aligned16(a.dq) &&

@@ -6,14 +6,17 @@
 // Bound by bytes: x in and y out; x, dy in and dx out.  Forms, chosen by size (plan()):
 //   rows  n = 1, a group is a power of two of 16-byte chunks, at most 64: a group lives in neighbouring lanes, every sum is a few lane moves,
 //         a workgroup walks many samples and keeps its channels' dw / db sums in registers.
+//   wide  n = 1, groups of more chunks than a wave has lanes, 1024 at most: a workgroup per group, likewise over many samples
+//         ((8192, 1, 4096) bf16, one group: 43 us forward, 92 backward; as row blocks 174 and 379).
 //   slab  a workgroup holds all rows of one sample's slice of whole groups in registers (up to 16 chunks a thread): one read, exact two-step
 //         variance, one write.  Slices are as narrow as 64-byte row segments allow, so that small batches still fill the chip.
 //   long  a sample does not fit: row blocks leave (mean, M2) / (sum t, sum t xhat) of every group, a small launch joins a sample's blocks (one
 //         wave per sample and group; done by every workgroup of the next pass it cost 50 us at (2, 65536, 512), 32 groups), a third
 //         writes.  Block sums are taken about each thread's own first value, so a large mean costs no precision.
-//   any   groups of more than 256 chunks: one workgroup per (sample, group), re-reading.
+//         Groups of more than 256 chunks are cut into parts, which join like row blocks ((4, 2048, 4096) bf16, one group: 50 us forward, 94
+//         backward; a workgroup per sample and group that re-reads took 26 and 19 ms).
 // Chunks are 16 bytes where pointers, strides and the group width allow, single elements otherwise (a chunk never straddles two groups).
-// dw and db: one record [2][channels] per workgroup (rows), sample (slab, any) or row block (long), summed in a fixed order by a last launch.
+// dw and db: one record [2][channels] per workgroup (rows, wide), sample (slab) or row block (long), summed in a fixed order by a last launch.
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
 
@@ -21,13 +24,14 @@ namespace is {
 namespace gn {
 
 typedef IsGroupNorm Args;
-enum Form { ROWS, SLAB, LONG, ANY };
+enum Form { ROWS, WIDE, SLAB, LONG };
 struct Plan {
   Form form;
   int ve;              // elements of a chunk
   int slice, slices;   // channels of a workgroup (whole groups), their number
-  int per_thread;      // slab: chunks a thread holds
-  int blocks, rows;    // long: row blocks of a sample, rows of one; rows: workgroups
+  int per_thread;      // slab, wide: chunks a thread holds
+  int blocks, rows;    // long: row blocks of a sample, rows of one; rows, wide: workgroups
+  int parts;           // long: slices of a group (more than one: a slice is at most a group's part, the last one may be narrower)
   int records;         // of dw / db
 };
 
@@ -85,24 +89,17 @@ __device__ __forceinline__ float wave_sum(float v) {
   v = sum_over_r(v);
   return v + other_half(v);
 }
-__device__ __forceinline__ float block_sum(float v, float* scratch) {      // 256 threads; the sum in every thread
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
-}
 
 // Threads of a workgroup over a slice: thread = (row lane rl, column chunk col); cols chunks side by side, rl < lanes.
 struct Place {
   int cols, lanes, col, rl;
   bool on;
-  __device__ __forceinline__ Place(int slice, int ve) {
+  __device__ __forceinline__ Place(int slice, int ve, int width) {      // width: the channels of the slice that are there
     cols = slice / ve;
     lanes = 256 / cols;
     rl = threadIdx.x / cols;
     col = threadIdx.x - rl * cols;
-    on = rl < lanes;
+    on = rl < lanes && col * ve < width;
   }
 };
 // sum of v over a slice's group (the threads of cpg neighbouring columns and every row lane), in each of its threads.  256 floats of LDS each.
@@ -125,7 +122,7 @@ __device__ __forceinline__ float group_sum(float v, const Place& p, int cpg, flo
 }
 // the channels' sums of (dz xhat, dz) over the row lanes -> record [2][channels]
 template <int VE>
-__device__ __forceinline__ void channel_record(const float (&sw)[VE], const float (&sb)[VE], const Place& p, float* lds, float* record, int channels, int c0) {
+__device__ __forceinline__ void channel_record(const float (&sw)[VE], const float (&sb)[VE], const Place& p, float* lds, float* record, int channels, int c0, int there) {
   const int width = p.cols * VE;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -135,7 +132,7 @@ __device__ __forceinline__ void channel_record(const float (&sw)[VE], const floa
       for (int e = 0; e < VE; ++e) lds[p.rl * width + p.col * VE + e] = m == 0 ? sw[e] : sb[e];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < width; c += 256) {
+    for (int c = threadIdx.x; c < there; c += 256) {
       float s = 0.0f;
       for (int r = 0; r < p.lanes; ++r) s += lds[r * width + c];
       record[(long long)m * channels + c0 + c] = s;
@@ -244,13 +241,124 @@ __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, 
   }
 }
 
+// ---- wide: n = 1, a workgroup per group -----------------------------------------------------------------------------------------------
+template <typename T, int VE, int K, bool BACK>
+__global__ __launch_bounds__(256) void wide_kernel(const Args a) {
+  __shared__ float scratch[2][2][4];
+  const int g = blockIdx.y, cg = a.channels / a.groups, tid = threadIdx.x, c = g * cg + tid * VE;
+  bool on[K];
+  float w[K][VE], o[K][VE], sw[K][VE], sb[K][VE];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    on[k] = (tid + k * 256) * VE < cg;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      w[k][e] = on[k] ? param<T>(a, a.weight, c + k * 256 * VE + e, 1.0f) : 0.0f;
+      o[k][e] = on[k] ? param<T>(a, a.bias, c + k * 256 * VE + e, 0.0f) : 0.0f;
+      sw[k][e] = sb[k][e] = 0.0f;
+    }
+  }
+  const float inv = 1.0f / (float)cg;
+  auto sums = [&](float (&v)[2], float (&lds)[2][4]) {      // over the workgroup, in every thread
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      v[m] = wave_sum(v[m]);
+      if ((tid & 63) == 0) lds[m][tid >> 6] = v[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m) v[m] = (lds[m][0] + lds[m][1]) + (lds[m][2] + lds[m][3]);
+  };
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {      // (uniform: every barrier is met)
+    const bool live = length_of(a, b) > 0;
+    Chunk<T, VE> x[K], d[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[k].x[e] = d[k].x[e] = 0.0f;
+      if (live && on[k]) {
+        x[k].load(reinterpret_cast<const T*>(a.x) + b * a.x_b + c + k * 256 * VE);
+        if constexpr (BACK) d[k].load(reinterpret_cast<const T*>(a.dy) + (long long)b * a.channels + c + k * 256 * VE);
+      }
+    }
+    float* st = a.stats + 2 * ((long long)b * a.groups + g);
+    if constexpr (!BACK) {
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s[0] += x[k].x[e];
+      sums(s, scratch[0]);
+      const float mean = s[0] * inv;
+      s[0] = s[1] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float off = on[k] ? x[k].x[e] - mean : 0.0f;
+          s[0] += off * off;
+        }
+      sums(s, scratch[1]);      // (the next sample's first sums use the other half: its readers are past this barrier)
+      const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[k].x[e] = live ? act((x[k].x[e] - mean) * rstd * w[k][e] + o[k][e], a.activation) : 0.0f;
+        if (on[k]) x[k].store(reinterpret_cast<T*>(a.y) + (long long)b * a.channels + c + k * 256 * VE);
+      }
+      if (tid == 0) {
+        st[0] = mean;
+        st[1] = rstd;
+      }
+    } else {
+      const float mean = live ? st[0] : 0.0f, rstd = live ? st[1] : 0.0f;
+      float t[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float hat = (x[k].x[e] - mean) * rstd;
+          const float dz = live && on[k] ? d[k].x[e] * act_slope(hat * w[k][e] + o[k][e], a.activation) : 0.0f;
+          sw[k][e] += dz * hat;
+          sb[k][e] += dz;
+          x[k].x[e] = hat;
+          d[k].x[e] = dz * w[k][e];
+          t[0] += d[k].x[e];
+          t[1] += d[k].x[e] * hat;
+        }
+      sums(t, scratch[(b / gridDim.x) & 1]);      // (halves in turn: a sample's writers have passed the barrier behind the last readers of theirs)
+      t[0] *= inv;
+      t[1] *= inv;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) d[k].x[e] = live ? rstd * (d[k].x[e] - t[0] - x[k].x[e] * t[1]) : 0.0f;
+        if (on[k]) d[k].store(reinterpret_cast<T*>(a.dx) + (long long)b * a.channels + c + k * 256 * VE);
+      }
+    }
+  }
+  if constexpr (BACK) {
+    if (a.weight != nullptr) {
+      float* record = a.work + (long long)blockIdx.x * 2 * a.channels + c;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (on[k]) {
+            record[k * 256 * VE + e] = sw[k][e];
+            record[a.channels + k * 256 * VE + e] = sb[k][e];
+          }
+    }
+  }
+}
+
 // ---- slab: a sample's slice in registers ------------------------------------------------------------------------------------------------
 template <typename T, int VE, int K>
 __global__ __launch_bounds__(256) void slab_fwd_kernel(const Args a, const int slice) {
   __shared__ float all[256], out[256];
   const int slices = a.channels / slice, b = blockIdx.x / slices, c0 = (blockIdx.x - b * slices) * slice, cg = a.channels / a.groups;
   const int len = length_of(a, b), cpg = cg / VE;
-  const Place p(slice, VE);
+  const Place p(slice, VE, slice);
   const int c = c0 + p.col * VE;
   const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + c;
   T* y = reinterpret_cast<T*>(a.y) + (long long)b * a.n * a.channels + c;
@@ -309,7 +417,7 @@ __global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int s
   __shared__ float all[256], out[256], lds[256 * VE];
   const int slices = a.channels / slice, b = blockIdx.x / slices, c0 = (blockIdx.x - b * slices) * slice, cg = a.channels / a.groups;
   const int len = length_of(a, b), cpg = cg / VE;
-  const Place p(slice, VE);
+  const Place p(slice, VE, slice);
   const int c = c0 + p.col * VE;
   const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + c;
   const long long at = (long long)b * a.n * a.channels + c;
@@ -377,17 +485,20 @@ __global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int s
       }
     }
   }
-  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + (long long)b * 2 * a.channels, a.channels, c0);
+  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + (long long)b * 2 * a.channels, a.channels, c0, slice);
 }
 
 // ---- long: row blocks ---------------------------------------------------------------------------------------------------------------------
-// workspace: pairs[sample][group][block][2], joined[sample][group][2], then the dw / db records.  Workgroup = (sample, block, slice)
+// workspace: pairs[sample][group][block][part][2], joined[sample][group][2], then the dw / db records.  Workgroup = (sample, block, slice)
 struct Block {
-  int b, block, c0, first, last, len;
+  int b, block, part, c0, width, first, last, len;
   __device__ __forceinline__ Block(const Args& a, const Plan& p) {
-    const int slices = p.slices;
+    const int slices = p.slices, cg = a.channels / a.groups;
     int id = blockIdx.x;
-    c0 = id % slices * p.slice;
+    const int s = id % slices;
+    part = s % p.parts;
+    c0 = p.parts == 1 ? s * p.slice : s / p.parts * cg + part * p.slice;
+    width = p.parts == 1 ? p.slice : min(p.slice, cg - part * p.slice);
     id /= slices;
     block = id % p.blocks;
     b = id / p.blocks;
@@ -398,7 +509,7 @@ struct Block {
 };
 
 __device__ __forceinline__ float* pair_at(const Args& a, const Plan& plan, const Block& k, int group) {
-  return a.work + 2 * (((long long)k.b * a.groups + group) * plan.blocks + k.block);
+  return a.work + 2 * ((((long long)k.b * a.groups + group) * plan.blocks + k.block) * plan.parts + k.part);
 }
 
 // rows first, first + step ... below end, four at a time: all loads of a batch are in flight before its first use
@@ -424,8 +535,8 @@ template <typename T, int VE>
 __global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan plan) {
   __shared__ float all[256], out[256];
   const Block k(a, plan);
-  const int cg = a.channels / a.groups, cpg = cg / VE;
-  const Place p(plan.slice, VE);
+  const int cg = a.channels / a.groups, share = plan.parts == 1 ? cg : k.width, cpg = (plan.parts == 1 ? cg : plan.slice) / VE;
+  const Place p(plan.slice, VE, k.width);
   const int c = k.c0 + p.col * VE;
   float s[VE], q[VE], base[VE];
   int count = 0;
@@ -452,7 +563,7 @@ __global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan
       ++count;
     });
   }
-  const float rows = (float)(k.last > k.first ? k.last - k.first : 0), total = rows * (float)cg;
+  const float rows = (float)(k.last > k.first ? k.last - k.first : 0), total = rows * (float)share;
   float sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < VE; ++e) sum += (float)count * base[e] + s[e];
@@ -480,31 +591,35 @@ __global__ __launch_bounds__(256) void long_join_kernel(const Args a, const Plan
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= (long long)a.batch * a.groups) return;
   const int lane = threadIdx.x & 63, len = length_of(a, (int)(i / a.groups)), cg = a.channels / a.groups;
-  const float2* at = reinterpret_cast<const float2*>(a.work) + i * plan.blocks;
-  const float total = (float)(len > 0 ? len : 1);
-  auto rows = [&](int n) { return (float)max(min((n + 1) * plan.rows, len) - n * plan.rows, 0); };
+  const int entries = plan.blocks * plan.parts;
+  const float2* at = reinterpret_cast<const float2*>(a.work) + i * entries;
+  const float total = (float)(len > 0 ? len : 1) * (float)cg;
+  auto count = [&](int n) {      // elements behind entry n
+    const int block = n / plan.parts, part = n - block * plan.parts, width = plan.parts == 1 ? cg : min(plan.slice, cg - part * plan.slice);
+    return (float)max(min((block + 1) * plan.rows, len) - block * plan.rows, 0) * (float)width;
+  };
   float s0 = 0.0f, s1 = 0.0f;
-  for (int n = lane; n < plan.blocks; n += 64) {
+  for (int n = lane; n < entries; n += 64) {
     const float2 x = at[n];
     if constexpr (BACK) {
       s0 += x.x;
       s1 += x.y;
     } else {
-      s0 += x.x * (rows(n) / total);
+      s0 += x.x * (count(n) / total);
     }
   }
   s0 = wave_sum(s0);
   if constexpr (BACK) {
     s1 = wave_sum(s1);
-    if (lane == 0) reinterpret_cast<float2*>(a.work)[(long long)a.batch * a.groups * plan.blocks + i] = make_float2(s0 / (total * cg), s1 / (total * cg));
+    if (lane == 0) reinterpret_cast<float2*>(a.work)[(long long)a.batch * a.groups * entries + i] = make_float2(s0 / total, s1 / total);
   } else {
-    for (int n = lane; n < plan.blocks; n += 64) {
+    for (int n = lane; n < entries; n += 64) {
       const float2 x = at[n];
       const float off = x.x - s0;
-      s1 += x.y + rows(n) * (float)cg * off * off;
+      s1 += x.y + count(n) * off * off;
     }
     s1 = wave_sum(s1);
-    if (lane == 0) reinterpret_cast<float2*>(a.stats)[i] = make_float2(s0, 1.0f / sqrtf(s1 / (total * cg) + a.eps));
+    if (lane == 0) reinterpret_cast<float2*>(a.stats)[i] = make_float2(s0, 1.0f / sqrtf(s1 / total + a.eps));
   }
 }
 
@@ -512,7 +627,7 @@ template <typename T, int VE>
 __global__ __launch_bounds__(256) void long_apply_kernel(const Args a, const Plan plan) {
   const Block k(a, plan);
   const int cg = a.channels / a.groups;
-  const Place p(plan.slice, VE);
+  const Place p(plan.slice, VE, k.width);
   if (!p.on) return;
   const int c = k.c0 + p.col * VE;
   const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
@@ -542,8 +657,8 @@ template <typename T, int VE>
 __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan plan) {
   __shared__ float all[256], out[256], lds[256 * VE];
   const Block k(a, plan);
-  const int cg = a.channels / a.groups, cpg = cg / VE;
-  const Place p(plan.slice, VE);
+  const int cg = a.channels / a.groups, cpg = (plan.parts == 1 ? cg : plan.slice) / VE;
+  const Place p(plan.slice, VE, k.width);
   const int c = k.c0 + p.col * VE;
   float w[VE], o[VE], sw[VE], sb[VE];
 #pragma unroll
@@ -580,23 +695,23 @@ __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan 
   }
   t1 = group_sum(t1, p, cpg, all, out);
   t2 = group_sum(t2, p, cpg, all, out);
-  const long long pairs = 2LL * a.batch * (plan.blocks + 1) * a.groups, index = (long long)k.b * plan.blocks + k.block;
+  const long long pairs = 2LL * a.batch * (plan.blocks * plan.parts + 1) * a.groups, index = (long long)k.b * plan.blocks + k.block;
   if (p.on && p.rl == 0 && p.col % cpg == 0) {
     float* at = pair_at(a, plan, k, c / cg);
     at[0] = t1;
     at[1] = t2;
   }
-  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0);
+  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0, k.width);
 }
 
 template <typename T, int VE>
 __global__ __launch_bounds__(256) void long_dx_kernel(const Args a, const Plan plan) {
   const Block k(a, plan);
   const int cg = a.channels / a.groups;
-  const Place p(plan.slice, VE);
+  const Place p(plan.slice, VE, k.width);
   if (!p.on) return;
   const int c = k.c0 + p.col * VE;
-  const float* joined = a.work + 2LL * a.batch * a.groups * plan.blocks + 2 * ((long long)k.b * a.groups + c / cg);
+  const float* joined = a.work + 2LL * a.batch * a.groups * plan.blocks * plan.parts + 2 * ((long long)k.b * a.groups + c / cg);
   const float t1 = joined[0], t2 = joined[1];
   const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
   const float mean = st[0], rstd = st[1];
@@ -632,79 +747,6 @@ __global__ __launch_bounds__(256) void long_dx_kernel(const Args a, const Plan p
   });
 }
 
-// ---- any: one workgroup per (sample, group), re-reading -----------------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void any_fwd_kernel(const Args a) {
-  __shared__ float scratch[4];
-  const int b = blockIdx.x / a.groups, g = blockIdx.x % a.groups, cg = a.channels / a.groups, len = length_of(a, b);
-  const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + g * cg;
-  T* y = reinterpret_cast<T*>(a.y) + ((long long)b * a.n) * a.channels + g * cg;
-  const float count = (float)(len > 0 ? len : 1) * (float)cg;
-  float s = 0.0f;
-  for (int row = 0; row < len; ++row)
-    for (int c = threadIdx.x; c < cg; c += 256) s += (float)x[row * a.x_n + c];
-  const float mean = block_sum(s, scratch) / count;
-  s = 0.0f;
-  for (int row = 0; row < len; ++row)
-    for (int c = threadIdx.x; c < cg; c += 256) {
-      const float d = (float)x[row * a.x_n + c] - mean;
-      s += d * d;
-    }
-  const float rstd = 1.0f / sqrtf(block_sum(s, scratch) / count + a.eps);
-  if (threadIdx.x == 0) {
-    a.stats[2 * (long long)blockIdx.x] = mean;
-    a.stats[2 * (long long)blockIdx.x + 1] = rstd;
-  }
-  for (int c = threadIdx.x; c < cg; c += 256) {
-    const float w = param<T>(a, a.weight, g * cg + c, 1.0f), o = param<T>(a, a.bias, g * cg + c, 0.0f);
-    for (int row = 0; row < a.n; ++row)
-      y[row * (long long)a.channels + c] = (T)(row < len ? act(((float)x[row * a.x_n + c] - mean) * rstd * w + o, a.activation) : 0.0f);
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void any_bwd_kernel(const Args a) {
-  __shared__ float scratch[4];
-  const int b = blockIdx.x / a.groups, g = blockIdx.x % a.groups, cg = a.channels / a.groups, len = length_of(a, b);
-  const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + g * cg;
-  const long long at = ((long long)b * a.n) * a.channels + g * cg;
-  const T* dy = reinterpret_cast<const T*>(a.dy) + at;
-  T* dx = reinterpret_cast<T*>(a.dx) + at;
-  const float mean = a.stats[2 * (long long)blockIdx.x], rstd = a.stats[2 * (long long)blockIdx.x + 1];
-  float t1 = 0.0f, t2 = 0.0f;
-  for (int c = threadIdx.x; c < cg; c += 256) {
-    const float w = param<T>(a, a.weight, g * cg + c, 1.0f), o = param<T>(a, a.bias, g * cg + c, 0.0f);
-    float sb = 0.0f, sw = 0.0f;
-    for (int row = 0; row < len; ++row) {
-      const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
-      const float dz = (float)dy[row * (long long)a.channels + c] * act_slope(hat * w + o, a.activation);
-      sb += dz;
-      sw += dz * hat;
-    }
-    t1 += sb * w;
-    t2 += sw * w;
-    if (a.weight != nullptr) {
-      a.work[(2LL * b) * a.channels + g * cg + c] = sw;
-      a.work[(2LL * b + 1) * a.channels + g * cg + c] = sb;
-    }
-  }
-  const float count = (float)(len > 0 ? len : 1) * (float)cg;
-  t1 = block_sum(t1, scratch) / count;
-  t2 = block_sum(t2, scratch) / count;
-  for (int c = threadIdx.x; c < cg; c += 256) {
-    const float w = param<T>(a, a.weight, g * cg + c, 1.0f), o = param<T>(a, a.bias, g * cg + c, 0.0f);
-    for (int row = 0; row < a.n; ++row) {
-      float v = 0.0f;
-      if (row < len) {
-        const float hat = ((float)x[row * a.x_n + c] - mean) * rstd;
-        const float dz = (float)dy[row * (long long)a.channels + c] * act_slope(hat * w + o, a.activation);
-        v = rstd * (dz * w - t1 - hat * t2);
-      }
-      dx[row * (long long)a.channels + c] = (T)v;
-    }
-  }
-}
-
 // dweight, dbias = the sums of `records` records [2][channels]: 16 columns x 64 record lanes a workgroup, then the lanes in order
 template <typename T>
 __global__ __launch_bounds__(1024) void param_grad_kernel(const Args a, const float* part, int records) {
@@ -732,7 +774,7 @@ __global__ __launch_bounds__(1024) void param_grad_kernel(const Args a, const fl
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 bool sizes_ok(const Args& a) {
-  return a.batch >= 1 && a.n >= 1 && a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0 && a.channels <= (1 << 24) &&
+  return a.batch >= 1 && a.n >= 1 && a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0 && a.channels <= (1 << 24) && a.n <= (1 << 30) &&
          (long long)a.batch * a.groups <= 0x3fffffffLL && a.type >= TYPE_F32 && a.type <= TYPE_F16;
 }
 
@@ -756,15 +798,20 @@ Plan plan(const Args& a) {
     p.records = p.blocks;
     return p;
   }
-  if (cpg > 256) {
-    p.form = ANY;
-    p.records = a.batch;
+  if (a.n == 1 && cpg > 64 && cpg <= 1024 && a.groups <= 32768) {      // (groups: the grid's second dimension)
+    p.form = WIDE;
+    p.per_thread = cpg <= 256 ? 1 : cpg <= 512 ? 2 : 4;
+    const int most = 1024 / a.groups > 1 ? 1024 / a.groups : 1;      // 4 workgroups a CU
+    p.blocks = a.batch < most ? a.batch : most;
+    p.slices = a.groups;
+    p.records = p.blocks;
     return p;
   }
   // slices of whole groups: 64 bytes of a row at least, more while that still leaves 1024 workgroups, 256 chunks at most
   auto fits = [&](int gs) { return (long long)gs * cpg <= 256; };
   int gs = 1;
-  for (int k = 1; k <= a.groups; ++k) {
+  p.parts = (cpg + 255) / 256;
+  for (int k = 1; k <= a.groups && p.parts == 1; ++k) {
     if (!fits(k)) break;
     if (a.groups % k != 0) continue;
     const bool narrow = (long long)gs * cg * size < 64, many = (long long)a.batch * (a.groups / k) >= 1024;
@@ -774,10 +821,10 @@ Plan plan(const Args& a) {
       gs = k;
     }
   }
-  p.slice = gs * cg;
-  p.slices = a.groups / gs;
-  const int lanes = 256 / (gs * cpg), need = (a.n + lanes - 1) / lanes;
-  if (need <= 16) {
+  const int lanes = p.parts == 1 ? 256 / (gs * cpg) : 0, need = p.parts == 1 ? (a.n + lanes - 1) / lanes : 0;
+  if (p.parts == 1 && need <= 16) {
+    p.slice = gs * cg;
+    p.slices = a.groups / gs;
     p.form = SLAB;
     p.per_thread = need <= 1 ? 1 : need <= 4 ? 4 : 16;
     p.records = a.batch;
@@ -787,9 +834,9 @@ Plan plan(const Args& a) {
   // rows as wide as 256 chunks allow; 1024 workgroups, 16 rows a thread at least
   for (int k = 1; k <= a.groups && fits(k); ++k)
     if (a.groups % k == 0) gs = k;
-  p.slice = gs * cg;
-  p.slices = a.groups / gs;
-  const int per = 256 / (gs * cpg) * 16;
+  p.slice = p.parts == 1 ? gs * cg : (cpg + p.parts - 1) / p.parts * p.ve;
+  p.slices = a.groups / gs * p.parts;
+  const int per = 256 / (p.slice / p.ve) * 16;
   const long long want = 1024 / ((long long)a.batch * p.slices) > 1 ? 1024 / ((long long)a.batch * p.slices) : 1, most = (a.n + per - 1) / per;
   const int blocks = (int)(want < most ? want : most);
   p.rows = (a.n + blocks - 1) / blocks;
@@ -799,7 +846,7 @@ Plan plan(const Args& a) {
 }
 
 long long work_floats(const Args& a, const Plan& p, bool backward) {
-  const long long pairs = p.form == LONG ? 2LL * a.batch * (p.blocks + 1) * a.groups : 0;
+  const long long pairs = p.form == LONG ? 2LL * a.batch * (p.blocks * p.parts + 1) * a.groups : 0;
   return pairs + (backward && a.weight != nullptr ? 2LL * p.records * a.channels : 0);
 }
 
@@ -815,6 +862,19 @@ void launch_slab(const Args& a, const Plan& p, bool backward, hipStream_t st) {
     else if (p.per_thread == 4) slab_fwd_kernel<T, VE, 4><<<grid, 256, 0, st>>>(a, p.slice);
     else slab_fwd_kernel<T, VE, 16><<<grid, 256, 0, st>>>(a, p.slice);
   }
+}
+
+template <typename T, int VE, int K>
+void launch_wide(const Args& a, const Plan& p, bool backward, hipStream_t st) {
+  const dim3 grid(p.blocks, p.slices);
+  if (backward) wide_kernel<T, VE, K, true><<<grid, 256, 0, st>>>(a);
+  else wide_kernel<T, VE, K, false><<<grid, 256, 0, st>>>(a);
+}
+template <typename T, int VE>
+void launch_wide(const Args& a, const Plan& p, bool backward, hipStream_t st) {
+  if (p.per_thread == 1) launch_wide<T, VE, 1>(a, p, backward, st);
+  else if (p.per_thread == 2) launch_wide<T, VE, 2>(a, p, backward, st);
+  else launch_wide<T, VE, 4>(a, p, backward, st);
 }
 
 template <typename T, int VE>
@@ -839,16 +899,15 @@ void launch(const Args& a, const Plan& p, bool backward, hipStream_t st) {
     const dim3 grid(p.blocks, p.slices);
     if (backward) rows_kernel<T, true><<<grid, 256, 0, st>>>(a, cpg, p.slice);
     else rows_kernel<T, false><<<grid, 256, 0, st>>>(a, cpg, p.slice);
+  } else if (p.form == WIDE) {
+    if (p.ve == 1) launch_wide<T, 1>(a, p, backward, st);
+    else launch_wide<T, N>(a, p, backward, st);
   } else if (p.form == SLAB) {
     if (p.ve == 1) launch_slab<T, 1>(a, p, backward, st);
     else launch_slab<T, N>(a, p, backward, st);
-  } else if (p.form == LONG) {
+  } else {
     if (p.ve == 1) launch_long<T, 1>(a, p, backward, st);
     else launch_long<T, N>(a, p, backward, st);
-  } else {
-    const unsigned grid = (unsigned)((long long)a.batch * a.groups);
-    if (backward) any_bwd_kernel<T><<<grid, 256, 0, st>>>(a);
-    else any_fwd_kernel<T><<<grid, 256, 0, st>>>(a);
   }
   if (backward && a.weight != nullptr) {
     const float* records = a.work + work_floats(a, p, false);
@@ -868,7 +927,8 @@ int run(const Args* args, bool backward, const char* entry, void* stream) {
   const uintptr_t own = backward ? reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx) : reinterpret_cast<uintptr_t>(a.y);
   if (p.ve > 1 && own % 16 != 0) return fail(entry, -22);
   if (a.work == nullptr && work_floats(a, p, backward) > 0) return fail(entry, -22);
-  if ((long long)a.batch * (p.slices > 0 ? p.slices : 1) * (p.blocks > 0 ? p.blocks : 1) > 0x7fffffffLL) return fail(entry, -22);
+  // workgroups of one launch (rows and wide: at most a few thousand)
+  if ((p.form == SLAB || p.form == LONG) && (long long)a.batch * p.slices * (p.form == LONG ? p.blocks : 1) > 0x7fffffffLL) return fail(entry, -22);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.type == TYPE_F32) launch<float>(a, p, backward, st);
   else if (a.type == TYPE_BF16) launch<__bf16>(a, p, backward, st);

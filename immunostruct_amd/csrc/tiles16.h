@@ -150,30 +150,30 @@ __device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NT], const char* at,
 
 // ROWS rows of N elements, global -> registers -> LDS by NTHREADS threads.  Thread t handles chunk t mod CH of the rows row_of(k); their byte
 // offsets from a base that is uniform over the workgroup are 32-bit (one 64-bit scalar base per tile and one 32-bit lane offset per load).
-// Rows of fewer than N elements: EXACT fills the rest with zeros, the other form repeats the row's last chunk there (no test per load):
-// the other operand of every product over that dimension is zero there, or the columns are never stored.
-template <typename T, int N, int ROWS, int NTHREADS, bool VEC, bool EXACT = false>
+// Rows of fewer than N elements: the loads repeat the row's last chunk (no test per load), the stores put zeros in its place.
+template <typename T, int N, int ROWS, int NTHREADS, bool VEC>
 struct Stage {
   static constexpr int ROWS_ = ROWS, CH = Tile<T, N>::CHUNKS, TOTAL = ROWS * CH, PER = (TOTAL + NTHREADS - 1) / NTHREADS;
+  static_assert(NTHREADS % CH == 0, "a thread's chunks lie whole rows apart");
   u32x4_t v[PER];
   static __device__ __forceinline__ int row_of(int tid, int k) { return (tid + k * NTHREADS) / CH; }
   static __device__ __forceinline__ bool has(int tid, int k) { return TOTAL % NTHREADS == 0 || tid + k * NTHREADS < TOTAL; }
   __device__ __forceinline__ void load(int tid, const char* base, const unsigned (&offset)[PER], int len) {
-    int c = tid % CH;
-    if constexpr (VEC && !EXACT) {
-      const int most = len / Vec<T>::N - 1;
-      c = c < most ? c : most;
-    }
+    const int c = tid % CH, most = len / Vec<T>::N - 1;
 #pragma unroll
     for (int k = 0; k < PER; ++k)
       if (has(tid, k)) {
-        if constexpr (VEC && !EXACT) v[k] = *reinterpret_cast<const u32x4_t*>(base + (offset[k] + (unsigned)c * 16u));
-        else v[k] = load_chunk<T, VEC>(base + offset[k], c, len);
+        if constexpr (VEC) v[k] = *reinterpret_cast<const u32x4_t*>(base + (offset[k] + (unsigned)(c < most ? c : most) * 16u));
+        else v[k] = load_chunk<T, false>(base + offset[k], c, len);
       }
   }
-  __device__ __forceinline__ void store(int tid, char* tile) const {
-    static_assert(NTHREADS % CH == 0, "a thread's chunks lie whole rows apart");
+  __device__ __forceinline__ void store(int tid, char* tile, int len) {
     char* at = tile + Tile<T, N>::offset(tid / CH, tid % CH);
+    if (VEC && len < N) {      // (uniform)
+      const bool there = (tid % CH) * Vec<T>::N < len;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[k] = there ? v[k] : u32x4_t{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
     for (int k = 0; k < PER; ++k)
       if (has(tid, k)) *reinterpret_cast<u32x4_t*>(at + k * (NTHREADS / CH) * Tile<T, N>::STRIDE) = v[k];

@@ -45,6 +45,11 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor like(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); }
 Tensor floats(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.options().dtype(at::kFloat)); }
+// contiguous and 16-byte aligned: an incoming gradient may be any view
+Tensor aligned(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the sequence operators are differentiable once: no create_graph=True"); }
@@ -110,10 +115,10 @@ std::pair<Tensor, OptTensor> rotary(const Tensor& q, const OptTensor& k_, const 
 }
 
 // ---- differential attention --------------------------------------------------------------------------------------------------------------
-// (B, n, heads, width) as the kernels read it: a copy where the innermost dimension is not laid out element by element or the rows of a tile lie
-// too far apart for their 32-bit offsets
-Tensor sequence_rows(const Tensor& t) {
-  const bool fits = (t.stride(3) == 1 || t.size(3) == 1) && t.stride(1) < (1 << 23) && t.stride(2) * t.size(2) < (1 << 27);
+// (B, n, heads, width) as the kernels read it: a copy where the innermost dimension is not laid out element by element, or the rows (query heads,
+// the two maps' keys) of one tile lie too far apart for their 32-bit offsets
+Tensor sequence_rows(const Tensor& t, int64_t heads) {
+  const bool fits = (t.stride(3) == 1 || t.size(3) == 1) && t.stride(1) < (1 << 23) && t.stride(2) * heads < (1 << 27);
   return fits ? t : t.contiguous();
 }
 
@@ -159,7 +164,7 @@ Attended diff_forward(const Tensor& q, const Tensor& k, const Tensor& v, const T
 struct DiffAttention : torch::autograd::Function<DiffAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& lam_, const OptTensor& lengths_, int64_t causal, double scale) {
     const Tensor lengths = value(lengths_);
-    const Tensor q = sequence_rows(q_), k = sequence_rows(k_), v = sequence_rows(v_), lam = lam_.contiguous();
+    const Tensor q = sequence_rows(q_, q_.size(2)), k = sequence_rows(k_, 1), v = sequence_rows(v_, 0), lam = lam_.contiguous();
     Attended r = diff_forward(q, k, v, lam, lengths, causal, scale, true);
     ctx->save_for_backward({q, k, v, lam, lengths, r.out, r.o2, r.lse});
     ctx->saved_data["causal"] = causal;
@@ -173,7 +178,7 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
     const c10::DeviceGuard guard(q.device());
     Tensor dq = like(q), dk = like(k), dv = like(v), dlam = like(lam);
     if (s[5].numel() == 0 || v.size(1) == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), Tensor(), Tensor(), Tensor()};
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = aligned(grads[0]);
     IsDiffAttention a = diff_args(q, k, v, lam, s[4], ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble());
     const int rows = (int)lse.size(3);
     a.row_splits = entry.row_splits(a.batch, a.kv_heads, rows, a.nk, a.causal);
@@ -189,7 +194,7 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
 
 Tensor differential_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptTensor& lengths, int64_t causal, double scale) {
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v) || wanted(lam))) return DiffAttention::apply(q, k, v, lam, lengths, causal, scale);
-  return diff_forward(sequence_rows(q), sequence_rows(k), sequence_rows(v), lam.contiguous(), value(lengths), causal, scale, false).out;
+  return diff_forward(sequence_rows(q, q.size(2)), sequence_rows(k, 1), sequence_rows(v, 0), lam.contiguous(), value(lengths), causal, scale, false).out;
 }
 
 // ---- group norm ----------------------------------------------------------------------------------------------------------------------------
@@ -238,8 +243,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
       if (dw.defined()) dw.zero_(), db.zero_();
       return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
     }
-    Tensor g = grads[0].contiguous();
-    if (reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 != 0) g = g.clone();      // (an incoming gradient may be any view)
+    const Tensor g = aligned(grads[0]);
     IsGroupNorm a = norm_args(x, weight, bias, s[3], ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["activation"].toInt());
     const int64_t n = entry.norm_floats(&a, 1);
     if (n > 0) work = floats(x, {n});

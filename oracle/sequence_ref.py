@@ -112,7 +112,9 @@ def group_norm(x, groups, weight, bias, eps, activation, lengths, dy=None):
         return {"y": out["y"]}
     more = (b / 4 + 8) * E32      # the records of the samples, added in a few chains
     for k, (v, e) in grads.items():
-        grads[k] = (v, e * (1 + more) + more * v.abs() * 4 + wu * v.abs() + E32 * e)
+        # (the rounding to the weight's type has a relative part and, below the smallest normal number, a fixed one: an fp16 gradient of 2.4e-5 lies
+        # under 2^-14, where the steps are 2^-24 apart: off by up to 2^-25 = 3.0e-8, where 2^-11 of it is 1.2e-8)
+        grads[k] = (v, e * (1 + more) + more * v.abs() * 4 + wu * v.abs() + E32 * e + (tiny_step(weight.dtype) if weight is not None else 0.0))
     return {**out, **grads}
 
 

@@ -169,6 +169,56 @@ def test_attention_strides_scale_and_types(cuda_device):
     assert not empty.any() and empty.requires_grad
 
 
+@each_type
+def test_attention_lam_of_any_sign(cuda_device, dtype):
+    """negative, zero and mixed weights of the second map, in groups that do and do not divide a tile of 32 rows"""
+    for heads, lam in ((2, (-0.7, -0.2)), (2, (0.0, 0.4)), (3, (0.5, -1.5, 0.0)), (5, (0.1, 2.0, -0.3, 1.0, 0.6))):
+        q, k, v, _ = _attention_inputs(dtype, 2, 50, 77, heads, 1, 32, 64)
+        leaves = [t.requires_grad_(True) for t in (q, k, v, torch.tensor(lam, dtype=dtype, device="cuda"))]
+        do = _randn(2, 50, heads, 64, dtype=dtype, seed=17)
+        lens = torch.tensor([77, 60], dtype=torch.int32, device="cuda")
+        want = SR.differential_attention(*leaves, lens.tolist(), "end", 32 ** -0.5, do)
+        out = HF.differential_attention(*leaves, lens, "end")
+        _within(out, want["o"], f"o {lam}")
+        for g, name in zip(torch.autograd.grad(out, leaves, do), ("dq", "dk", "dv", "dlam")):
+            _within(g, want[name], f"{name} {lam}")
+
+
+def test_attention_infinite_scores_of_narrow_heads(cuda_device):
+    """a key whose last element is -inf has weight 0 for the queries that are positive there (heads narrower than the kernels' width: the
+    elements that are not there must not meet the infinity)"""
+    for dtype, d in ((torch.float32, 8), (torch.bfloat16, 40), (torch.float16, 8)):
+        q, k, v, lam = _attention_inputs(dtype, 1, 40, 70, 1, 1, d, 2 * d)
+        q[..., -1] = q[..., -1].abs() + 0.5
+        k[:, 13, :, -1] = float("-inf")
+        keep = [i for i in range(70) if i != 13]
+        want = SR.differential_attention(q, k[:, keep], v[:, keep], lam, None, None, d ** -0.5)
+        _within(HF.differential_attention(q, k, v, lam), want["o"], "o")
+
+
+def test_attention_unaligned_gradient_and_second_derivative(cuda_device):
+    q, k, v, lam = (t.requires_grad_(True) for t in _attention_inputs(torch.bfloat16, 1, 33, 33, 1, 1, 16, 32))
+    out = HF.differential_attention(q, k, v, lam)
+    g = _randn(1 * 33 * 32 + 1, dtype=torch.bfloat16, seed=18)[1:].view(1, 33, 1, 32)
+    got = torch.autograd.grad(out, (q, k, v, lam), g, retain_graph=True)
+    want = torch.autograd.grad(out, (q, k, v, lam), g.clone(), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out, q, g, create_graph=True)
+    x = _randn(3, 8, dtype=torch.float32, seed=19).requires_grad_(True)
+    y = HF.group_norm(x, 2)
+    gy = _randn(25, dtype=torch.float32, seed=20)[1:].view(3, 8)
+    assert torch.equal(*(torch.autograd.grad(y, x, t, retain_graph=True)[0] for t in (gy, gy.clone())))
+
+
+def test_errors_are_the_packages(cuda_device):
+    """what the library refuses behind the package's own checks arrives as HipExtensionError with the library's text"""
+    from immunostruct_amd import _lib
+    q, k, v, lam = _attention_inputs(torch.float32, 1, 3, 3, 1, 1, 8, 16)
+    with pytest.raises(_lib.HipExtensionError, match="is_diff_attention_fwd: invalid argument"):
+        HF.differential_attention(q, k, v, lam, scale=3e38)
+
+
 def test_attention_large_scores_and_offsets(cuda_device):
     """scores far apart (the running maximum moves at the end), all equal, and of magnitude 1e4"""
     for dtype in TYPES:
@@ -215,6 +265,32 @@ def test_group_norm(cuda_device, dtype, activation, b, n, c, groups, lengths):
         _within(g, want[name], name)
     again = torch.autograd.grad(HF.group_norm(x, groups, w, o, activation=activation, lengths=lens), (x, w, o), dy)
     assert all(torch.equal(p, r) for p, r in zip(grads, again)), "not reproducible"
+
+
+@each_type
+@pytest.mark.parametrize("b,n,c,groups", [(3, 5, 4096, 1), (2, 1, 8200, 2), (1, 40, 2056, 1), (2, 9, 1031, 1), (4, 3, 514, 1), (2, 33, 3 * 2072, 3), (2100, 1, 1040, 1), (7, 1, 4 * 519, 4), (5, 1, 8192, 2),
+                                        (3, 1, 516, 1)])
+def test_group_norm_wide_groups(cuda_device, dtype, b, n, c, groups):
+    """groups wider than a workgroup (a last part that is narrower; single elements and chunks), a sample that is short or empty"""
+    x, dy = (_randn(b, n, c, dtype=dtype, seed=s, mean=0.2).requires_grad_(s == 21) for s in (21, 22))
+    w, o = (_randn(c, dtype=dtype, seed=s).requires_grad_(True) for s in (23, 24))
+    lengths = [max(n - 2 * i, 0) for i in range(b)] if n > 1 else [i % 3 != 1 for i in range(b)]
+    want = SR.group_norm(x, groups, w, o, 1e-5, "gelu", lengths, dy)
+    y = HF.group_norm(x, groups, w, o, activation="gelu", lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    _within(y, want["y"], "y")
+    for g, name in zip(torch.autograd.grad(y, (x, w, o), dy), ("dx", "dweight", "dbias")):
+        _within(g, want[name], name)
+
+
+def test_group_norm_many_rows(cuda_device):
+    """more rows than 2^20: every row as in a small call"""
+    x = _randn(1 << 12, 64, dtype=torch.bfloat16, seed=25)
+    w, o = _randn(64, dtype=torch.float32, seed=26), _randn(64, dtype=torch.float32, seed=27)
+    y = HF.group_norm(x, 4, w, o, activation="silu")
+    many = HF.group_norm(x.repeat(300, 1), 4, w, o, activation="silu")
+    assert torch.equal(many, y.repeat(300, 1))
+    wide = HF.group_norm(x.view(64, 4096).repeat(33000, 1)[:, :1040], 1)
+    assert torch.equal(wide, HF.group_norm(x.view(64, 4096)[:, :1040], 1).repeat(33000, 1))
 
 
 def test_group_norm_forms(cuda_device):
