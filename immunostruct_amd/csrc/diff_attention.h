@@ -3,8 +3,9 @@
 //   rows      the queries of one (sample, key head) and its G = heads / kv_heads query heads are packed into R = nq G rows, row r = query
 //             r / G, head r % G of the group: a key tile is read once for all heads that share it, and the gradients of shared keys
 //             are sums inside one workgroup (no atomics anywhere; every result has one fixed summation order).
-//   visible   key j < end(i): end = len (no mask), min(len, i + 1) ("start") or len - nq + 1 + i ("end").  Keys at or behind len are never
-//             read (their rows are clamped to the last valid one and their scores replaced), so anything may stand there.
+//   visible   key j < end(i): end = len (no mask), min(len, i + 1) ("start") or len - nq + 1 + i ("end").  Keys at or behind len, or that no row
+//             of the workgroup sees, are not multiplied (their rows are clamped to the last seen one, their scores replaced, and dK / dV replace the
+//             products), so anything may stand there.  A value that a mask hides from one row and not from its neighbours has to be a number.
 //             A row that sees nothing gives 0, lse = +inf, and no gradient.
 //   waves     a wave works on 32 rows (or 32 keys) of ONE map; two neighbouring waves hold the two maps of the same rows and meet once at the end,
 //             lane to lane through LDS.  That halves a wave's registers (one accumulator set, one resident operand), so that two to four
@@ -181,8 +182,8 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
   const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + hk * a.v_h) * SZ;
   auto fetch = [&](int j0) {
     unsigned ko[StageK::PER], vo[StageV::PER];
-    key_offsets<StageK, 2>(ko, tid, (unsigned)a.k_n * SZ, (unsigned)a.k_h * SZ, len - 1 - j0);
-    key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, len - 1 - j0);
+    key_offsets<StageK, 2>(ko, tid, (unsigned)a.k_n * SZ, (unsigned)a.k_h * SZ, wg_end - 1 - j0);
+    key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, wg_end - 1 - j0);
     sk.load(tid, kp + j0 * a.k_n * SZ, ko, a.d);
     sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };
@@ -667,8 +668,8 @@ __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_wa
   const char* vp = reinterpret_cast<const char*>(a.v) + (b * a.v_b + hk * a.v_h) * SZ;
   auto fetch = [&](int j0) {
     unsigned ko[StageK::PER], vo[StageV::PER];
-    key_offsets<StageK, 2>(ko, tid, (unsigned)a.k_n * SZ, (unsigned)a.k_h * SZ, len - 1 - j0);
-    key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, len - 1 - j0);
+    key_offsets<StageK, 2>(ko, tid, (unsigned)a.k_n * SZ, (unsigned)a.k_h * SZ, wg_end - 1 - j0);
+    key_offsets<StageV, 1>(vo, tid, (unsigned)a.v_n * SZ, 0, wg_end - 1 - j0);
     sk.load(tid, kp + j0 * a.k_n * SZ, ko, a.d);
     sv.load(tid, vp + j0 * a.v_n * SZ, vo, a.dv);
   };

@@ -1813,6 +1813,7 @@ def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
     ``lengths`` (B,) int32: keys at or behind a sample's length do not exist (whatever their memory holds); all nk without it.
     ``causal``: None; "start": query i is position i and sees keys <= i; "end": the queries are the sample's last nq positions, i.e. new
     tokens over a cache, and see keys <= i + length - nq.  ``scale``: a positive number, d ** -0.5 by default.
+    Keys that no query sees may hold anything; a key that the order hides from some queries only has to hold numbers (its weight there is 0).
     A query that sees no key gives zeros and passes no gradient.  Returns (B, nq, heads, dv).  Deterministic; scores, softmax statistics
     and sums are 32-bit, softmax weights and score gradients are rounded once to the inputs' type for the matrix products."""
     _sequence_type("differential_attention", q, k, v)

@@ -137,6 +137,23 @@ def test_attention_garbage_behind_the_lengths(cuda_device):
         assert not clean[2][1, 41:].any() and not clean[3][1, 41:].any() and not clean[2][2].any() and not clean[0][2].any()
 
 
+@each_type
+@pytest.mark.parametrize("nq,nk", [(5, 64), (40, 200), (130, 131)])
+def test_attention_garbage_that_no_query_sees(cuda_device, dtype, nq, nk):
+    """queries from the start over a buffer that is longer than they are: what stands behind the last query's position does not matter"""
+    q, k, v, lam = _attention_inputs(dtype, 2, nq, nk, 2, 1, 32, 64)
+    k[:, nq:], v[:, nq:] = float("nan"), float("inf")
+    do = _randn(2, nq, 2, 64, dtype=dtype, seed=16)
+    want = SR.differential_attention(q, k[:, :nq], v[:, :nq], lam, None, "start", 32 ** -0.5, do)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    out = HF.differential_attention(*leaves, causal="start")
+    _within(out, want["o"], "o")
+    grads = torch.autograd.grad(out, leaves, do)
+    assert not grads[1][:, nq:].any() and not grads[2][:, nq:].any()
+    for g, name in zip(grads, ("dq", "dk", "dv", "dlam")):
+        _within(g[:, :nq] if name in ("dk", "dv") else g, want[name], name)
+
+
 def test_attention_strides_scale_and_types(cuda_device):
     dtype = torch.bfloat16
     q, k, v, lam = _attention_inputs(dtype, 2, 70, 70, 4, 2, 32, 64)
