@@ -18,7 +18,10 @@
 //   backward  dP = dO V^T; D_m = dO . O_m; dS_1 = P1 (dP - D_1), dS_2 = -lam P2 (dP - D_2);
 //             dQ_m = scale dS_m K_m, dK_m = scale dS_m^T Q_m, dV = (P1 - lam P2)^T dO, dlam = -sum D_2.  Scores are recomputed from lse.
 //             dK / dV: a wave owns 32 keys and walks the rows; dQ: a wave owns 32 rows and walks the keys.
-// Scores, sums, lse, D and all accumulators are 32-bit; P and dS are rounded once to the inputs' type for the matrix instructions.
+// Scores, sums, lse, D and all accumulators are 32-bit.  P and dS are rounded once to the inputs' type, which the matrix instructions ask of both
+// operands: half a step per term, of random sign, about as much as the output's own rounding (0.0025 of the norm in bf16 instead of
+// 0.0017).  The softmax sums are taken before it.  Multiplying what the rounding left out as well restores 0.0017 for 5 % of a single
+// token's time and more of a long sequence's.
 #pragma once
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
@@ -141,6 +144,10 @@ __device__ __forceinline__ void hand_over(const f32x16 (&acc)[NT], char* lds, in
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
 // grid: (row tiles x splits x kv_heads x batch), GROUPS x 2 waves of 32 rows and one map.  splits > 1: every workgroup takes one range of the
 // keys and leaves unnormalised sums with their maxima in the workspace; join_kernel puts them together.
+// Bound by matrix instructions and the exponentials between them: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 283 us = 0.73 PFLOP/s executed
+// (the product with V once per map; a large library product reaches 1.18); (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 88 us; (128, 190, 1, 32 / 64, fp32)
+// 28 us, where fp32 matrix instructions share the vector pipe.  Single tokens are bound by the cache: (16, 1 x 16384 ragged, 16 / 4, 64 / 128, bf16)
+// 75 us = 4.8 TB/s.
 template <typename T, int D, int GROUPS, bool VEC>
 __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2))) void fwd_kernel(const Args a) {
   constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 128 * GROUPS, SZ = sizeof(T);
@@ -371,7 +378,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
-// D_2 = dO . O_2 and D_1 = dO . O + lam D_2 of every row (16 lanes per row)
+// D_2 = dO . O_2 and D_1 = dO . O + lam D_2 of every row (16 lanes per row); bound by bytes: 17.7 us for 3 x 33.5 MB (5.7 TB/s, partly cached)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   constexpr int N = Vec<T>::N;
@@ -404,7 +411,8 @@ __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   }
 }
 
-// dlam_h = - sum over samples and queries of sum_j P_2 dP (dq_kernel's unrounded sums; one workgroup per head, fixed order)
+// dlam_h = - sum over samples and queries of sum_j P_2 dP (dq_kernel's unrounded sums; one workgroup per head, fixed order).
+// One chain of loads and a tree: 5 - 7 us, latency.
 template <typename T>
 __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
   __shared__ float part[16];
@@ -437,6 +445,8 @@ __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
 // the last by few, and one workgroup per key tile would leave half the chip idle half the time.
 // Both waves run the same code on (lse, D): map 1's weight is taken as +|lam| P_2 with |lam| folded into lse, and its results are negated when they
 // leave the wave.  Only where a lam of the group is negative do its rows' signs have to be put back (flip).
+// Bound by matrix instructions: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 535 us = 0.77 PFLOP/s executed (582 with lam applied to each weight);
+// (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 145 us, 120 workgroups; (128, 190, 1, 32 / 64, fp32) 49 us.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) <= 128 ? 2 : 1))) void dkv_kernel(const Args a) {
   constexpr int GROUPS = key_groups<T, D>(), NTH = 128 * GROUPS, KEYS = 32 * GROUPS;
@@ -595,7 +605,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
   });
 }
 
-// dK, dV = the row splits' sums, in order; a thread per four elements (VEC) or one
+// dK, dV = the row splits' sums, in order; a thread per four elements (VEC) or one; bytes: 13.7 us for 50 MB in, 8 out
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void key_join_kernel(const Args a) {
   constexpr int N = VEC ? 4 : 1;
@@ -617,7 +627,9 @@ __global__ __launch_bounds__(256) void key_join_kernel(const Args a) {
   else *out = (T)x[0];
 }
 
-// dQ of 32 rows per wave: grid (row tiles x kv_heads x batch), GROUPS x 2 waves; dO of the workgroup's rows stays in LDS (registers)
+// dQ of 32 rows per wave: grid (row tiles x kv_heads x batch), GROUPS x 2 waves; dO of the workgroup's rows stays in LDS (the registers hold
+// Q, the sums and two tiles of scores).  Bound by matrix instructions: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 385 us = 0.71 PFLOP/s executed;
+// (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 87 us; (128, 190, 1, 32 / 64, fp32) 33 us.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(2))) void dq_kernel(const Args a) {
   constexpr int GROUPS = dq_groups<T, D>(), NTH = 128 * GROUPS, ROWS = 32 * GROUPS;

