@@ -19,9 +19,9 @@
 //             dQ_m = scale dS_m K_m, dK_m = scale dS_m^T Q_m, dV = (P1 - lam P2)^T dO, dlam = -sum D_2.  Scores are recomputed from lse.
 //             dK / dV: a wave owns 32 keys and walks the rows; dQ: a wave owns 32 rows and walks the keys.
 // Scores, sums, lse, D and all accumulators are 32-bit.  P and dS are rounded once to the inputs' type, which the matrix instructions ask of both
-// operands: half a step per term, of random sign, about as much as the output's own rounding (0.0025 of the norm in bf16 instead of
-// 0.0017).  The softmax sums are taken before it.  Multiplying what the rounding left out as well restores 0.0017 for 5 % of a single
-// token's time and more of a long sequence's.
+// operands: half a step per term, of random sign, about as much as the output's own rounding (0.0025 of the norm in bf16 where the output's
+// alone is 0.0017).  The softmax sums are taken before it.  Up to 32 rows (single tokens, bound by the cache's bytes) the forward multiplies what
+// the rounding left out as well: 0.0017, 74.6 -> 76 - 78 us at 16 tokens; long sequences would pay 285 -> 417 us at (2, 4096, 16 / 4 heads, 64 / 128).
 #pragma once
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
@@ -147,7 +147,7 @@ __device__ __forceinline__ void hand_over(const f32x16 (&acc)[NT], char* lds, in
 // Bound by matrix instructions and the exponentials between them: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 283 us = 0.73 PFLOP/s executed
 // (the product with V once per map; a large library product reaches 1.18); (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 88 us; (128, 190, 1, 32 / 64, fp32)
 // 28 us, where fp32 matrix instructions share the vector pipe.  Single tokens are bound by the cache: (16, 1 x 16384 ragged, 16 / 4, 64 / 128, bf16)
-// 75 us = 4.8 TB/s.
+// 77 us = 4.7 TB/s.
 template <typename T, int D, int GROUPS, bool VEC>
 __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2))) void fwd_kernel(const Args a) {
   constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 128 * GROUPS, SZ = sizeof(T);
@@ -235,6 +235,11 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
         }
         sum += add;
         mm_transposed<T, DV, NT>(o, buf + v_at, p);
+        if constexpr (GROUPS == 1 && SZ == 2) {      // a handful of rows: what the rounding left out is multiplied as well
+#pragma unroll
+          for (int t = 0; t < 16; ++t) p[t] -= (float)(T)p[t];
+          mm_transposed<T, DV, NT>(o, buf + v_at, p);
+        }
       }
       if (more) {
         place(lds + (CUR ^ 1) * BUF);
