@@ -201,6 +201,24 @@ def test_attention_lam_of_any_sign(cuda_device, dtype):
             _within(g, want[name], f"{name} {lam}")
 
 
+@each_type
+@pytest.mark.parametrize("nq,nk,heads,kv,lengths,causal", [
+    (1, 700, 33, 1, [700, 31], "end"), (5, 300, 7, 1, [300, 3], "end"), (1, 2100, 4, 2, [5000, -3], "end"), (3, 40, 40, 1, [-1, 41], None),
+    (33, 129, 64, 2, [129, 64], "end"), (2, 5000, 1, 1, [4999, 1], None)])
+def test_attention_group_sizes_and_lengths_out_of_range(cuda_device, dtype, nq, nk, heads, kv, lengths, causal):
+    """groups that do not divide a tile or are wider than one, lengths below zero and above nk (taken as 0 and nk), split keys and rows"""
+    leaves = [t.requires_grad_(True) for t in _attention_inputs(dtype, 2, nq, nk, heads, kv, 16, 32)]
+    do = _randn(2, nq, heads, 32, dtype=dtype, seed=19)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = SR.differential_attention(*leaves, [max(0, min(nk, n)) for n in lengths], causal, 0.25, do)
+    with torch.no_grad():
+        _within(HF.differential_attention(*leaves, lens, causal), want["o"], "o (no gradient)")
+    out = HF.differential_attention(*leaves, lens, causal)
+    _within(out, want["o"], "o")
+    for g, name in zip(torch.autograd.grad(out, leaves, do), ("dq", "dk", "dv", "dlam")):
+        _within(g, want[name], name)
+
+
 def test_attention_infinite_scores_of_narrow_heads(cuda_device):
     """a key whose last element is -inf has weight 0 for the queries that are positive there (heads narrower than the kernels' width: the
     elements that are not there must not meet the infinity)"""
