@@ -4,6 +4,7 @@
 // it Python objects moving between the caller's thread and autograd's.  This file does only what the Python functions did -- allocate with
 // torch, fill in the C ABI's argument structures, launch on the current stream, keep what the backward needs; kernels and their rules
 // are behind the C ABI (include/immunostruct_hip.h), whose entry points are handed over at import (bind) so that one library serves both.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
@@ -53,6 +54,19 @@ Tensor aligned(const Tensor& t) {
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the sequence operators are differentiable once: no create_graph=True"); }
+
+// A leaf whose gradient node an eager graph on another stream keeps alive cannot be differentiated in a capture: the engine would make that stream wait
+// for the captured one, which ends the capture and with it the process.  Refused while nothing is captured yet.
+void capturable(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (!stream.has_value() || stream->id() == c10::hip::getCurrentHIPStream(t->device().index()).id()) continue;
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "the sequence operators: an eager graph of a captured leaf is still alive; release its outputs before the capture");
+  }
+}
 
 // ---- rotary ----------------------------------------------------------------------------------------------------------------------------
 struct Turn {
@@ -107,6 +121,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 std::pair<Tensor, OptTensor> rotary(const Tensor& q, const OptTensor& k_, const Tensor& freq, const OptTensor& positions_, bool interleaved, double amplitude) {
   const Tensor k = value(k_), positions = value(positions_);
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k))) {
+    capturable({&q, &k});
     variable_list out = Rotary::apply(q, k_, positions_, freq, interleaved, amplitude);
     return {out[0], k.defined() ? OptTensor(out[1]) : std::nullopt};
   }
@@ -193,7 +208,10 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
 };
 
 Tensor differential_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptTensor& lengths, int64_t causal, double scale) {
-  if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v) || wanted(lam))) return DiffAttention::apply(q, k, v, lam, lengths, causal, scale);
+  if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v) || wanted(lam))) {
+    capturable({&q, &k, &v, &lam});
+    return DiffAttention::apply(q, k, v, lam, lengths, causal, scale);
+  }
   return diff_forward(sequence_rows(q, q.size(2)), sequence_rows(k, 1), sequence_rows(v, 0), lam.contiguous(), value(lengths), causal, scale, false).out;
 }
 
@@ -256,7 +274,10 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 Tensor group_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, const OptTensor& lengths_, int64_t groups, double eps, int64_t activation) {
   const Tensor weight = value(weight_), bias = value(bias_), lengths = value(lengths_);
-  if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight) || wanted(bias))) return GroupNorm::apply(x, weight_, bias_, lengths_, groups, eps, activation);
+  if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight) || wanted(bias))) {
+    capturable({&x, &weight, &bias});
+    return GroupNorm::apply(x, weight_, bias_, lengths_, groups, eps, activation);
+  }
   return norm_forward(unit_rows(x), weight, bias, lengths, groups, eps, activation).first;
 }
 

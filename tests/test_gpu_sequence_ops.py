@@ -451,6 +451,30 @@ def test_block_in_captured_graphs(cuda_device):
             assert all(torch.equal(x, y) for x, y in zip(want, held))
 
 
+def test_capture_beside_a_living_eager_graph_is_refused(cuda_device):
+    """an eager graph of the same leaves on another stream: the capture is refused with an error before anything is recorded, and works once the
+    eager outputs are gone"""
+    q, k, v, lam = (t.requires_grad_(True) for t in _attention_inputs(torch.bfloat16, 1, 40, 40, 2, 2, 16, 32))
+    x, w, o = (_randn(*s, dtype=torch.float32, seed=i).requires_grad_(True) for i, s in enumerate([(3, 8), (8,), (8,)]))
+    freq = HN.RotaryEmbedding(16).freq
+    calls = [lambda: HF.differential_attention(q, k, v, lam), lambda: HF.group_norm(x, 2, w, o), lambda: HF.rotary(q, k, freq)[1]]
+    eager = [f() for f in calls]
+    torch.cuda.synchronize()
+    for f in calls:
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                f()
+    want = [e.detach().clone() for e in eager]
+    del eager
+    for f, value in zip(calls, want):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held = f()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, value)
+
+
 def test_token_equals_the_last_row_of_the_prompt(cuda_device):
     """serving: the new token over the cache against the same position of the whole causal pass (another kernel and summation order)"""
     for dtype in TYPES:
