@@ -15,7 +15,7 @@
 //   long  a sample does not fit: row blocks leave (mean, M2) / (sum t, sum t xhat) of every group, a small launch joins a sample's blocks (one
 //         wave per sample and group; done by every workgroup of the next pass it cost 50 us at (2, 65536, 512), 32 groups), a third
 //         writes.  Block sums are taken about each thread's own first value, so a large mean costs no precision
-//         ((2, 65536, 512) bf16, 32 groups: 30 + 6 + 50 us forward, 68 + 5 + 73 + 6 backward; 940 MB in all, 4.1 TB/s).
+//         ((2, 65536, 512) bf16, 32 groups: 30 + 6 + 50 us forward, 68 + 5 + 73 + 6 backward; eight passes of 134 MB in all, 4.5 TB/s).
 //         Groups of more than 256 chunks are cut into parts, which join like row blocks ((4, 2048, 4096) bf16, one group: 50 us forward, 94
 //         backward; a workgroup per sample and group that re-reads took 26 and 19 ms).
 // Chunks are 16 bytes where pointers, strides and the group width allow, single elements otherwise (a chunk never straddles two groups).
