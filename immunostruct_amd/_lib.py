@@ -149,7 +149,7 @@ class CopyJob(ctypes.Structure):
 
 class DiffAttention(ctypes.Structure):
     """arguments of is_diff_attention_{fwd,bwd} (mirrors `IsDiffAttention` in include/immunostruct_hip.h)"""
-    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "lam", "lengths", "o", "o2", "lse", "work", "d_o", "dots", "dq", "dk",
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "lam", "lengths", "o", "maps", "lse", "work", "d_o", "dots", "dq", "dk",
                                                "dv_out", "dlam")] + \
                [(n, ctypes.c_longlong) for n in ("q_b", "q_n", "q_h", "k_b", "k_n", "k_h", "v_b", "v_n", "v_h")] + \
                [(n, ctypes.c_int) for n in ("batch", "nq", "nk", "heads", "kv_heads", "d", "dv", "causal", "type", "lam_type", "splits",

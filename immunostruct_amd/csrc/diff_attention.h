@@ -18,10 +18,10 @@
 //   backward  dP = dO V^T; D_m = dO . O_m; dS_1 = P1 (dP - D_1), dS_2 = -lam P2 (dP - D_2);
 //             dQ_m = scale dS_m K_m, dK_m = scale dS_m^T Q_m, dV = (P1 - lam P2)^T dO, dlam = -sum D_2.  Scores are recomputed from lse.
 //             dK / dV: a wave owns 32 keys and walks the rows; dQ: a wave owns 32 rows and walks the keys.
-// Scores, sums, lse, D and all accumulators are 32-bit.  P and dS are rounded once to the inputs' type, which the matrix instructions ask of both
-// operands: half a step per term, of random sign, about as much as the output's own rounding (0.0025 of the norm in bf16 where the output's
-// alone is 0.0017).  The softmax sums are taken before it.  Up to 32 rows (single tokens, bound by the cache's bytes) the forward multiplies what
-// the rounding left out as well: 0.0017, 74.6 -> 76 - 78 us at 16 tokens; long sequences would pay 285 -> 417 us at (2, 4096, 16 / 4 heads, 64 / 128).
+// Scores, sums, lse, D, the maps' own products that D is formed from and all accumulators are 32-bit; only results are rounded to the inputs' type.  P
+// and dS are the left operands of 16-bit matrix instructions: they enter as two terms (mm_transposed), for any number of rows.  At (2, 4096, 16 / 4 heads,
+// 64 / 128, bf16, causal) that is 1430 us a training pass where one rounding took 1016, and results are as far from 64 bits as their own rounding is (0.0017
+// of the norm in bf16, 0.0002 in fp16; one rounding: 0.0027, 0.0003); single tokens are bound by the cache's bytes and pay nothing.
 #pragma once
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
@@ -84,6 +84,8 @@ __device__ __forceinline__ int query_of(const Args& a, int r, int& g) {
 }
 // element (b, query i, head h) of a contiguous (batch, nq, heads, dv) tensor
 __device__ __forceinline__ long long o_at(const Args& a, int b, int i, int h) { return (((long long)b * a.nq + i) * a.heads + h) * a.dv; }
+// elements of one map's product in `maps` (2, batch, nq, heads, dv)
+__device__ __forceinline__ long long maps_plane(const Args& a) { return (long long)a.batch * a.nq * a.heads * a.dv; }
 
 // The two maps' rows of a tile lie behind each other: tile rows [0, n) are map 0's, [n, 2 n) map 1's (MAPS = 2; 1: values, one set).
 // byte offsets of a tile's key rows, clamped to the last valid one, from its first row
@@ -235,11 +237,6 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
         }
         sum += add;
         mm_transposed<T, DV, NT>(o, buf + v_at, p);
-        if constexpr (GROUPS == 1 && SZ == 2) {      // a handful of rows: what the rounding left out is multiplied as well
-#pragma unroll
-          for (int t = 0; t < 16; ++t) p[t] -= (float)(T)p[t];
-          mm_transposed<T, DV, NT>(o, buf + v_at, p);
-        }
       }
       if (more) {
         place(lds + (CUR ^ 1) * BUF);
@@ -270,13 +267,13 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
     for (int e = 0; e < 16; ++e) o[t][e] *= inv;
   if (a.lse != nullptr && live && g == 0) a.lse[((long long)base * 2 + map) * R + r] = total != 0.0f ? __builtin_fmaf(top, c, __log2f(total)) : INFINITY;
   const long long at = o_at(a, b, query, head);
-  if (a.o2 != nullptr && live && map == 1) {
-    T* out2 = reinterpret_cast<T*>(a.o2) + at;
+  if (a.maps != nullptr && live) {
+    float* mine = a.maps + map * maps_plane(a) + at;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        store4<T, VEC>(out2, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[t][4 * u], o[t][4 * u + 1], o[t][4 * u + 2], o[t][4 * u + 3]});
+        store4<float, VEC>(mine, 32 * t + 8 * u + 4 * g, a.dv, f32x4{o[t][4 * u], o[t][4 * u + 1], o[t][4 * u + 2], o[t][4 * u + 3]});
   }
   const float lam = lam_at<T>(a, head);
   T* out = reinterpret_cast<T*>(a.o) + at;
@@ -346,7 +343,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   }
   const float lam = lam_at<T>(a, head);
   T* out = reinterpret_cast<T*>(a.o) + o_at(a, b, query, head);
-  T* out2 = reinterpret_cast<T*>(a.o2) + o_at(a, b, query, head);
+  float* maps = a.maps + o_at(a, b, query, head);
   for (int c0 = 0; c0 < a.dv; c0 += 128) {      // (uniform over a row's waves)
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};      // two columns of map 0, two of map 1
     for (int s0 = wave; s0 < a.splits; s0 += WAVES * BATCH) {
@@ -375,7 +372,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
         const int col = c0 + 2 * lane + e;
         if (col < a.dv) {
           out[col] = (T)(acc[e] - lam * acc[2 + e]);
-          if (a.o2 != nullptr) out2[col] = (T)acc[2 + e];
+          if (a.maps != nullptr) {
+            maps[col] = acc[e];
+            maps[maps_plane(a) + col] = acc[2 + e];
+          }
         }
       }
     }
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
-// D_2 = dO . O_2 and D_1 = dO . O + lam D_2 of every row (16 lanes per row); bound by bytes: 17.7 us for 3 x 33.5 MB (5.7 TB/s, partly cached)
+// D_1 = dO . O_1 and D_2 = dO . O_2 of every row (16 lanes per row), of the maps' own unrounded products; bound by bytes
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   constexpr int N = Vec<T>::N;
@@ -394,25 +394,26 @@ __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
   int gi;
   const int query = query_of(a, r, gi), head = hk * a.group + gi;
-  const long long at = o_at(a, b, query, head) * sizeof(T);
-  const char *o = reinterpret_cast<const char*>(a.o) + at, *o2 = reinterpret_cast<const char*>(a.o2) + at, *go = reinterpret_cast<const char*>(a.d_o) + at;
-  float s = 0.0f, s2 = 0.0f;
+  const long long at = o_at(a, b, query, head);
+  const char* go = reinterpret_cast<const char*>(a.d_o) + at * sizeof(T);
+  const char* maps[2] = {reinterpret_cast<const char*>(a.maps + at), reinterpret_cast<const char*>(a.maps + maps_plane(a) + at)};
+  float s[2] = {0.0f, 0.0f};
   for (int c = lane; c * N < a.dv; c += 16) {
-    float x[N], y[N], y2[N];
+    float x[N], y[4];
     Vec<T>::unpack(load_chunk<T, VEC>(go, c, a.dv), x);
-    Vec<T>::unpack(load_chunk<T, VEC>(o, c, a.dv), y);
-    Vec<T>::unpack(load_chunk<T, VEC>(o2, c, a.dv), y2);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      s += x[e] * y[e];
-      s2 += x[e] * y2[e];
-    }
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int u = 0; u < N / 4; ++u) {
+        Vec<float>::unpack(load_chunk<float, VEC>(maps[m], c * (N / 4) + u, a.dv), y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[m] += x[4 * u + e] * y[e];
+      }
   }
-  s = sum_over_r16(s);
-  s2 = sum_over_r16(s2);
-  if (lane == 0) {
-    a.dots[(base * 2) * R + r] = s + lam_at<T>(a, head) * s2;
-    a.dots[(base * 2 + 1) * R + r] = s2;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    s[m] = sum_over_r16(s[m]);
+    if (lane == 0) a.dots[(base * 2 + m) * R + r] = s[m];
   }
 }
 

@@ -9,7 +9,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // what both directions check; fills in the derived fields
 int prepare(da::Args& a) {
-  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.lam == nullptr || a.o == nullptr) return -22;
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.lam == nullptr) return -22;
   if (a.batch < 1 || a.nq < 1 || a.nk < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.d < 1 || a.dv < 1) return -22;
   if (a.type < TYPE_F32 || a.type > TYPE_F16 || (a.lam_type != TYPE_F32 && a.lam_type != a.type) || a.causal < 0 || a.causal > 2) return -22;
   if (!(a.scale > 0.0f) || !(a.scale < 2e38f) || a.splits < 1 || a.splits > 64 || a.row_splits < 1) return -22;
@@ -25,7 +25,7 @@ int prepare(da::Args& a) {
   if (a.q_n < 0 || a.q_h < 0 || a.k_n < 0 || a.k_h < 0 || a.v_n < 0 || a.k_h > near / 4 || a.q_n > near / 64 || a.k_n > near / 64 || a.v_n > near / 64 ||
       a.q_h > near / 4 / a.group || (long long)a.heads * a.dv > near / 64) return -22;
   const long long strides = a.q_b | a.q_n | a.q_h | a.k_b | a.k_n | a.k_h | a.v_b | a.v_n | a.v_h;
-  a.vec = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.o) && aligned16(a.o2) && aligned16(a.d_o) && aligned16(a.dq) &&
+  a.vec = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.o) && aligned16(a.maps) && aligned16(a.d_o) && aligned16(a.dq) &&
           aligned16(a.dk) && aligned16(a.dv_out) && strides % n == 0 && a.d % n == 0 && a.dv % n == 0;
   return da::class_of(a) == 0 ? -38 : 0;
 }
@@ -81,7 +81,7 @@ int is_diff_attention_fwd(const IsDiffAttention* args, void* stream) {
   a.row_splits = 1;
   const int rc = prepare(a);
   if (rc != 0) return fail("is_diff_attention_fwd", rc);
-  if ((a.lse == nullptr) != (a.o2 == nullptr) || (a.splits > 1 && a.work == nullptr)) return fail("is_diff_attention_fwd", -22);
+  if (a.o == nullptr || (a.lse == nullptr) != (a.maps == nullptr) || (a.splits > 1 && a.work == nullptr)) return fail("is_diff_attention_fwd", -22);
   return run(a, false, "is_diff_attention_fwd", stream);
 }
 
@@ -89,9 +89,10 @@ int is_diff_attention_bwd(const IsDiffAttention* args, void* stream) {
   if (args == nullptr) return fail("is_diff_attention_bwd", -22);
   da::Args a = *args;
   a.splits = 1;
+  a.o = nullptr;
   const int rc = prepare(a);
   if (rc != 0) return fail("is_diff_attention_bwd", rc);
-  if (a.o2 == nullptr || a.lse == nullptr || a.d_o == nullptr || a.dots == nullptr || a.dq == nullptr || a.dk == nullptr ||
+  if (a.maps == nullptr || a.lse == nullptr || a.d_o == nullptr || a.dots == nullptr || a.dq == nullptr || a.dk == nullptr ||
       a.dv_out == nullptr || a.dlam == nullptr || (a.row_splits > 1 && a.work == nullptr))
     return fail("is_diff_attention_bwd", -22);
   return run(a, true, "is_diff_attention_bwd", stream);

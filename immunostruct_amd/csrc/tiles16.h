@@ -115,7 +115,10 @@ __device__ __forceinline__ f32x16 mm_tiles(const char* at, const char* other) {
   return acc;
 }
 
-// acc[t] (32 x 32: rows = columns 32 t .. of the tile, columns = p's columns) += (32 tile rows)^T . p;  `at` = tile + columns_at(lane) of the first row
+// acc[t] (32 x 32: rows = columns 32 t .. of the tile, columns = p's columns) += (32 tile rows)^T . p;  `at` = tile + columns_at(lane) of the first row.
+// The 16-bit matrix instructions take both operands in 16 bits: p goes in as two terms, its rounding and the rounding of what that left out (2^-16 of p
+// at most remains in bf16, 2^-22 in fp16), which meet the same tile read.  One term alone is off by up to
+// half a step per weight, which added as much error to a result as its own rounding does (0.0025 of the norm for 0.0017 in bf16).
 template <typename T, int N, int NT>
 __device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NT], const char* at, const f32x16& p) {
   if constexpr (sizeof(T) == 4) {
@@ -131,10 +134,13 @@ __device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NT], const char* at,
     // 16 lanes read 4 rows x 16 columns (lane i: row i / 4, columns 4 (i mod 4) ..) and receive column i of the 4 rows
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      V v;
+      V v, w;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)p[8 * h + e];      // one rounding to the inputs' type: what the matrix instruction takes
-      const u32x4_t b = __builtin_bit_cast(u32x4_t, v);
+      for (int e = 0; e < 8; ++e) {
+        v[e] = (T)p[8 * h + e];
+        w[e] = (T)(p[8 * h + e] - (float)v[e]);
+      }
+      const u32x4_t b = __builtin_bit_cast(u32x4_t, v), rest = __builtin_bit_cast(u32x4_t, w);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         u32x2 half[2];
@@ -142,7 +148,9 @@ __device__ __forceinline__ void mm_transposed(f32x16 (&acc)[NT], const char* at,
         for (int w = 0; w < 2; ++w)
           half[w] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (__attribute__((address_space(3))) s16x4*)(at + 8 * (2 * h + w) * Tile<T, N>::STRIDE + t * 64)));
-        acc[t] = mfma_chunk<T>(u32x4_t{half[0][0], half[0][1], half[1][0], half[1][1]}, b, acc[t]);
+        const u32x4_t a = {half[0][0], half[0][1], half[1][0], half[1][1]};
+        acc[t] = mfma_chunk<T>(a, b, acc[t]);
+        acc[t] = mfma_chunk<T>(a, rest, acc[t]);
       }
     }
   }

@@ -151,7 +151,7 @@ IsDiffAttention diff_args(const Tensor& q, const Tensor& k, const Tensor& v, con
 }
 
 struct Attended {
-  Tensor out, o2, lse;
+  Tensor out, maps, lse;
 };
 Attended diff_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& lengths, int64_t causal, double scale, bool need) {
   const c10::DeviceGuard guard(q.device());
@@ -160,7 +160,7 @@ Attended diff_forward(const Tensor& q, const Tensor& k, const Tensor& v, const T
   Attended r;
   r.out = at::empty({a.batch, a.nq, a.heads, a.dv}, q.options());
   if (need) {
-    r.o2 = like(r.out);
+    r.maps = floats(q, {2, a.batch, a.nq, a.heads, a.dv});
     r.lse = floats(q, {a.batch, a.kv_heads, 2, rows});
   }
   if (r.out.numel() == 0 || a.nk == 0) {      // nobody asks, or there is nothing to see
@@ -171,7 +171,7 @@ Attended diff_forward(const Tensor& q, const Tensor& k, const Tensor& v, const T
   const long long need_floats = entry.work_floats(a.batch, a.kv_heads, rows, a.dv, a.splits);
   Tensor work;
   if (need_floats > 0) work = floats(q, {(int64_t)need_floats});
-  a.o = r.out.data_ptr(), a.o2 = ptr(r.o2), a.lse = static_cast<float*>(ptr(r.lse)), a.work = static_cast<float*>(ptr(work));
+  a.o = r.out.data_ptr(), a.maps = static_cast<float*>(ptr(r.maps)), a.lse = static_cast<float*>(ptr(r.lse)), a.work = static_cast<float*>(ptr(work));
   check(entry.diff_fwd(&a, stream_of(q)), "is_diff_attention_fwd");
   return r;
 }
@@ -181,7 +181,7 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
     const Tensor lengths = value(lengths_);
     const Tensor q = sequence_rows(q_, q_.size(2)), k = sequence_rows(k_, 1), v = sequence_rows(v_, 0), lam = lam_.contiguous();
     Attended r = diff_forward(q, k, v, lam, lengths, causal, scale, true);
-    ctx->save_for_backward({q, k, v, lam, lengths, r.out, r.o2, r.lse});
+    ctx->save_for_backward({q, k, v, lam, lengths, r.maps, r.lse});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return r.out;
@@ -189,17 +189,17 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once();
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &lam = s[3], &lse = s[7];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &lam = s[3], &maps = s[5], &lse = s[6];
     const c10::DeviceGuard guard(q.device());
     Tensor dq = like(q), dk = like(k), dv = like(v), dlam = like(lam);
-    if (s[5].numel() == 0 || v.size(1) == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), Tensor(), Tensor(), Tensor()};
+    if (maps.numel() == 0 || v.size(1) == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), Tensor(), Tensor(), Tensor()};
     const Tensor g = aligned(grads[0]);
     IsDiffAttention a = diff_args(q, k, v, lam, s[4], ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble());
     const int rows = (int)lse.size(3);
     a.row_splits = entry.row_splits(a.batch, a.kv_heads, rows, a.nk, a.causal);
     const int64_t parts = entry.row_work_floats(a.batch, a.kv_heads, a.nk, a.d, a.dv, a.row_splits);
     Tensor work = floats(q, {parts + 3LL * a.batch * a.kv_heads * rows});      // the row splits' sums, then the rows' three dot products
-    a.o = s[5].data_ptr(), a.o2 = s[6].data_ptr(), a.lse = lse.data_ptr<float>(), a.d_o = g.data_ptr();
+    a.maps = maps.data_ptr<float>(), a.lse = lse.data_ptr<float>(), a.d_o = g.data_ptr();
     a.work = work.data_ptr<float>(), a.dots = a.work + parts;
     a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv_out = dv.data_ptr(), a.dlam = dlam.data_ptr();
     check(entry.diff_bwd(&a, stream_of(q)), "is_diff_attention_bwd");

@@ -1814,8 +1814,8 @@ def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
     ``causal``: None; "start": query i is position i and sees keys <= i; "end": the queries are the sample's last nq positions, i.e. new
     tokens over a cache, and see keys <= i + length - nq.  ``scale``: a positive number, d ** -0.5 by default.
     Keys that no query sees may hold anything; a key that the order hides from some queries only has to hold numbers (its weight there is 0).
-    A query that sees no key gives zeros and passes no gradient.  Returns (B, nq, heads, dv).  Deterministic; scores, softmax statistics
-    and sums are 32-bit, softmax weights and score gradients are rounded once to the inputs' type for the matrix products."""
+    A query that sees no key gives zeros and passes no gradient.  Returns (B, nq, heads, dv).  Deterministic; scores, softmax weights
+    and statistics, score gradients and sums are 32-bit: nothing but the results is rounded to the inputs' type."""
     _sequence_type("differential_attention", q, k, v)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or lam.dim() != 1:
         raise ValueError("differential_attention: expected q (B, nq, 2 heads, d), k (B, nk, 2 kv_heads, d), v (B, nk, kv_heads, dv), lam (heads,)")

@@ -447,17 +447,17 @@ int is_rotary(const void* q, long long q_b, long long q_n, long long q_h, void* 
  *   not exist.  causal: 0 every key, 1 query i sees keys <= i, 2 the queries are the last nq positions (keys <= i + length - nq).
  *   A row that sees no key gives 0 and no gradient.  d <= 128 and dv <= 256 (fp32: 64 and 128); -38 beyond.
  * is_diff_attention_fwd: reads q, k, v, lam, lengths; writes o (batch, nq, heads, dv); lse (batch, kv_heads, 2, nq heads / kv_heads; fp32) and
- *   o2 (like o: the second map's product) are what the backward needs, both or neither.  splits = is_diff_attention_splits(...) ranges of
+ *   maps (2, batch, nq, heads, dv; fp32: each map's own product) are what the backward needs, both or neither.  splits = is_diff_attention_splits(...) ranges of
  *   the keys per row (1: none); splits > 1 needs work[is_diff_attention_work_floats(...)] (rows = nq heads / kv_heads in both).
- * is_diff_attention_bwd: reads those and d_o (contiguous); writes dq, dk, dv_out (contiguous), dlam (lam's type); dots: scratch of 1.5
+ * is_diff_attention_bwd: reads those two, the inputs and d_o (contiguous), not o; writes dq, dk, dv_out (contiguous), dlam (lam's type); dots: scratch of 1.5
  *   times lse's size; row_splits = is_diff_attention_row_splits(...) parts of the rows per key tile (1: none), more than one need
  *   work[is_diff_attention_row_work_floats(...)].  rows, group, vec and group_magic are set by the library.  Row strides below 2^31 / 64
  *   bytes.  No atomics: bitwise reproducible.                                                                                         */
 typedef struct {
   const void *q, *k, *v, *lam;
   const int* lengths;
-  void *o, *o2;
-  float *lse, *work;
+  void* o;
+  float *maps, *lse, *work;
   const void* d_o;
   float* dots;
   void *dq, *dk, *dv_out, *dlam;

@@ -118,11 +118,16 @@ def group_norm(x, groups, weight, bias, eps, activation, lengths, dy=None):
     return {**out, **grads}
 
 
-def differential_attention(q, k, v, lam, lengths, causal, scale, do=None):
+def differential_attention(q, k, v, lam, lengths, causal, scale, do=None, full=False):
     """Scores: d products summed in 32 bits (d e of the sum of magnitudes), an exponential (8 e); weights P rounded once (u) for the product
-    with V, summed in 32 bits (64 e: chains per 32 keys and the rescalings); D from the rounded outputs (u each); dS rounded once (u)."""
+    with V, summed in 32 bits (64 e: chains per 32 keys and the rescalings); D from the rounded outputs (u each); dS rounded once (u).
+
+    ``full``: nothing but the results is rounded to the type.  P and dS enter as two terms of the type, the second one the first one's remainder
+    (at most u of it, rounded by u: u^2 is left out of 1), and D is a sum in 32 bits over 32-bit factors (no u)."""
     u = half_step(q.dtype) if q.dtype != torch.float32 else 0.0      # 32-bit operands enter the matrix instructions as they are
     ot, tiny = half_step(q.dtype), tiny_step(q.dtype)
+    saved, saved_tiny = (0.0, 0.0) if full else (ot, tiny)      # of the outputs that D is formed from
+    u = u * u if full else u
     Q, K, V, L = _d(q), _d(k), _d(v), _d(lam)
     b, nq, h2, d = Q.shape
     nk, hk, dv = V.shape[1:]
@@ -171,9 +176,9 @@ def differential_attention(q, k, v, lam, lengths, causal, scale, do=None):
             out["dv"][1][i, :n, kv] += (dw + u * wa + 2 * sub + 64 * E32 * wa).t() @ ga
             dp, dpa = g @ val.t(), (dv + 4) * E32 * (ga @ val.abs().t())
             d2 = (g * o[1]).sum(1, keepdim=True)
-            e2 = (ga * (do_[1] + ot * o[1].abs() + tiny + dv * E32 * o[1].abs())).sum(1, keepdim=True)
+            e2 = (ga * (do_[1] + saved * o[1].abs() + saved_tiny + dv * E32 * o[1].abs())).sum(1, keepdim=True)
             d1 = (g * o[0]).sum(1, keepdim=True)
-            e1 = (ga * (err_o + ot * res.abs() + tiny + dv * E32 * res.abs())).sum(1, keepdim=True) + lm.abs() * (e2 + dv * E32 * (ga * o[1].abs()).sum(1, keepdim=True))
+            e1 = (ga * (err_o + saved * res.abs() + saved_tiny + dv * E32 * res.abs())).sum(1, keepdim=True) + lm.abs() * (e2 + dv * E32 * (ga * o[1].abs()).sum(1, keepdim=True))
             out["dlam"][0][head] -= d2.sum()
             out["dlam"][1][head] += e2.sum() + (b * nq / 1024 + 32) * E32 * d2.abs().sum()
             for m, (sign, dm, em) in enumerate(((1.0, d1, e1), (-lm, d2, e2))):
