@@ -30,7 +30,11 @@ namespace is {
 namespace da {
 
 typedef IsDiffAttention Args;
-constexpr float SLACK = 8.0f;      // log2 of how far a weight may pass 1 before the running maximum follows
+// The forward's weights are taken as 2^LIFT exp(score - running maximum), which may fall behind the true one by 2^SLACK.  fp16 has no steps below 2^-24:
+// there the largest weight is kept at 2^11 ... 2^15, so that what is lost lies below 2^-36 of it (unlifted, 4000 keys of weight 2^-26 beside one of weight 1
+// came out as nothing).  The other types have fp32's range; the larger slack makes rescaling rarer.
+template <typename T> constexpr float lift_of() { return __is_same(T, _Float16) ? 11.0f : 0.0f; }
+template <typename T> constexpr float slack_of() { return __is_same(T, _Float16) ? 4.0f : 8.0f; }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <int V> struct Int { static constexpr int value = V; };
@@ -143,6 +147,36 @@ __device__ __forceinline__ void hand_over(const f32x16 (&acc)[NT], char* lds, in
   }
 }
 
+// Keeps the left operands of a sum of products inside fp16's range: x is multiplied by a power of two of the lane's column, chosen at the first values and
+// lowered (with the sums so far) only when one passes 2^15; values below 2^-34 of a column's largest are lost.  Score gradients are P dO V: over thousands of
+// keys, or of small upstream gradients, they lie far below fp16's steps while the sums they belong to do not (dO of 1e-4 over 4096 keys: dQ was off by 6 x
+// what rounding it costs), and large ones pass its largest number.  The other types have fp32's range and take x as it is.
+template <typename T>
+struct ColumnScale {
+  static constexpr bool USED = __is_same(T, _Float16);
+  float factor = USED ? 0x1p60f : 1.0f;
+  template <int NT>
+  __device__ __forceinline__ void fit(f32x16& x, f32x16 (&acc)[NT]) {
+    if constexpr (USED) {
+      float high = fabsf(x[0]);
+#pragma unroll
+      for (int t = 1; t < 16; ++t) high = fmaxf(high, fabsf(x[t]));
+      if (__any(high * factor > 0x1p15f)) {
+        const float most = fmaxf(high, other_half(high));      // (both halves of a wave hold rows of the same 32 columns)
+        const float now = most * factor > 0x1p15f ? __builtin_ldexpf(1.0f, 10 - __builtin_amdgcn_frexp_expf(most)) : factor;
+        const float shrink = now / factor;
+        factor = now;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[t][e] *= shrink;
+      }
+#pragma unroll
+      for (int t = 0; t < 16; ++t) x[t] *= factor;
+    }
+  }
+};
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
 // grid: (row tiles x splits x kv_heads x batch), GROUPS x 2 waves of 32 rows and one map.  splits > 1: every workgroup takes one range of the
 // keys and leaves unnormalised sums with their maxima in the workspace; join_kernel puts them together.
@@ -173,6 +207,7 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
   const int per = ((wg_end + a.splits - 1) / a.splits + KT - 1) / KT * KT;
   const int first = split * per, last = min(wg_end, first + per);
   const float c = a.scale * 1.44269504088896340736f;
+  constexpr float LIFT = lift_of<T>(), SLACK = slack_of<T>();
 
   u32x4_t q[NJ];
   const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + query * a.q_n + (2 * head + map) * a.q_h) * SZ;
@@ -181,7 +216,7 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
   const int k_at = map * KB + Tile<T, D>::rows_at(lane), v_at = 2 * KB + Tile<T, DV>::columns_at(lane);
   f32x16 o[NT];
   zero_acc(o);
-  float top = -INFINITY, ref = 0.0f, sum = 0.0f;      // ref: what the exponents are taken against (-top c; 0 before the first key)
+  float top = -INFINITY, ref = 0.0f, sum = 0.0f;      // ref: what the exponents are taken against (LIFT - top c; 0 before the first key)
 
   typedef Stage<T, D, 2 * KT, NTH, VEC> StageK;
   typedef Stage<T, DV, KT, NTH, VEC> StageV;
@@ -222,7 +257,7 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
           const float now = fmaxf(top, fmaxf(high, other_half(high)));
           const float shrink = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - now) * c);
           top = now;
-          ref = now == -INFINITY ? 0.0f : -now * c;
+          ref = now == -INFINITY ? 0.0f : LIFT - now * c;
           sum *= shrink;
 #pragma unroll
           for (int t = 0; t < NT; ++t)
@@ -250,7 +285,7 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
     if (!live) return;
     float* w = a.work + (((long long)base * a.splits + split) * 2 + map) * ((long long)R * (a.dv + 2)) + (long long)r * (a.dv + 2);
     if (g == 0) {
-      w[a.dv] = top == -INFINITY ? -INFINITY : top * c;
+      w[a.dv] = top == -INFINITY ? -INFINITY : top * c - LIFT;
       w[a.dv + 1] = total;
     }
 #pragma unroll
@@ -265,7 +300,7 @@ __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2)
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[t][e] *= inv;
-  if (a.lse != nullptr && live && g == 0) a.lse[((long long)base * 2 + map) * R + r] = total != 0.0f ? __builtin_fmaf(top, c, __log2f(total)) : INFINITY;
+  if (a.lse != nullptr && live && g == 0) a.lse[((long long)base * 2 + map) * R + r] = total != 0.0f ? __builtin_fmaf(top, c, __log2f(total)) - LIFT : INFINITY;
   const long long at = o_at(a, b, query, head);
   if (a.maps != nullptr && live) {
     float* mine = a.maps + map * maps_plane(a) + at;
@@ -477,6 +512,8 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
   f32x16 dk[NT], dv[NTV];
   zero_acc(dk);
   zero_acc(dv);
+  ColumnScale<T> range;
+  float lift = 0.0f;      // fp16: the weights are taken 2^lift times as large, up to 2^15 (over thousands of keys they lie below its normal range)
   bool flip = false;
   const int seen_from = wg_key < len ? first_query(a, wg_key, len) * a.group / RT * RT : R;
   const int per = ((R - seen_from + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
@@ -503,7 +540,13 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
     float st = 0.0f;
     const char* qp = reinterpret_cast<const char*>(a.q) + (b * a.q_b + 2 * hk * a.group * a.q_h) * SZ;
     const char* op = reinterpret_cast<const char*>(a.d_o) + o_at(a, b, 0, hk * a.group) * SZ;
-    for (int gi = 0; gi < a.group; ++gi) flip = flip || lam_at<T>(a, hk * a.group + gi) < 0.0f;
+    float largest = 1.0f;
+    for (int gi = 0; gi < a.group; ++gi) {
+      const float lam = lam_at<T>(a, hk * a.group + gi);
+      flip = flip || lam < 0.0f;
+      largest = fmaxf(largest, fabsf(lam));
+    }
+    if constexpr (ColumnScale<T>::USED) lift = largest < 0x1p100f ? (float)(15 - __builtin_amdgcn_frexp_expf(largest)) : 0.0f;
     static_assert(NTH >= 6 * RT, "a thread stages one statistic");
     const int sw = tid >> 5, sm = sw >= 3 ? 1 : 0, sk = sw - 3 * sm;      // which statistic of which map
     // a tile of 32 rows holds whole queries where the group divides 32: its rows' offsets then are the same in every tile
@@ -516,7 +559,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
       int gi;
       query_of(a, min(r0 + (tid & 31), R - 1), gi);
       const float lam = sm == 0 ? 1.0f : lam_at<T>(a, hk * a.group + gi);
-      extra = sk == 0 ? -__log2f(fabsf(lam)) : sk == 1 ? 0.0f : lam < 0.0f ? -1.0f : 1.0f;
+      extra = sk == 0 ? -__log2f(fabsf(lam)) - lift : sk == 1 ? 0.0f : lam < 0.0f ? -1.0f : 1.0f;
     };
     offsets(r_first, r_first / a.group);
     auto fetch = [&](int r0) {
@@ -573,6 +616,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
           }
         }
         mm_transposed<T, DV, NTV>(dv, buf + gt_at, w);
+        range.fit(ds, dk);
         mm_transposed<T, D, NT>(dk, buf + qt_at, ds);
       }
       if (more) {
@@ -584,6 +628,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
   const bool live = key < len, there = key < a.nk;      // (rows behind the length: the clamped key's sums are not theirs)
   const long long at = ((long long)b * a.nk + key) * a.kv_heads + hk;
   const int width = 2 * a.d + a.dv;
+  const float lower = __builtin_amdgcn_exp2f(-lift), back = lower / range.factor;
   float* part = a.work + ((long long)split * a.batch * a.nk * a.kv_heads + at) * width;      // [split][sample, key, head][dk1 | dk2 | dv]
   auto put = [&](int which, int col, f32x4 x) {
     if (!there) return;
@@ -597,7 +642,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
     for (int u = 0; u < 4; ++u) {
       f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dk[t][4 * u + e] * (map == 0 ? a.scale : -a.scale);
+      for (int e = 0; e < 4; ++e) x[e] = dk[t][4 * u + e] * back * (map == 0 ? a.scale : -a.scale);
       put(map, 32 * t + 8 * u + 4 * g, x);
     }
   hand_over<NTV, GROUPS, 2 * BUF>(dv, lds, group, map, lane, [&](int t, const f32x16& x, const f32x16& y) {
@@ -605,7 +650,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
     for (int u = 0; u < 4; ++u) {
       f32x4 z;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = x[4 * u + e] - y[4 * u + e];
+      for (int e = 0; e < 4; ++e) z[e] = (x[4 * u + e] - y[4 * u + e]) * lower;
       put(2, 32 * t + 8 * u + 4 * g, z);
     }
   });
@@ -678,6 +723,7 @@ __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_wa
   const char* own = gt + Tile<T, DV>::bytes(32) * group + Tile<T, DV>::rows_at(lane);
   f32x16 dq[NT];
   zero_acc(dq);
+  ColumnScale<T> range;
   typedef Stage<T, D, 2 * KT, NTH, VEC> StageK;
   typedef Stage<T, DV, KT, NTH, VEC> StageV;
   StageK sk;
@@ -728,6 +774,7 @@ __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_wa
 #pragma unroll
           for (int t = 0; t < 16; ++t) ds[t] = j0 + tile_row(t, g) < my_end ? ds[t] : 0.0f;
         }
+        range.fit(ds, dq);
         mm_transposed<T, D, NT>(dq, buf + kt_at, ds);
       }
       if (more) {
@@ -740,14 +787,14 @@ __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_wa
   if (r >= R) return;
   if (map == 1 && g == 0) a.dots[(2LL * a.batch * a.kv_heads + base) * R + r] = dot;
   T* out = reinterpret_cast<T*>(a.dq) + ((((long long)b * a.nq + query) * a.heads + head) * 2 + map) * a.d;
-  const float f = a.scale * cf;
+  const float f = a.scale * cf, back = 1.0f / range.factor;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dq[t][4 * u + e] * f;
+      for (int e = 0; e < 4; ++e) x[e] = dq[t][4 * u + e] * back * f;
       store4<T, VEC>(out, 32 * t + 8 * u + 4 * g, a.d, x);
     }
 }

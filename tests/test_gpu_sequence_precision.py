@@ -23,7 +23,7 @@ def _inputs(dtype, b, nq, nk, h, hk, d, dv):
 SHAPES = [(2, 150, 150, 2, 1, 32, 64, [150, 97], None), (1, 200, 200, 4, 2, 64, 128, None, "start"), (2, 70, 260, 2, 2, 128, 256, [260, 131], "end"),
           (1, 90, 1100, 1, 1, 20, 36, None, None), (3, 1, 600, 8, 2, 64, 128, [600, 0, 333], "end"), (1, 64, 2048, 1, 1, 32, 64, None, None),
           (1, 700, 90, 2, 1, 64, 128, None, "start")]
-CASES = [(t, s) for s in SHAPES for t in (torch.bfloat16, torch.float16) if t == torch.bfloat16 or s[2] < 2048]
+CASES = [(t, s) for s in SHAPES for t in (torch.bfloat16, torch.float16)]
 
 
 @pytest.mark.parametrize("dtype,shape", CASES, ids=lambda x: str(x)[6:] if isinstance(x, torch.dtype) else "-".join(str(i) for i in x[:7]) + f"-{x[8]}")
@@ -41,9 +41,57 @@ def test_only_the_results_are_rounded(cuda_device, dtype, shape):
         value, bound = want[name.split()[0]]
         off = (t.detach().cpu().double() - value).abs()
         assert bool((off <= bound).all()), f"{name}: {float((off / bound.clamp(min=1e-300)).max()):.2f} x its bound"
-        if t.numel() >= 1000:
-            # the norm of the error against that of rounding the 64-bit value.  A 32-bit score of d = 128 products is off by 1.2e-4 / sqrt(d) =
-            # 1.1e-5 (f of the oracle, with random signs), a result by the like of it, dS by three such (P, dP, D); rounding to fp16 alone is
-            # 2.1e-4 of the norm: sqrt(1 + 3 (1.1e-5 / 2.1e-4)^2) = 1.004
-            alone = (value.to(dtype).double() - value).norm()
-            assert off.norm() <= 1.01 * alone, f"{name}: {float(off.norm() / alone):.3f} x the error of rounding alone"
+        _like_rounding(t, value, name)
+
+
+def _like_rounding(t, value, name):
+    """the norm of the error against that of rounding the 64-bit value.  A 32-bit score of d = 128 products is off by 1.2e-4 / sqrt(d) = 1.1e-5 (f of the
+    oracle, with random signs), a result by the like of it, dS by three such (P, dP, D); rounding to fp16 alone is 2.1e-4 of the norm:
+    sqrt(1 + 3 (1.1e-5 / 2.1e-4)^2) = 1.004"""
+    if t.numel() >= 1000:
+        off, alone = (t.detach().cpu().double() - value).norm(), (value.to(t.dtype).double() - value).norm()
+        assert off <= 1.01 * alone, f"{name}: {float(off / alone):.3f} x the error of rounding alone"
+
+
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1.0, 1e3])
+@pytest.mark.parametrize("spread", [1.0, 0.01], ids=["scores", "equal weights"])
+@pytest.mark.parametrize("nq,nk,h,hk,d,causal", [(256, 4096, 2, 1, 64, None), (1500, 1500, 1, 1, 32, "start"), (70, 3000, 1, 1, 128, "end")])
+def test_half_gradients_of_any_size(cuda_device, size, spread, nq, nk, h, hk, d, causal):
+    """weights over thousands of keys and the score gradients of small (and large) upstream gradients lie outside fp16's range, the gradients that
+    they are summed to do not"""
+    q, k, v, lam, do = _inputs(torch.float16, 1, nq, nk, h, hk, d, 2 * d)
+    q, do = (q.float() * spread).half(), (do.float() * size).half()
+    want = SR.differential_attention(q, k, v, lam, None, causal, d ** -0.5, do, full=True)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    out = HF.differential_attention(*leaves, causal=causal)
+    _like_rounding(out, want["o"][0], "o")
+    for name, t in zip(("dq", "dk", "dv", "dlam"), torch.autograd.grad(out, leaves, do)):
+        _like_rounding(t, want[name][0], name)
+
+
+@pytest.mark.parametrize("lam", [0.0, -0.25, 3.0, 900.0])
+def test_half_weights_of_the_second_map(cuda_device, lam):
+    """lam of any size is part of the weights that dV is summed from"""
+    q, k, v, _, do = _inputs(torch.float16, 1, 100, 1200, 1, 1, 32, 64)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, torch.tensor([lam], device="cuda"))]
+    want = SR.differential_attention(*leaves, None, None, 32 ** -0.5, do, full=True)
+    out = HF.differential_attention(*leaves)
+    for name, t in zip(("o", "dq", "dk", "dv"), (out,) + torch.autograd.grad(out, leaves, do)):
+        _like_rounding(t, want[name][0], name)
+
+
+def test_half_weights_far_below_the_largest(cuda_device):
+    """one key of weight 1 with a value of 0 and 3999 of weight 2^-26 each with a value of 100: 0.006, not 0.  A weight may be off by 2^-36 (half a step
+    below fp16's normal range is 2^-25, the largest weight at 2^11 or above): 2^-10 of its own, so is their sum; the result's rounding adds 2^-11"""
+    b, nq, nk, d = 64, 40, 4000, 16      # (enough rows that no keys are split: all weights are relative to the one)
+    q = torch.zeros(b, nq, 4, d, dtype=torch.float16, device="cuda")
+    k = torch.zeros(b, nk, 4, d, dtype=torch.float16, device="cuda")
+    q[..., 0], k[:, 17, :, 0] = 2.0, 13.0      # scores 26 and 0, in powers of 2 by the scale
+    v = torch.full((b, nk, 2, 32), 100.0, dtype=torch.float16, device="cuda")
+    v[:, 17] = 0.0
+    lam = torch.tensor([0.0, 0.5], dtype=torch.float16, device="cuda")
+    out = HF.differential_attention(q, k, v, lam, scale=0.6931471805599453).double()
+    tail = 3999 * 2.0 ** -26
+    for h in range(2):
+        want = (1.0 - float(lam[h])) * 100.0 * tail / (1.0 + tail)
+        assert float((out[:, :, h] - want).abs().max()) <= 3.1 * 2.0 ** -11 * want
