@@ -5,8 +5,10 @@
 // torch, fill in the C ABI's argument structures, launch on the current stream, keep what the backward needs; kernels and their rules
 // are behind the C ABI (include/immunostruct_hip.h), whose entry points are handed over at import (bind) so that one library serves both.
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/immunostruct_hip.h"
@@ -54,6 +56,16 @@ Tensor aligned(const Tensor& t) {
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the sequence operators are differentiable once: no create_graph=True"); }
+
+// What would drop these calls without a word: a tangent of a forward-mode derivative (known to the operators' autograd nodes only, which a call without
+// gradients has none of), and the recorders of torch.jit.trace and make_fx, which see the output's allocation and not the launch.
+void direct(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "the sequence operators have no forward-mode derivatives");
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                              "the sequence operators cannot be traced");
+}
 
 // A leaf whose gradient node an eager graph on another stream keeps alive cannot be differentiated in a capture: the engine would make that stream wait
 // for the captured one, which ends the capture and with it the process.  Refused while nothing is captured yet.
@@ -120,6 +132,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 
 std::pair<Tensor, OptTensor> rotary(const Tensor& q, const OptTensor& k_, const Tensor& freq, const OptTensor& positions_, bool interleaved, double amplitude) {
   const Tensor k = value(k_), positions = value(positions_);
+  direct({&q, &k});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k))) {
     capturable({&q, &k});
     variable_list out = Rotary::apply(q, k_, positions_, freq, interleaved, amplitude);
@@ -208,6 +221,7 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
 };
 
 Tensor differential_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptTensor& lengths, int64_t causal, double scale) {
+  direct({&q, &k, &v, &lam});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v) || wanted(lam))) {
     capturable({&q, &k, &v, &lam});
     return DiffAttention::apply(q, k, v, lam, lengths, causal, scale);
@@ -274,6 +288,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 Tensor group_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, const OptTensor& lengths_, int64_t groups, double eps, int64_t activation) {
   const Tensor weight = value(weight_), bias = value(bias_), lengths = value(lengths_);
+  direct({&x, &weight, &bias});
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight) || wanted(bias))) {
     capturable({&x, &weight, &bias});
     return GroupNorm::apply(x, weight_, bias_, lengths_, groups, eps, activation);
