@@ -4,9 +4,11 @@
 //   dz = dy act'(z),  dw = sum dz xhat,  db = sum dz,  t = dz w,  dx = rstd (t - mean(t) - xhat mean(t xhat))
 //
 // Bound by bytes: x in and y out; x, dy in and dx out.  Forms, chosen by size (plan()):
-//   rows  n = 1, a group is a power of two of 16-byte chunks, at most 64: a group lives in neighbouring lanes, every sum is a few lane moves,
+//   rows  n = 1, a group has at most 64 chunks: a group lives in neighbouring lanes, every sum is a few lane moves,
 //         a workgroup walks many samples and keeps its channels' dw / db sums in registers
 //         ((24320, 1, 512) bf16, 8 groups: 19 us forward, 28 + 6 backward = 2.6 / 2.7 TB/s, launch and drain included).
+//         A group of any other width goes into neighbouring lanes too, whole groups to a wave ((20000, 1, 768) bf16, 32 groups of 24 channels: 24 us forward,
+//         51 a backward call; as slabs of a sample a workgroup, with a record of dw / db each, 104 and 185).
 //   wide  n = 1, groups of more chunks than a wave has lanes, 1024 at most: a workgroup per group, likewise over many samples
 //         ((8192, 1, 4096) bf16, one group: 43 us forward, 92 backward; as row blocks 174 and 379).
 //   slab  a workgroup holds all rows of one sample's slice of whole groups in registers (up to 16 chunks a thread): one read, exact two-step
@@ -19,7 +21,8 @@
 //         Groups of more than 256 chunks are cut into parts, which join like row blocks ((4, 2048, 4096) bf16, one group: 50 us forward, 94
 //         backward; a workgroup per sample and group that re-reads took 26 and 19 ms).
 // Chunks are 16 bytes where pointers, strides and the group width allow, single elements otherwise (a chunk never straddles two groups).
-// dw and db: one record [2][channels] per workgroup (rows, wide), sample (slab) or row block (long), summed in a fixed order by a last launch.
+// dw and db: one record [2][channels] per workgroup (long: per row block where a sample has several), summed in a fixed order by a last launch.  Where there
+// are more samples than the chip holds workgroups, a workgroup walks many.
 #include "../../include/immunostruct_hip.h"
 #include "tiles16.h"
 
@@ -36,6 +39,7 @@ struct Plan {
   int blocks, rows;    // long: row blocks of a sample, rows of one; rows, wide: workgroups
   int parts;           // long: slices of a group (more than one: a slice is at most a group's part, the last one may be narrower)
   int records;         // of dw / db
+  bool pow2;           // rows: groups of a power of two of 16-byte chunks
 };
 
 __device__ __forceinline__ int length_of(const Args& a, int b) {
@@ -144,13 +148,30 @@ __device__ __forceinline__ void channel_record(const float (&sw)[VE], const floa
 }
 
 // ---- rows: n = 1 ---------------------------------------------------------------------------------------------------------------------
-template <typename T, bool BACK>
+// POW2: cols chunk columns side by side (a group of a power of two of chunks never straddles a wave), sums by exchange.  Otherwise a wave holds as many whole
+// groups as fit its lanes, the rest of them idle; cols is the number of group columns, sums go down a tree to the group's first lane and back.
+template <typename T, int VE, bool POW2, bool BACK>
 __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, const int cols) {
-  constexpr int VE = Vec<T>::N;
   __shared__ float lds[BACK ? 256 * VE : 1];
-  const int lanes = 256 / cols, rl = threadIdx.x / cols, cl = threadIdx.x - rl * cols;
-  const int c = (blockIdx.y * cols + cl) * VE, cg = cpg * VE;
-  const bool on = rl < lanes && c < a.channels;
+  const int lane = threadIdx.x & 63, cg = cpg * VE;
+  int lanes, rl, cl, pos;      // rows side by side, this thread's row, its chunk column, its place in the group
+  bool there;                  // part of the layout
+  if constexpr (POW2) {
+    lanes = 256 / cols;
+    rl = threadIdx.x / cols;
+    cl = threadIdx.x - rl * cols;
+    pos = cl & (cpg - 1);
+    there = rl < lanes;
+  } else {
+    const int whole = 64 / cpg, slot = lane / cpg, at = (threadIdx.x >> 6) * whole + slot;
+    pos = lane - slot * cpg;
+    lanes = 4 * whole / cols;
+    rl = at / cols;
+    cl = (at - rl * cols) * cpg + pos;
+    there = slot < whole && rl < lanes;
+  }
+  const int width = (POW2 ? cols : cols * cpg) * VE, c = blockIdx.y * width + cl * VE;
+  const bool on = there && c < a.channels;
   const int cc = on ? c : 0, g = cc / cg;
   float w[VE], o[VE], sw[VE], sb[VE];
 #pragma unroll
@@ -160,9 +181,19 @@ __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, 
     sw[e] = sb[e] = 0.0f;
   }
   const float inv = 1.0f / (float)cg;
-  auto sum = [&](float v) {      // over the group's cpg neighbouring lanes (cpg divides 64 and the lanes of a group never straddle a wave)
-    for (int m = 1; m < cpg; m *= 2) v += __shfl_xor(v, m);
-    return v;
+  int half = 1;
+  while (2 * half < cpg) half *= 2;
+  auto sum = [&](float v) {      // over the group's cpg neighbouring lanes
+    if constexpr (POW2) {
+      for (int m = 1; m < cpg; m *= 2) v += __shfl_xor(v, m);
+      return v;
+    } else {
+      for (int m = half; m > 0; m /= 2) {
+        const float other = __shfl_down(v, m);
+        v += pos + m < cpg ? other : 0.0f;
+      }
+      return __shfl(v, lane - pos);
+    }
   };
   const int step = gridDim.x * lanes;
   for (int b0 = blockIdx.x * lanes; b0 < a.batch; b0 += step) {      // uniform: every lane takes part in the lane moves
@@ -188,7 +219,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, 
 #pragma unroll
         for (int e = 0; e < VE; ++e) x.x[e] = live ? act((x.x[e] - mean) * rstd * w[e] + o[e], a.activation) : 0.0f;
         x.store(reinterpret_cast<T*>(a.y) + (long long)b * a.channels + c);
-        if (cl % cpg == 0) {
+        if (pos == 0) {
           float* st = a.stats + 2 * ((long long)b * a.groups + g);
           st[0] = mean;
           st[1] = rstd;
@@ -224,12 +255,12 @@ __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, 
   }
   if constexpr (BACK) {
     if (a.weight != nullptr) {
-      const int width = cols * VE, c0 = blockIdx.y * width;
+      const int c0 = blockIdx.y * width;
       float* record = a.work + (long long)blockIdx.x * 2 * a.channels;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         __syncthreads();
-        if (rl < lanes) {
+        if (there) {
 #pragma unroll
           for (int e = 0; e < VE; ++e) lds[rl * width + cl * VE + e] = m == 0 ? sw[e] : sb[e];
         }
@@ -415,84 +446,95 @@ __global__ __launch_bounds__(256) void slab_fwd_kernel(const Args a, const int s
   }
 }
 
-template <typename T, int VE, int K>
+// WALK: a workgroup walks the samples blockIdx.x / slices, + gridDim.x / slices, ...; without it there is one for every sample
+template <typename T, int VE, int K, bool WALK>
 __global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int slice) {
   __shared__ float all[256], out[256], lds[256 * VE];
-  const int slices = a.channels / slice, b = blockIdx.x / slices, c0 = (blockIdx.x - b * slices) * slice, cg = a.channels / a.groups;
-  const int len = length_of(a, b), cpg = cg / VE;
+  const int slices = a.channels / slice, b0 = blockIdx.x / slices, step = gridDim.x / slices, c0 = (blockIdx.x - b0 * slices) * slice, cg = a.channels / a.groups;
+  const int cpg = cg / VE;
   const Place p(slice, VE, slice);
   const int c = c0 + p.col * VE;
-  const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + c;
-  const long long at = (long long)b * a.n * a.channels + c;
-  const T* dy = reinterpret_cast<const T*>(a.dy) + at;
-  T* dx = reinterpret_cast<T*>(a.dx) + at;
-  Held<T, VE> h[K], d[K];
+  float tw[VE], tb[VE];      // over the workgroup's samples
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int row = p.rl + k * p.lanes;
-    h[k].zero();
-    d[k].zero();
-    if (p.on && row < len) {
-      h[k].load(x + row * a.x_n);
-      d[k].load(dy + (long long)row * a.channels);
-    }
-  }
-  float w[VE], o[VE], sw[VE], sb[VE], v[VE], u[VE];
-  float mean = 0.0f, rstd = 0.0f;
-  if (p.on) {
-    const float* st = a.stats + 2 * ((long long)b * a.groups + c / cg);
-    mean = st[0];
-    rstd = st[1];
-  }
-#pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    w[e] = p.on ? param<T>(a, a.weight, c + e, 1.0f) : 0.0f;
-    o[e] = p.on ? param<T>(a, a.bias, c + e, 0.0f) : 0.0f;
-    sw[e] = sb[e] = 0.0f;
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    if (p.rl + k * p.lanes < len) {
-      h[k].get(v);
-      d[k].get(u);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float hat = (v[e] - mean) * rstd, dz = u[e] * act_slope(hat * w[e] + o[e], a.activation);
-        sw[e] += dz * hat;
-        sb[e] += dz;
-      }
-    }
-  float t1 = 0.0f, t2 = 0.0f;
-#pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    t1 += sb[e] * w[e];
-    t2 += sw[e] * w[e];
-  }
-  const float inv = 1.0f / ((float)(len > 0 ? len : 1) * (float)cg);
-  t1 = group_sum(t1, p, cpg, all, out) * inv;
-  t2 = group_sum(t2, p, cpg, all, out) * inv;
-  if (p.on) {
+  for (int e = 0; e < VE; ++e) tw[e] = tb[e] = 0.0f;
+  for (int b = b0; b < a.batch; b += step) {      // (uniform: every barrier is met)
+    const int len = length_of(a, b);
+    const T* x = reinterpret_cast<const T*>(a.x) + b * a.x_b + c;
+    const long long at = (long long)b * a.n * a.channels + c;
+    const T* dy = reinterpret_cast<const T*>(a.dy) + at;
+    T* dx = reinterpret_cast<T*>(a.dx) + at;
+    Held<T, VE> h[K], d[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int row = p.rl + k * p.lanes;
-      if (row < a.n) {
-        Chunk<T, VE> r;
+      h[k].zero();
+      d[k].zero();
+      if (p.on && row < len) {
+        h[k].load(x + row * a.x_n);
+        d[k].load(dy + (long long)row * a.channels);
+      }
+    }
+    float w[VE], o[VE], sw[VE], sb[VE], v[VE], u[VE];
+    float mean = 0.0f, rstd = 0.0f;
+    if (p.on) {
+      const float* st = a.stats + 2 * ((long long)b * a.groups + c / cg);
+      mean = st[0];
+      rstd = st[1];
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      w[e] = p.on ? param<T>(a, a.weight, c + e, 1.0f) : 0.0f;
+      o[e] = p.on ? param<T>(a, a.bias, c + e, 0.0f) : 0.0f;
+      sw[e] = sb[e] = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (p.rl + k * p.lanes < len) {
         h[k].get(v);
         d[k].get(u);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const float hat = (v[e] - mean) * rstd, dz = u[e] * act_slope(hat * w[e] + o[e], a.activation);
-          r.x[e] = row < len ? rstd * (dz * w[e] - t1 - hat * t2) : 0.0f;
+          sw[e] += dz * hat;
+          sb[e] += dz;
         }
-        r.store(dx + (long long)row * a.channels);
+      }
+    float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      t1 += sb[e] * w[e];
+      t2 += sw[e] * w[e];
+      tw[e] += sw[e];
+      tb[e] += sb[e];
+    }
+    const float inv = 1.0f / ((float)(len > 0 ? len : 1) * (float)cg);
+    t1 = group_sum(t1, p, cpg, all, out) * inv;
+    t2 = group_sum(t2, p, cpg, all, out) * inv;
+    if (p.on) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int row = p.rl + k * p.lanes;
+        if (row < a.n) {
+          Chunk<T, VE> r;
+          h[k].get(v);
+          d[k].get(u);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float hat = (v[e] - mean) * rstd, dz = u[e] * act_slope(hat * w[e] + o[e], a.activation);
+            r.x[e] = row < len ? rstd * (dz * w[e] - t1 - hat * t2) : 0.0f;
+          }
+          r.store(dx + (long long)row * a.channels);
+        }
       }
     }
+    if constexpr (!WALK) break;
   }
-  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + (long long)b * 2 * a.channels, a.channels, c0, slice);
+  if (a.weight != nullptr) channel_record<VE>(tw, tb, p, lds, a.work + (long long)b0 * 2 * a.channels, a.channels, c0, slice);
 }
 
 // ---- long: row blocks ---------------------------------------------------------------------------------------------------------------------
-// workspace: pairs[sample][group][block][part][2], joined[sample][group][2], then the dw / db records.  Workgroup = (sample, block, slice)
+// workspace: pairs[sample][group][block][part][2], joined[sample][group][2], then the dw / db records.  Workgroup = (sample, block, slice); the
+// backward's first pass walks every records / blocks-th sample where there are many, so that the records stay few
 struct Block {
   int b, block, part, c0, width, first, last, len;
   __device__ __forceinline__ Block(const Args& a, const Plan& p) {
@@ -504,9 +546,12 @@ struct Block {
     width = p.parts == 1 ? p.slice : min(p.slice, cg - part * p.slice);
     id /= slices;
     block = id % p.blocks;
-    b = id / p.blocks;
-    len = length_of(a, b);
     first = block * p.rows;
+    at(a, p, id / p.blocks);
+  }
+  __device__ __forceinline__ void at(const Args& a, const Plan& p, int sample) {
+    b = sample;
+    len = sample < a.batch ? length_of(a, sample) : 0;
     last = min(first + p.rows, len);
   }
 };
@@ -656,55 +701,63 @@ __global__ __launch_bounds__(256) void long_apply_kernel(const Args a, const Pla
   });
 }
 
-template <typename T, int VE>
+template <typename T, int VE, bool WALK>
 __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan plan) {
   __shared__ float all[256], out[256], lds[256 * VE];
-  const Block k(a, plan);
+  Block k(a, plan);
   const int cg = a.channels / a.groups, cpg = (plan.parts == 1 ? cg : plan.slice) / VE;
   const Place p(plan.slice, VE, k.width);
-  const int c = k.c0 + p.col * VE;
-  float w[VE], o[VE], sw[VE], sb[VE];
+  const int c = k.c0 + p.col * VE, step = plan.records / plan.blocks;
+  const long long pairs = 2LL * a.batch * (plan.blocks * plan.parts + 1) * a.groups, index = (long long)k.b * plan.blocks + k.block;
+  float w[VE], o[VE], tw[VE], tb[VE];      // tw, tb: over the workgroup's samples
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
     w[e] = p.on ? param<T>(a, a.weight, c + e, 1.0f) : 0.0f;
     o[e] = p.on ? param<T>(a, a.bias, c + e, 0.0f) : 0.0f;
-    sw[e] = sb[e] = 0.0f;
+    tw[e] = tb[e] = 0.0f;
   }
-  if (p.on) {
-    const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
-    const float mean = st[0], rstd = st[1];
-    const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
-    const T* dy = reinterpret_cast<const T*>(a.dy) + (long long)k.b * a.n * a.channels + c;
-    batches<Pair<T, VE>>(k.first + p.rl, k.last, p.lanes, [&](int row, Pair<T, VE>& h) {
-      h.x.load(x + row * a.x_n);
-      h.d.load(dy + (long long)row * a.channels);
-    }, [&](int, const Pair<T, VE>& h) {
-      float v[VE], d[VE];
-      h.x.get(v);
-      h.d.get(d);
+  for (; k.b < a.batch; k.at(a, plan, k.b + step)) {      // (uniform: every barrier is met)
+    float sw[VE], sb[VE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float hat = (v[e] - mean) * rstd, dz = d[e] * act_slope(hat * w[e] + o[e], a.activation);
-        sw[e] += dz * hat;
-        sb[e] += dz;
-      }
-    });
-  }
-  float t1 = 0.0f, t2 = 0.0f;
+    for (int e = 0; e < VE; ++e) sw[e] = sb[e] = 0.0f;
+    if (p.on) {
+      const float* st = a.stats + 2 * ((long long)k.b * a.groups + c / cg);
+      const float mean = st[0], rstd = st[1];
+      const T* x = reinterpret_cast<const T*>(a.x) + k.b * a.x_b + c;
+      const T* dy = reinterpret_cast<const T*>(a.dy) + (long long)k.b * a.n * a.channels + c;
+      batches<Pair<T, VE>>(k.first + p.rl, k.last, p.lanes, [&](int row, Pair<T, VE>& h) {
+        h.x.load(x + row * a.x_n);
+        h.d.load(dy + (long long)row * a.channels);
+      }, [&](int, const Pair<T, VE>& h) {
+        float v[VE], d[VE];
+        h.x.get(v);
+        h.d.get(d);
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    t1 += sb[e] * w[e];
-    t2 += sw[e] * w[e];
+        for (int e = 0; e < VE; ++e) {
+          const float hat = (v[e] - mean) * rstd, dz = d[e] * act_slope(hat * w[e] + o[e], a.activation);
+          sw[e] += dz * hat;
+          sb[e] += dz;
+        }
+      });
+    }
+    float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      t1 += sb[e] * w[e];
+      t2 += sw[e] * w[e];
+      tw[e] += sw[e];
+      tb[e] += sb[e];
+    }
+    t1 = group_sum(t1, p, cpg, all, out);
+    t2 = group_sum(t2, p, cpg, all, out);
+    if (p.on && p.rl == 0 && p.col % cpg == 0) {
+      float* at = pair_at(a, plan, k, c / cg);
+      at[0] = t1;
+      at[1] = t2;
+    }
+    if constexpr (!WALK) break;
   }
-  t1 = group_sum(t1, p, cpg, all, out);
-  t2 = group_sum(t2, p, cpg, all, out);
-  const long long pairs = 2LL * a.batch * (plan.blocks * plan.parts + 1) * a.groups, index = (long long)k.b * plan.blocks + k.block;
-  if (p.on && p.rl == 0 && p.col % cpg == 0) {
-    float* at = pair_at(a, plan, k, c / cg);
-    at[0] = t1;
-    at[1] = t2;
-  }
-  if (a.weight != nullptr) channel_record<VE>(sw, sb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0, k.width);
+  if (a.weight != nullptr) channel_record<VE>(tw, tb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0, k.width);
 }
 
 template <typename T, int VE>
@@ -781,6 +834,16 @@ bool sizes_ok(const Args& a) {
          (long long)a.batch * a.groups <= 0x3fffffffLL && a.type >= TYPE_F32 && a.type <= TYPE_F16;
 }
 
+// Samples that a backward pass works on at a time, each workgroup walking its share of them: bounds the records of dw and db (8 bytes a channel each).
+// 2048 workgroups, 8 a CU, are as many as the chip holds.  The long form walks from there on: (8192, 2, 4112) bf16, 2 groups 313 us instead of 507 with a record
+// a sample, (2500, 3000, 64), 8 groups 958 for 965.  The slab form's loop costs registers ((8192, 17, 512), 8 groups 344 for 240): it walks only beyond 64 MB
+// of records, and with 32 rows or more, where they are at most 1 / 8 of x in 16 bits, not at all.
+int walkers(const Args& a, int slices, bool slab) {
+  long long most = 2048 / slices > 1 ? 2048 / slices : 1;
+  if (slab) most = a.n >= 32 ? a.batch : most > (1 << 23) / a.channels ? most : (1 << 23) / a.channels;
+  return (int)(a.batch < most ? a.batch : most);
+}
+
 // The form of a call, by sizes and alignment alone (dy, y and dx are contiguous; their pointers do not enter: x's alignment decides, and the
 // library's callers allocate theirs 16-byte aligned -- checked in run()).
 Plan plan(const Args& a) {
@@ -789,17 +852,18 @@ Plan plan(const Args& a) {
   const bool chunks = (a.x_b | a.x_n) % full == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && cg % full == 0;
   p.ve = chunks ? full : 1;
   const int cpg = cg / p.ve;
-  if (a.n == 1 && chunks && cpg <= 64 && (cpg & (cpg - 1)) == 0) {
+  if (a.n == 1 && cpg <= 64) {
     p.form = ROWS;
-    const int lanes_of = a.channels / p.ve < 256 ? a.channels / p.ve : 256;
-    const int per_pass = 256 / lanes_of, columns = (a.channels / p.ve + lanes_of - 1) / lanes_of;
+    p.pow2 = chunks && (cpg & (cpg - 1)) == 0;
+    const int whole = 4 * (64 / cpg), all = p.pow2 ? a.channels / p.ve : a.groups, side = p.pow2 ? 256 : whole;      // columns: chunks or groups
+    const int lanes_of = all < side ? all : side, per_pass = side / lanes_of, columns = (all + lanes_of - 1) / lanes_of;
     const long long passes = ((long long)a.batch + per_pass - 1) / per_pass;
     const long long most = 2048 / columns > 1 ? 2048 / columns : 1;      // 8 workgroups a CU
     p.blocks = (int)(passes < most ? passes : most);
     p.slice = lanes_of;
     p.slices = columns;
     p.records = p.blocks;
-    return p;
+    if (columns <= 32768) return p;      // (the grid's second dimension)
   }
   if (a.n == 1 && cpg > 64 && cpg <= 1024 && a.groups <= 32768) {      // (groups: the grid's second dimension)
     p.form = WIDE;
@@ -830,7 +894,7 @@ Plan plan(const Args& a) {
     p.slices = a.groups / gs;
     p.form = SLAB;
     p.per_thread = need <= 1 ? 1 : need <= 4 ? 4 : 16;
-    p.records = a.batch;
+    p.records = walkers(a, p.slices, true);
     return p;
   }
   p.form = LONG;
@@ -844,7 +908,7 @@ Plan plan(const Args& a) {
   const int blocks = (int)(want < most ? want : most);
   p.rows = (a.n + blocks - 1) / blocks;
   p.blocks = (a.n + p.rows - 1) / p.rows;
-  p.records = a.batch * p.blocks;
+  p.records = (p.blocks > 1 ? a.batch : walkers(a, p.slices, false)) * p.blocks;      // (row blocks: a batch of fewer than 1024 workgroups)
   return p;
 }
 
@@ -855,16 +919,28 @@ long long work_floats(const Args& a, const Plan& p, bool backward) {
 
 template <typename T, int VE>
 void launch_slab(const Args& a, const Plan& p, bool backward, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)a.batch * p.slices);
-  if (backward) {
-    if (p.per_thread == 1) slab_bwd_kernel<T, VE, 1><<<grid, 256, 0, st>>>(a, p.slice);
-    else if (p.per_thread == 4) slab_bwd_kernel<T, VE, 4><<<grid, 256, 0, st>>>(a, p.slice);
-    else slab_bwd_kernel<T, VE, 16><<<grid, 256, 0, st>>>(a, p.slice);
+  const unsigned grid = (unsigned)((long long)a.batch * p.slices), walking = (unsigned)(p.records * p.slices);
+  if (backward && p.records < a.batch) {
+    if (p.per_thread == 1) slab_bwd_kernel<T, VE, 1, true><<<walking, 256, 0, st>>>(a, p.slice);
+    else if (p.per_thread == 4) slab_bwd_kernel<T, VE, 4, true><<<walking, 256, 0, st>>>(a, p.slice);
+    else slab_bwd_kernel<T, VE, 16, true><<<walking, 256, 0, st>>>(a, p.slice);
+  } else if (backward) {
+    if (p.per_thread == 1) slab_bwd_kernel<T, VE, 1, false><<<grid, 256, 0, st>>>(a, p.slice);
+    else if (p.per_thread == 4) slab_bwd_kernel<T, VE, 4, false><<<grid, 256, 0, st>>>(a, p.slice);
+    else slab_bwd_kernel<T, VE, 16, false><<<grid, 256, 0, st>>>(a, p.slice);
   } else {
     if (p.per_thread == 1) slab_fwd_kernel<T, VE, 1><<<grid, 256, 0, st>>>(a, p.slice);
     else if (p.per_thread == 4) slab_fwd_kernel<T, VE, 4><<<grid, 256, 0, st>>>(a, p.slice);
     else slab_fwd_kernel<T, VE, 16><<<grid, 256, 0, st>>>(a, p.slice);
   }
+}
+
+template <typename T, int VE, bool POW2>
+void launch_rows(const Args& a, const Plan& p, bool backward, hipStream_t st) {
+  const int cpg = a.channels / a.groups / VE;
+  const dim3 grid(p.blocks, p.slices);
+  if (backward) rows_kernel<T, VE, POW2, true><<<grid, 256, 0, st>>>(a, cpg, p.slice);
+  else rows_kernel<T, VE, POW2, false><<<grid, 256, 0, st>>>(a, cpg, p.slice);
 }
 
 template <typename T, int VE, int K>
@@ -884,7 +960,8 @@ template <typename T, int VE>
 void launch_long(const Args& a, const Plan& p, bool backward, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)a.batch * p.blocks * p.slices), join = (unsigned)(((long long)a.batch * a.groups + 3) / 4);
   if (backward) {
-    long_sum_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
+    if (p.records < a.batch) long_sum_kernel<T, VE, true><<<(unsigned)((long long)p.records * p.slices), 256, 0, st>>>(a, p);
+    else long_sum_kernel<T, VE, false><<<grid, 256, 0, st>>>(a, p);
     long_join_kernel<true><<<join, 256, 0, st>>>(a, p);
     long_dx_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
   } else {
@@ -898,10 +975,9 @@ template <typename T>
 void launch(const Args& a, const Plan& p, bool backward, hipStream_t st) {
   constexpr int N = Vec<T>::N;
   if (p.form == ROWS) {
-    const int cpg = a.channels / a.groups / N;
-    const dim3 grid(p.blocks, p.slices);
-    if (backward) rows_kernel<T, true><<<grid, 256, 0, st>>>(a, cpg, p.slice);
-    else rows_kernel<T, false><<<grid, 256, 0, st>>>(a, cpg, p.slice);
+    if (p.pow2) launch_rows<T, N, true>(a, p, backward, st);
+    else if (p.ve > 1) launch_rows<T, N, false>(a, p, backward, st);
+    else launch_rows<T, 1, false>(a, p, backward, st);
   } else if (p.form == WIDE) {
     if (p.ve == 1) launch_wide<T, 1>(a, p, backward, st);
     else launch_wide<T, N>(a, p, backward, st);
