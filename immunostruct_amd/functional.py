@@ -12,6 +12,7 @@ import torch
 from . import _lib
 
 import ctypes
+import math
 import os
 
 HIDDEN = 64
@@ -1771,6 +1772,12 @@ def _sequence_type(name, *tensors):
             raise ValueError(f"{name}: tensors of different types {t} and {u.dtype}")
 
 
+def _check_sizes(name, *sizes):
+    """raises where a size does not fit the C ABI's 32-bit integers (a tensor may be a view of few elements, and its results still fit the card)"""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{name}: sizes have to be below 2^31")
+
+
 def _check_lengths(name, lengths, batch):
     if lengths is None:
         return None
@@ -1790,6 +1797,7 @@ def rotary(q, k, freq, positions=None, layout="half", amplitude=1.0):
     _sequence_type("rotary", q, k)
     if q.dim() != 4 or q.shape[2] < 1 or (k is not None and (k.dim() != 4 or k.shape[2] < 1 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise ValueError("rotary: expected q (B, n, heads, width) and k (B, n, kv_heads, width)")
+    _check_sizes("rotary", *q.shape, 0 if k is None else k.shape[2])
     if freq.is_cuda or freq.dtype != torch.float64 or freq.dim() != 1 or not 1 <= freq.numel() <= 256 or 2 * freq.numel() > q.shape[3]:
         raise ValueError("rotary: freq has to be a float64 host tensor of 1 ... min(256, width / 2) frequencies")
     if layout not in ("half", "interleaved"):
@@ -1823,6 +1831,7 @@ def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
     nk, hk, dv = v.shape[1:]
     if (min(h2, hk, d, dv) < 1 or h2 % 2 or (h2 // 2) % hk or tuple(k.shape) != (b, nk, 2 * hk, d) or v.shape[0] != b or lam.shape[0] != h2 // 2):
         raise ValueError(f"differential_attention: shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, lam {tuple(lam.shape)}")
+    _check_sizes("differential_attention", *q.shape, *k.shape)
     if lam.dtype not in (torch.float32, q.dtype):
         raise ValueError(f"differential_attention: lam has to be float32 or {q.dtype}")
     if causal not in _CAUSAL:
@@ -1851,6 +1860,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, len
     _sequence_type("group_norm", x)
     if x.dim() < 2 or groups < 1 or x.shape[-1] < 1 or x.shape[-1] % groups:
         raise ValueError(f"group_norm: expected x (B, ..., channels) with channels a multiple of {groups} groups, got {tuple(x.shape)}")
+    _check_sizes("group_norm", x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1])
     if activation not in _ACTIVATIONS:
         raise ValueError(f"group_norm: unknown activation {activation!r}")
     if (weight is None) != (bias is None):
