@@ -423,32 +423,33 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   constexpr int N = Vec<T>::N;
   const int R = a.rows, lane = threadIdx.x & 15;
-  const long long w = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (w >= (long long)a.batch * a.kv_heads * R) return;
-  const long long base = w / R;
-  const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
-  int gi;
-  const int query = query_of(a, r, gi), head = hk * a.group + gi;
-  const long long at = o_at(a, b, query, head);
-  const char* go = reinterpret_cast<const char*>(a.d_o) + at * sizeof(T);
-  const char* maps[2] = {reinterpret_cast<const char*>(a.maps + at), reinterpret_cast<const char*>(a.maps + maps_plane(a) + at)};
-  float s[2] = {0.0f, 0.0f};
-  for (int c = lane; c * N < a.dv; c += 16) {
-    float x[N], y[4];
-    Vec<T>::unpack(load_chunk<T, VEC>(go, c, a.dv), x);
+  const long long all = (long long)a.batch * a.kv_heads * R;
+  for (long long w = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); w < all; w += gridDim.x * 16LL) {
+    const long long base = w / R;
+    const int r = (int)(w - base * R), b = (int)base / a.kv_heads, hk = (int)base - b * a.kv_heads;
+    int gi;
+    const int query = query_of(a, r, gi), head = hk * a.group + gi;
+    const long long at = o_at(a, b, query, head);
+    const char* go = reinterpret_cast<const char*>(a.d_o) + at * sizeof(T);
+    const char* maps[2] = {reinterpret_cast<const char*>(a.maps + at), reinterpret_cast<const char*>(a.maps + maps_plane(a) + at)};
+    float s[2] = {0.0f, 0.0f};
+    for (int c = lane; c * N < a.dv; c += 16) {
+      float x[N], y[4];
+      Vec<T>::unpack(load_chunk<T, VEC>(go, c, a.dv), x);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int u = 0; u < N / 4; ++u) {
-        Vec<float>::unpack(load_chunk<float, VEC>(maps[m], c * (N / 4) + u, a.dv), y);
+        for (int u = 0; u < N / 4; ++u) {
+          Vec<float>::unpack(load_chunk<float, VEC>(maps[m], c * (N / 4) + u, a.dv), y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[m] += x[4 * u + e] * y[e];
-      }
-  }
+          for (int e = 0; e < 4; ++e) s[m] += x[4 * u + e] * y[e];
+        }
+    }
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    s[m] = sum_over_r16(s[m]);
-    if (lane == 0) a.dots[(base * 2 + m) * R + r] = s[m];
+    for (int m = 0; m < 2; ++m) {
+      s[m] = sum_over_r16(s[m]);
+      if (lane == 0) a.dots[(base * 2 + m) * R + r] = s[m];
+    }
   }
 }
 
@@ -819,7 +820,8 @@ template <typename T, int D, bool VEC>
 void launch_bwd(const Args& a, hipStream_t st) {
   const int heads = a.kv_heads * a.batch;
   constexpr int KEYS = 32 * key_groups<T, D>(), ROWS = 32 * dq_groups<T, D>();
-  rowdot_kernel<T, VEC><<<(unsigned)(((long long)heads * a.rows + 15) / 16), 256, 0, st>>>(a);
+  const long long sums = ((long long)heads * a.rows + 15) / 16;
+  rowdot_kernel<T, VEC><<<(unsigned)(sums < 1 << 23 ? sums : 1 << 23), 256, 0, st>>>(a);      // (a launch of 2^24 workgroups runs short of them)
   dkv_kernel<T, D, VEC><<<(a.nk + KEYS - 1) / KEYS * a.row_splits * heads, 4 * KEYS, 0, st>>>(a);
   if (a.row_splits > 1)
     key_join_kernel<T, VEC><<<(unsigned)(((long long)heads * a.nk * (2 * a.d + a.dv) / (VEC ? 4 : 1) + 255) / 256), 256, 0, st>>>(a);

@@ -17,8 +17,11 @@ int prepare(da::Args& a) {
   a.group_magic = 0xffffffffu / (unsigned)a.group;
   const long long rows = (long long)a.nq * a.group, big = 0x7fffff00LL;
   const int n = a.type == TYPE_F32 ? 4 : 8, size = 16 / n;
-  if (rows > big || a.nk > big || (rows / 32 + 1) * a.splits * a.kv_heads > big / a.batch || (rows + 3) * a.kv_heads > big / a.batch ||
-      (a.nk / 64 + 1LL) * a.row_splits * a.kv_heads > big / a.batch || (a.nk * (2LL * a.d + a.dv) + 255) / 256 * a.kv_heads > big / a.batch) return -22;
+  // a launch has to stay below 2^32 threads: 128 for 32 rows or keys, up to 256 for a row that is joined, one for an element of joined key gradients
+  const long long tiles = 0x1ffffffLL;
+  if (rows > big || a.nk > big || (rows / 32 + 4) * a.splits * a.kv_heads > tiles / a.batch || (rows + 3) * a.kv_heads > big / a.batch ||
+      (a.nk / 32 + 4LL) * a.row_splits * a.kv_heads > tiles / a.batch || (a.splits > 1 && (rows + 3) * a.kv_heads > tiles / 2 / a.batch) ||
+      (a.row_splits > 1 && (a.nk * (2LL * a.d + a.dv) + 255) / 256 * a.kv_heads > tiles / 2 / a.batch)) return -22;
   a.rows = (int)rows;
   // a tile's rows lie within 31 bits of its first
   const long long near = 0x7fffffffLL / size;

@@ -636,38 +636,39 @@ __global__ __launch_bounds__(256) void long_stat_kernel(const Args a, const Plan
 // one wave per (sample, group): forward -> mean and rstd; backward -> the means of t and t xhat
 template <bool BACK>
 __global__ __launch_bounds__(256) void long_join_kernel(const Args a, const Plan plan) {
-  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= (long long)a.batch * a.groups) return;
-  const int lane = threadIdx.x & 63, len = length_of(a, (int)(i / a.groups)), cg = a.channels / a.groups;
-  const int entries = plan.blocks * plan.parts;
-  const float2* at = reinterpret_cast<const float2*>(a.work) + i * entries;
-  const float total = (float)(len > 0 ? len : 1) * (float)cg;
-  auto count = [&](int n) {      // elements behind entry n
-    const int block = n / plan.parts, part = n - block * plan.parts, width = plan.parts == 1 ? cg : min(plan.slice, cg - part * plan.slice);
-    return (float)max(min((block + 1) * plan.rows, len) - block * plan.rows, 0) * (float)width;
-  };
-  float s0 = 0.0f, s1 = 0.0f;
-  for (int n = lane; n < entries; n += 64) {
-    const float2 x = at[n];
-    if constexpr (BACK) {
-      s0 += x.x;
-      s1 += x.y;
-    } else {
-      s0 += x.x * (count(n) / total);
-    }
-  }
-  s0 = wave_sum(s0);
-  if constexpr (BACK) {
-    s1 = wave_sum(s1);
-    if (lane == 0) reinterpret_cast<float2*>(a.work)[(long long)a.batch * a.groups * entries + i] = make_float2(s0 / total, s1 / total);
-  } else {
+  const int lane = threadIdx.x & 63, cg = a.channels / a.groups, entries = plan.blocks * plan.parts;
+  const long long all = (long long)a.batch * a.groups;
+  for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < all; i += gridDim.x * 4LL) {
+    const int len = length_of(a, (int)(i / a.groups));
+    const float2* at = reinterpret_cast<const float2*>(a.work) + i * entries;
+    const float total = (float)(len > 0 ? len : 1) * (float)cg;
+    auto count = [&](int n) {      // elements behind entry n
+      const int block = n / plan.parts, part = n - block * plan.parts, width = plan.parts == 1 ? cg : min(plan.slice, cg - part * plan.slice);
+      return (float)max(min((block + 1) * plan.rows, len) - block * plan.rows, 0) * (float)width;
+    };
+    float s0 = 0.0f, s1 = 0.0f;
     for (int n = lane; n < entries; n += 64) {
       const float2 x = at[n];
-      const float off = x.x - s0;
-      s1 += x.y + count(n) * off * off;
+      if constexpr (BACK) {
+        s0 += x.x;
+        s1 += x.y;
+      } else {
+        s0 += x.x * (count(n) / total);
+      }
     }
-    s1 = wave_sum(s1);
-    if (lane == 0) reinterpret_cast<float2*>(a.stats)[i] = make_float2(s0, 1.0f / sqrtf(s1 / total + a.eps));
+    s0 = wave_sum(s0);
+    if constexpr (BACK) {
+      s1 = wave_sum(s1);
+      if (lane == 0) reinterpret_cast<float2*>(a.work)[all * entries + i] = make_float2(s0 / total, s1 / total);
+    } else {
+      for (int n = lane; n < entries; n += 64) {
+        const float2 x = at[n];
+        const float off = x.x - s0;
+        s1 += x.y + count(n) * off * off;
+      }
+      s1 = wave_sum(s1);
+      if (lane == 0) reinterpret_cast<float2*>(a.stats)[i] = make_float2(s0, 1.0f / sqrtf(s1 / total + a.eps));
+    }
   }
 }
 
@@ -829,6 +830,8 @@ __global__ __launch_bounds__(1024) void param_grad_kernel(const Args a, const fl
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
+constexpr unsigned LAUNCH = 1u << 23;      // workgroups: a launch of 2^32 threads (2^24 workgroups) and more runs short of them without an error
+
 bool sizes_ok(const Args& a) {
   return a.batch >= 1 && a.n >= 1 && a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0 && a.channels <= (1 << 24) && a.n <= (1 << 30) &&
          (long long)a.batch * a.groups <= 0x3fffffffLL && a.type >= TYPE_F32 && a.type <= TYPE_F16;
@@ -917,9 +920,25 @@ long long work_floats(const Args& a, const Plan& p, bool backward) {
   return pairs + (backward && a.weight != nullptr ? 2LL * p.records * a.channels : 0);
 }
 
+// the samples [first, first + count) of a call (slab form)
+template <typename T>
+Args samples(Args a, int first, int count) {
+  const long long at = (long long)first * a.n * a.channels * (long long)sizeof(T);
+  auto shift = [&](const void* p, long long bytes) { return p != nullptr ? static_cast<const char*>(p) + bytes : nullptr; };
+  a.x = shift(a.x, first * a.x_b * (long long)sizeof(T));
+  a.y = const_cast<char*>(shift(a.y, at));
+  a.dy = shift(a.dy, at);
+  a.dx = const_cast<char*>(shift(a.dx, at));
+  a.stats += 2LL * first * a.groups;
+  if (a.lengths != nullptr) a.lengths += first;
+  if (a.work != nullptr) a.work += 2LL * first * a.channels;
+  a.batch = count;
+  return a;
+}
+
 template <typename T, int VE>
 void launch_slab(const Args& a, const Plan& p, bool backward, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)a.batch * p.slices), walking = (unsigned)(p.records * p.slices);
+  const unsigned grid = (unsigned)((long long)a.batch * p.slices), walking = (unsigned)((long long)p.records * p.slices);
   if (backward && p.records < a.batch) {
     if (p.per_thread == 1) slab_bwd_kernel<T, VE, 1, true><<<walking, 256, 0, st>>>(a, p.slice);
     else if (p.per_thread == 4) slab_bwd_kernel<T, VE, 4, true><<<walking, 256, 0, st>>>(a, p.slice);
@@ -958,7 +977,8 @@ void launch_wide(const Args& a, const Plan& p, bool backward, hipStream_t st) {
 
 template <typename T, int VE>
 void launch_long(const Args& a, const Plan& p, bool backward, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)a.batch * p.blocks * p.slices), join = (unsigned)(((long long)a.batch * a.groups + 3) / 4);
+  const unsigned grid = (unsigned)((long long)a.batch * p.blocks * p.slices), pairs = (unsigned)(((long long)a.batch * a.groups + 3) / 4);
+  const unsigned join = pairs < LAUNCH ? pairs : LAUNCH;
   if (backward) {
     if (p.records < a.batch) long_sum_kernel<T, VE, true><<<(unsigned)((long long)p.records * p.slices), 256, 0, st>>>(a, p);
     else long_sum_kernel<T, VE, false><<<grid, 256, 0, st>>>(a, p);
@@ -982,8 +1002,13 @@ void launch(const Args& a, const Plan& p, bool backward, hipStream_t st) {
     if (p.ve == 1) launch_wide<T, 1>(a, p, backward, st);
     else launch_wide<T, N>(a, p, backward, st);
   } else if (p.form == SLAB) {
-    if (p.ve == 1) launch_slab<T, 1>(a, p, backward, st);
-    else launch_slab<T, N>(a, p, backward, st);
+    const int most = backward && p.records < a.batch ? a.batch : (int)LAUNCH / p.slices > 1 ? (int)LAUNCH / p.slices : 1;
+    for (int first = 0; first < a.batch; first += most) {
+      const Args part = samples<T>(a, first, a.batch - first < most ? a.batch - first : most);
+      if (p.ve == 1) launch_slab<T, 1>(part, p, backward, st);
+      else launch_slab<T, N>(part, p, backward, st);
+      if (a.batch - first <= most) break;
+    }
   } else {
     if (p.ve == 1) launch_long<T, 1>(a, p, backward, st);
     else launch_long<T, N>(a, p, backward, st);
@@ -1006,8 +1031,8 @@ int run(const Args* args, bool backward, const char* entry, void* stream) {
   const uintptr_t own = backward ? reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx) : reinterpret_cast<uintptr_t>(a.y);
   if (p.ve > 1 && own % 16 != 0) return fail(entry, -22);
   if (a.work == nullptr && work_floats(a, p, backward) > 0) return fail(entry, -22);
-  // workgroups of one launch (rows and wide: at most a few thousand)
-  if ((p.form == SLAB || p.form == LONG) && (long long)a.batch * p.slices * (p.form == LONG ? p.blocks : 1) > 0x7fffffffLL) return fail(entry, -22);
+  // workgroups of one launch (rows and wide: at most a few thousand; slab: several launches)
+  if (p.form == LONG && (long long)a.batch * p.slices * p.blocks > 2LL * LAUNCH - 1) return fail(entry, -22);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.type == TYPE_F32) launch<float>(a, p, backward, st);
   else if (a.type == TYPE_BF16) launch<__bf16>(a, p, backward, st);

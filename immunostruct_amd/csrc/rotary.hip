@@ -140,7 +140,7 @@ extern "C" int is_rotary(const void* q, long long q_b, long long q_n, long long 
   tokens = tokens > most ? most : tokens;
   a.tokens = (int)tokens;
   const long long total = (long long)batch * n;
-  if ((total + tokens - 1) / tokens > 0x7fffffffLL || (heads + kv_heads) * (long long)width * tokens > 0x7fffffffLL) return fail("is_rotary", -22);
+  if ((total + tokens - 1) / tokens > 0xffffffLL || (heads + kv_heads) * (long long)width * tokens > 0x7fffffffLL) return fail("is_rotary", -22);
   const int N = type == TYPE_F32 ? 4 : 8;
   const long long strides = q_b | q_n | q_h | (kv_heads > 0 ? k_b | k_n | k_h : 0);
   const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) |
