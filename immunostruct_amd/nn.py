@@ -185,7 +185,7 @@ class RotaryEmbedding(nn.Module):
             raise ValueError("RotaryEmbedding: base has to be above 1")
         self.dims, self.base, self.layout, self.scaling = dims, float(base), layout, dict(scaling) if scaling else None
         self.amplitude = 1.0
-        pair = torch.arange(dims // 2, dtype=torch.float64)
+        pair = torch.arange(dims // 2, dtype=torch.float64, device="cpu")      # (whatever device a model is built under)
         cfg = dict(self.scaling or {})
         kind, s = cfg.pop("kind", None), float(cfg.pop("factor", 1.0))
         if kind not in (None, "linear", "ntk", "yarn") or not 1.0 <= s < math.inf or (self.scaling and kind is None):
