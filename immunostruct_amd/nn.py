@@ -183,11 +183,20 @@ class RotaryEmbedding(nn.Module):
             raise ValueError(f"RotaryEmbedding: unknown layout {layout!r}")
         if not base > 1:
             raise ValueError("RotaryEmbedding: base has to be above 1")
+        if scaling is not None and not isinstance(scaling, dict):
+            raise ValueError(f"RotaryEmbedding: unknown scaling {scaling!r} (a dict of kind, factor, ...)")
         self.dims, self.base, self.layout, self.scaling = dims, float(base), layout, dict(scaling) if scaling else None
         self.amplitude = 1.0
         pair = torch.arange(dims // 2, dtype=torch.float64, device="cpu")      # (whatever device a model is built under)
         cfg = dict(self.scaling or {})
-        kind, s = cfg.pop("kind", None), float(cfg.pop("factor", 1.0))
+
+        def number(value):
+            try:
+                return float(value)
+            except (TypeError, ValueError):
+                raise ValueError(f"RotaryEmbedding: unknown scaling {scaling!r}") from None
+
+        kind, s = cfg.pop("kind", None), number(cfg.pop("factor", 1.0))
         if kind not in (None, "linear", "ntk", "yarn") or not 1.0 <= s < math.inf or (self.scaling and kind is None):
             raise ValueError(f"RotaryEmbedding: unknown scaling {scaling!r}")
         if kind == "ntk":
@@ -198,15 +207,16 @@ class RotaryEmbedding(nn.Module):
         if kind == "linear":
             freq = freq / s
         elif kind == "yarn":
-            length, fast, slow = float(cfg.pop("original_length")), float(cfg.pop("beta_fast", 32.0)), float(cfg.pop("beta_slow", 1.0))
+            length, fast, slow = (number(cfg.pop(name, other)) for name, other in (("original_length", None), ("beta_fast", 32.0), ("beta_slow", 1.0)))
             amplitude = cfg.pop("amplitude", None)
-            if length <= 0 or not fast > slow > 0:
+            amplitude = 0.1 * math.log(s) + 1.0 if amplitude is None else number(amplitude)
+            if not 0 < length < math.inf or not math.inf > fast > slow > 0 or not math.isfinite(amplitude):
                 raise ValueError(f"RotaryEmbedding: unknown scaling {scaling!r}")
             at = [dims * math.log(length / (2.0 * math.pi * turns)) / (2.0 * math.log(self.base)) for turns in (fast, slow)]
             low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
             ramp = ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
             freq = freq * (1.0 - ramp) + freq / s * ramp
-            self.amplitude = 0.1 * math.log(s) + 1.0 if amplitude is None else float(amplitude)
+            self.amplitude = amplitude
         if cfg:
             raise ValueError(f"RotaryEmbedding: unknown scaling options {sorted(cfg)}")
         self.freq = freq      # (a plain attribute: no part of state_dict, untouched by .half() / .to())

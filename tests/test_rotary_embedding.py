@@ -30,3 +30,12 @@ def test_turns_under_a_device_context(cuda_device):
         q = torch.randn(2, 5, 3, 16)
         got = rope(q)[0]
     assert torch.equal(got, HF.rotary(q, None, RotaryEmbedding(16).freq)[0])
+
+
+@pytest.mark.parametrize("scaling", ["linear", "yarn", ("kind", "linear"), 4.0, dict(kind="yarn", factor=4.0), dict(YARN, original_length=None),
+                                     dict(YARN, original_length=float("nan")), dict(YARN, original_length=float("inf")), dict(YARN, beta_fast=None),
+                                     dict(YARN, beta_fast=float("inf")), dict(kind="linear", factor=None), dict(kind="linear", factor="x"),
+                                     dict(YARN, amplitude=float("nan")), dict(YARN, amplitude="x")])
+def test_scalings_that_are_none(scaling):
+    with pytest.raises(ValueError, match="RotaryEmbedding: unknown scaling"):
+        RotaryEmbedding(16, scaling=scaling)
