@@ -10,7 +10,8 @@
 Both evaluate through one shared routine (:func:`attend`).
 
 * ``DifferentialAttention(feature_dim, n_head, ...)`` -- not in the reference: the difference of two softmax maps with learned weights, for
-  residue sequences and padded graphs (positions, lengths, causal order, grouped keys), every step a HIP kernel.
+  residue sequences and padded graphs (positions, lengths, causal order, grouped keys).  Positions, attention and norm are HIP kernels; the projections
+  are library products, mask and mean torch operations.
 """
 from __future__ import annotations
 
@@ -148,7 +149,8 @@ class DifferentialAttention(nn.Module):
     The norm's weight starts at ``1 - lambda_init``, which keeps the block's scale that of plain attention.
 
     ``forward(x, positions=None, lengths=None, causal=None) -> (B, n, feature_dim)``: see ``functional.differential_attention``; rows at or behind
-    ``lengths`` come back as zeros.  ``attend_cached`` is the same for new tokens over a cache of keys and values."""
+    ``lengths`` come back as zeros.  Samples padded at their end take ``causal="start"``; ``"end"`` counts the rows back from the length (row i sees keys
+    <= i + length - n), which is for queries that are a sample's last ones.  ``attend_cached`` is the same for new tokens over a cache of keys and values."""
 
     def __init__(self, feature_dim, n_head, kv_heads=None, input_dim=None, lambda_init=0.8, rotary=None):
         super().__init__()
@@ -200,8 +202,9 @@ class DifferentialAttention(nn.Module):
         return out
 
     def pooled_mean(self, x, positions=None, lengths=None):
-        """mean of the block's output over each sample's rows (an empty sample: zeros)"""
-        out = self.forward(x, positions, lengths)
+        """mean of the block's output over each sample's rows (an empty sample: zeros), its sum in fp32"""
+        out, n = self.forward(x, positions, lengths), x.shape[1]
         if lengths is None:
             return out.mean(dim=1)
-        return out.sum(dim=1) / lengths.clamp(min=1)[:, None].to(out.dtype)
+        rows = lengths.clamp(0, n).clamp(min=1)      # (as the attention takes them: above n means all)
+        return (out.sum(dim=1, dtype=torch.float32) / rows[:, None]).to(out.dtype)
