@@ -192,7 +192,8 @@ class DifferentialAttention(nn.Module):
         from .. import functional as HF
         b, n = q.shape[:2]
         y = HF.differential_attention(q, k, v, self.lam(), lengths, causal)
-        return self.w_concat(self.norm(y.view(b * n, -1)).view(b, n, -1))
+        width = 2 * self.n_head * self.head_dim      # (named: an empty batch has no size to find it from)
+        return self.w_concat(self.norm(y.view(b * n, width)).view(b, n, width))
 
     def forward(self, x, positions=None, lengths=None, causal=None):
         out = self.attend_cached(*self.project(x, positions), lengths, causal)
@@ -205,6 +206,6 @@ class DifferentialAttention(nn.Module):
         """mean of the block's output over each sample's rows (an empty sample: zeros), its sum in fp32"""
         out, n = self.forward(x, positions, lengths), x.shape[1]
         if lengths is None:
-            return out.mean(dim=1)
+            return out.mean(dim=1) if n > 0 else out.sum(dim=1)
         rows = lengths.clamp(0, n).clamp(min=1)      # (as the attention takes them: above n means all)
         return (out.sum(dim=1, dtype=torch.float32) / rows[:, None]).to(out.dtype)

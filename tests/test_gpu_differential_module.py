@@ -33,6 +33,19 @@ def test_pooled_mean_takes_lengths_as_the_attention_does(cuda_device):
     assert torch.equal(got, want) and not got[2].any() and got[0].any()
 
 
+@pytest.mark.parametrize("b,n", [(0, 5), (2, 0), (0, 0)])
+def test_empty_batches(cuda_device, b, n):
+    m = _module()
+    x, lens = torch.randn(b, n, 64, device="cuda", requires_grad=True), torch.zeros(b, dtype=torch.int32, device="cuda")
+    for args in ((), (None, lens), (None, lens, "end")):
+        out = m(x, *args)
+        assert out.shape == (b, n, 64)
+        out.sum().backward()
+    assert all(not p.grad.any() for p in m.parameters())
+    for pooled in (m.pooled_mean(x), m.pooled_mean(x, lengths=lens)):
+        assert pooled.shape == (b, 64) and not pooled.any()
+
+
 def test_end_is_the_order_of_a_samples_last_rows(cuda_device):
     """causal="end" over one's own rows: row i is the sample's position i + length - n, as with the operator; without lengths that is "start" """
     m, x = _module(), torch.randn(2, 9, 64, device="cuda")
