@@ -822,11 +822,11 @@ void launch_bwd(const Args& a, hipStream_t st) {
   constexpr int KEYS = 32 * key_groups<T, D>(), ROWS = 32 * dq_groups<T, D>();
   const long long sums = ((long long)heads * a.rows + 15) / 16;
   rowdot_kernel<T, VEC><<<(unsigned)(sums < 1 << 23 ? sums : 1 << 23), 256, 0, st>>>(a);      // (a launch of 2^24 workgroups runs short of them)
-  dkv_kernel<T, D, VEC><<<(a.nk + KEYS - 1) / KEYS * a.row_splits * heads, 4 * KEYS, 0, st>>>(a);
-  if (a.row_splits > 1)
+  if (a.dk != nullptr) dkv_kernel<T, D, VEC><<<(a.nk + KEYS - 1) / KEYS * a.row_splits * heads, 4 * KEYS, 0, st>>>(a);
+  if (a.dk != nullptr && a.row_splits > 1)
     key_join_kernel<T, VEC><<<(unsigned)(((long long)heads * a.nk * (2 * a.d + a.dv) / (VEC ? 4 : 1) + 255) / 256), 256, 0, st>>>(a);
-  dq_kernel<T, D, VEC><<<(a.rows + ROWS - 1) / ROWS * heads, 4 * ROWS, 0, st>>>(a);
-  dlam_kernel<T><<<a.heads, 1024, 0, st>>>(a);
+  if (a.dq != nullptr) dq_kernel<T, D, VEC><<<(a.rows + ROWS - 1) / ROWS * heads, 4 * ROWS, 0, st>>>(a);
+  if (a.dlam != nullptr) dlam_kernel<T><<<a.heads, 1024, 0, st>>>(a);
 }
 
 // the built width a call runs at: heads of at most D elements, values of at most 2 D (shorter rows are padded with zeros on chip);

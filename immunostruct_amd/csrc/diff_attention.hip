@@ -95,8 +95,8 @@ int is_diff_attention_bwd(const IsDiffAttention* args, void* stream) {
   a.o = nullptr;
   const int rc = prepare(a);
   if (rc != 0) return fail("is_diff_attention_bwd", rc);
-  if (a.maps == nullptr || a.lse == nullptr || a.d_o == nullptr || a.dots == nullptr || a.dq == nullptr || a.dk == nullptr ||
-      a.dv_out == nullptr || a.dlam == nullptr || (a.row_splits > 1 && a.work == nullptr))
+  if (a.maps == nullptr || a.lse == nullptr || a.d_o == nullptr || a.dots == nullptr || (a.dk == nullptr) != (a.dv_out == nullptr) ||
+      (a.dq == nullptr && (a.dk == nullptr || a.dlam != nullptr)) || (a.dk != nullptr && a.row_splits > 1 && a.work == nullptr))
     return fail("is_diff_attention_bwd", -22);
   return run(a, true, "is_diff_attention_bwd", stream);
 }

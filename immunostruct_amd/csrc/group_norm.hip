@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, 
       }
       t1 = sum(t1) * inv;
       t2 = sum(t2) * inv;
-      if (on && b < a.batch) {
+      if (on && b < a.batch && a.dx != nullptr) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) d.x[e] = live ? rstd * (d.x[e] - t1 - x.x[e] * t2) : 0.0f;
         d.store(reinterpret_cast<T*>(a.dx) + (long long)b * a.channels + c);
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const Args a, const int cpg, 
     }
   }
   if constexpr (BACK) {
-    if (a.weight != nullptr) {
+    if (a.dweight != nullptr) {
       const int c0 = blockIdx.y * width;
       float* record = a.work + (long long)blockIdx.x * 2 * a.channels;
 #pragma unroll
@@ -367,12 +367,12 @@ __global__ __launch_bounds__(256) void wide_kernel(const Args a) {
       for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) d[k].x[e] = live ? rstd * (d[k].x[e] - t[0] - x[k].x[e] * t[1]) : 0.0f;
-        if (on[k]) d[k].store(reinterpret_cast<T*>(a.dx) + (long long)b * a.channels + c + k * 256 * VE);
+        if (on[k] && a.dx != nullptr) d[k].store(reinterpret_cast<T*>(a.dx) + (long long)b * a.channels + c + k * 256 * VE);
       }
     }
   }
   if constexpr (BACK) {
-    if (a.weight != nullptr) {
+    if (a.dweight != nullptr) {
       float* record = a.work + (long long)blockIdx.x * 2 * a.channels + c;
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int s
     const float inv = 1.0f / ((float)(len > 0 ? len : 1) * (float)cg);
     t1 = group_sum(t1, p, cpg, all, out) * inv;
     t2 = group_sum(t2, p, cpg, all, out) * inv;
-    if (p.on) {
+    if (p.on && a.dx != nullptr) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int row = p.rl + k * p.lanes;
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(256) void slab_bwd_kernel(const Args a, const int s
     }
     if constexpr (!WALK) break;
   }
-  if (a.weight != nullptr) channel_record<VE>(tw, tb, p, lds, a.work + (long long)b0 * 2 * a.channels, a.channels, c0, slice);
+  if (a.dweight != nullptr) channel_record<VE>(tw, tb, p, lds, a.work + (long long)b0 * 2 * a.channels, a.channels, c0, slice);
 }
 
 // ---- long: row blocks ---------------------------------------------------------------------------------------------------------------------
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(256) void long_sum_kernel(const Args a, const Plan 
     }
     if constexpr (!WALK) break;
   }
-  if (a.weight != nullptr) channel_record<VE>(tw, tb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0, k.width);
+  if (a.dweight != nullptr) channel_record<VE>(tw, tb, p, lds, a.work + pairs + index * 2 * a.channels, a.channels, k.c0, k.width);
 }
 
 template <typename T, int VE>
@@ -982,6 +982,7 @@ void launch_long(const Args& a, const Plan& p, bool backward, hipStream_t st) {
   if (backward) {
     if (p.records < a.batch) long_sum_kernel<T, VE, true><<<(unsigned)((long long)p.records * p.slices), 256, 0, st>>>(a, p);
     else long_sum_kernel<T, VE, false><<<grid, 256, 0, st>>>(a, p);
+    if (a.dx == nullptr) return;
     long_join_kernel<true><<<join, 256, 0, st>>>(a, p);
     long_dx_kernel<T, VE><<<grid, 256, 0, st>>>(a, p);
   } else {
@@ -1013,7 +1014,7 @@ void launch(const Args& a, const Plan& p, bool backward, hipStream_t st) {
     if (p.ve == 1) launch_long<T, 1>(a, p, backward, st);
     else launch_long<T, N>(a, p, backward, st);
   }
-  if (backward && a.weight != nullptr) {
+  if (backward && a.dweight != nullptr) {
     const float* records = a.work + work_floats(a, p, false);
     param_grad_kernel<T><<<(2 * a.channels + 15) / 16, 1024, 0, st>>>(a, records, p.records);
   }
@@ -1026,11 +1027,12 @@ int run(const Args* args, bool backward, const char* entry, void* stream) {
       (a.weight_type != TYPE_F32 && a.weight_type != a.type) || !(a.eps >= 0.0f))
     return fail(entry, -22);
   if (!backward && a.y == nullptr) return fail(entry, -22);
-  if (backward && (a.dy == nullptr || a.dx == nullptr || (a.weight != nullptr && (a.dweight == nullptr || a.dbias == nullptr)))) return fail(entry, -22);
+  if (backward && (a.dy == nullptr || (a.dx == nullptr && a.dweight == nullptr) || (a.dweight == nullptr) != (a.dbias == nullptr) ||
+                   (a.dweight != nullptr && a.weight == nullptr))) return fail(entry, -22);
   const Plan p = plan(a);
   const uintptr_t own = backward ? reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx) : reinterpret_cast<uintptr_t>(a.y);
   if (p.ve > 1 && own % 16 != 0) return fail(entry, -22);
-  if (a.work == nullptr && work_floats(a, p, backward) > 0) return fail(entry, -22);
+  if (a.work == nullptr && work_floats(a, p, backward && a.dweight != nullptr) > 0) return fail(entry, -22);
   // workgroups of one launch (rows and wide: at most a few thousand; slab: several launches)
   if (p.form == LONG && (long long)a.batch * p.slices * p.blocks > 2LL * LAUNCH - 1) return fail(entry, -22);
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -117,13 +117,15 @@ struct Rotary : torch::autograd::Function<Rotary> {
     ctx->saved_data["amplitude"] = amplitude;
     ctx->set_materialize_grads(false);
     auto out = rotary_launch(q, k, positions, {freq.const_data_ptr<double>(), (int)freq.numel(), interleaved, amplitude}, false);
+    if (!wanted(q)) ctx->mark_non_differentiable({out.first});
+    if (k.defined() && !wanted(k)) ctx->mark_non_differentiable({out.second});
     return k.defined() ? variable_list{out.first, out.second} : variable_list{out.first};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once();
     const Tensor positions = ctx->get_saved_variables()[0], freq = ctx->saved_data["freq"].toTensor();
     const Turn t = {freq.const_data_ptr<double>(), (int)freq.numel(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["amplitude"].toDouble()};
-    Tensor gq = g[0], gk = g.size() > 1 ? g[1] : Tensor();
+    Tensor gq = ctx->needs_input_grad(0) ? g[0] : Tensor(), gk = g.size() > 1 && ctx->needs_input_grad(1) ? g[1] : Tensor();
     if (gq.defined()) std::tie(gq, gk) = rotary_launch(gq, gk, positions, t, true);
     else if (gk.defined()) gk = rotary_launch(gk, Tensor(), positions, t, true).first;
     return {gq, gk, Tensor(), Tensor(), Tensor(), Tensor()};
@@ -204,17 +206,25 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &q = s[0], &k = s[1], &v = s[2], &lam = s[3], &maps = s[5], &lse = s[6];
     const c10::DeviceGuard guard(q.device());
-    Tensor dq = like(q), dk = like(k), dv = like(v), dlam = like(lam);
-    if (maps.numel() == 0 || v.size(1) == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), dlam.zero_(), Tensor(), Tensor(), Tensor()};
+    // what is asked for, and what comes with it: dK and dV are one kernel's, dlam a sum of dQ's
+    const bool key = ctx->needs_input_grad(1) || ctx->needs_input_grad(2), second = ctx->needs_input_grad(3), query = ctx->needs_input_grad(0) || second;
+    auto if_asked = [](bool asked, const Tensor& t) { return asked ? like(t) : Tensor(); };
+    Tensor dq = if_asked(query, q), dk = if_asked(key, k), dv = if_asked(key, v), dlam = if_asked(second, lam);
+    if (maps.numel() == 0 || v.size(1) == 0) {
+      for (Tensor* t : {&dq, &dk, &dv, &dlam})
+        if (t->defined()) t->zero_();
+      return {dq, dk, dv, dlam, Tensor(), Tensor(), Tensor()};
+    }
+    if (!query && !key) return {dq, dk, dv, dlam, Tensor(), Tensor(), Tensor()};
     const Tensor g = aligned(grads[0]);
     IsDiffAttention a = diff_args(q, k, v, lam, s[4], ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble());
     const int rows = (int)lse.size(3);
-    a.row_splits = entry.row_splits(a.batch, a.kv_heads, rows, a.nk, a.causal);
+    a.row_splits = key ? entry.row_splits(a.batch, a.kv_heads, rows, a.nk, a.causal) : 1;
     const int64_t parts = entry.row_work_floats(a.batch, a.kv_heads, a.nk, a.d, a.dv, a.row_splits);
     Tensor work = floats(q, {parts + 3LL * a.batch * a.kv_heads * rows});      // the row splits' sums, then the rows' three dot products
     a.maps = maps.data_ptr<float>(), a.lse = lse.data_ptr<float>(), a.d_o = g.data_ptr();
     a.work = work.data_ptr<float>(), a.dots = a.work + parts;
-    a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv_out = dv.data_ptr(), a.dlam = dlam.data_ptr();
+    a.dq = ptr(dq), a.dk = ptr(dk), a.dv_out = ptr(dv), a.dlam = ptr(dlam);
     check(entry.diff_bwd(&a, stream_of(q)), "is_diff_attention_bwd");
     return {dq, dk, dv, dlam, Tensor(), Tensor(), Tensor()};
   }
@@ -270,17 +280,21 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &weight = s[1], &bias = s[2];
     const c10::DeviceGuard guard(x.device());
-    Tensor dx = like(x), dw = like(weight), db = like(bias), work;
+    const bool params = weight.defined() && (ctx->needs_input_grad(1) || ctx->needs_input_grad(2));      // (one kernel's sums)
+    Tensor dx, dw, db, work;
+    if (ctx->needs_input_grad(0)) dx = like(x);
+    if (params) dw = like(weight), db = like(bias);
     if (x.numel() == 0) {
-      if (dw.defined()) dw.zero_(), db.zero_();
+      if (params) dw.zero_(), db.zero_();
       return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
     }
+    if (!dx.defined() && !params) return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
     const Tensor g = aligned(grads[0]);
     IsGroupNorm a = norm_args(x, weight, bias, s[3], ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["activation"].toInt());
-    const int64_t n = entry.norm_floats(&a, 1);
+    const int64_t n = entry.norm_floats(&a, params);
     if (n > 0) work = floats(x, {n});
     a.stats = s[4].data_ptr<float>(), a.work = static_cast<float*>(ptr(work));
-    a.dy = g.data_ptr(), a.dx = dx.data_ptr(), a.dweight = ptr(dw), a.dbias = ptr(db);
+    a.dy = g.data_ptr(), a.dx = ptr(dx), a.dweight = ptr(dw), a.dbias = ptr(db);
     check(entry.norm_bwd(&a, stream_of(x)), "is_group_norm_bwd");
     return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
   }

@@ -449,8 +449,8 @@ int is_rotary(const void* q, long long q_b, long long q_n, long long q_h, void* 
  * is_diff_attention_fwd: reads q, k, v, lam, lengths; writes o (batch, nq, heads, dv); lse (batch, kv_heads, 2, nq heads / kv_heads; fp32) and
  *   maps (2, batch, nq, heads, dv; fp32: each map's own product) are what the backward needs, both or neither.  splits = is_diff_attention_splits(...) ranges of
  *   the keys per row (1: none); splits > 1 needs work[is_diff_attention_work_floats(...)] (rows = nq heads / kv_heads in both).
- * is_diff_attention_bwd: reads those two, the inputs and d_o (contiguous), not o; writes dq, dk, dv_out (contiguous), dlam (lam's type); dots: scratch of 1.5
- *   times lse's size; row_splits = is_diff_attention_row_splits(...) parts of the rows per key tile (1: none), more than one need
+ * is_diff_attention_bwd: reads those two, the inputs and d_o (contiguous), not o; writes dq, dk, dv_out (contiguous), dlam (lam's type); NULL: not wanted
+ *   (dk and dv_out together; dlam needs dq).  dots: scratch of 1.5 times lse's size; row_splits = is_diff_attention_row_splits(...) parts of the rows per key tile (1: none), more than one need
  *   work[is_diff_attention_row_work_floats(...)].  rows, group, vec and group_magic are set by the library.  Row strides below 2^31 / 64
  *   bytes.  No atomics: bitwise reproducible.                                                                                         */
 typedef struct {
@@ -477,7 +477,7 @@ int is_diff_attention_bwd(const IsDiffAttention* args, void* stream);
  * NULL: all n) and the channels / groups channels of a group; y = act((x - mean) rstd weight + bias); activation: 0 none, 1 SiLU, 2 GELU
  * (erf), 3 ReLU.  Rows behind the length give 0 and get no gradient.  weight, bias (channels) of weight_type, both or neither NULL.
  * is_group_norm_fwd writes y (contiguous) and stats (batch, groups, 2) = mean, rstd (fp32); is_group_norm_bwd reads x, stats, dy (contiguous)
- * and writes dx (contiguous), dweight, dbias (NULL with weight).  work[is_group_norm_work_floats(...)] floats of scratch for either.   */
+ * and writes dx (contiguous), dweight, dbias (NULL with weight); NULL: not wanted (dweight and dbias together).  work[is_group_norm_work_floats(...)] floats of scratch for either.   */
 typedef struct {
   const void *x, *weight, *bias;
   const int* lengths;
