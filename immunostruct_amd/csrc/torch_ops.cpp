@@ -11,6 +11,9 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <unordered_set>
+#include <vector>
+
 #include "../../include/immunostruct_hip.h"
 
 namespace {
@@ -68,15 +71,31 @@ void direct(std::initializer_list<const Tensor*> inputs) {
 }
 
 // A leaf whose gradient node an eager graph on another stream keeps alive cannot be differentiated in a capture: the engine would make that stream wait
-// for the captured one, which ends the capture and with it the process.  Refused while nothing is captured yet.
+// for the captured one, which ends the capture and with it the process.  Refused in the forward, for the inputs and for what the capture has computed
+// them from (nodes of the captured stream; what was computed before the capture is no part of it).
 void capturable(std::initializer_list<const Tensor*> inputs) {
-  for (const Tensor* t : inputs) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = node ? node->stream() : std::nullopt;
-    if (!stream.has_value() || stream->id() == c10::hip::getCurrentHIPStream(t->device().index()).id()) continue;
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+  const c10::DeviceGuard guard((*inputs.begin())->device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto captured = c10::hip::getCurrentHIPStream().id();
+  std::vector<torch::autograd::Node*> open;
+  std::unordered_set<torch::autograd::Node*> seen;
+  auto look = [&](torch::autograd::Node* node) {
+    if (node == nullptr || !seen.insert(node).second) return;
+    const auto stream = node->stream();
+    const bool elsewhere = stream.has_value() && stream->id() != captured;
+    TORCH_CHECK(!elsewhere || node->num_outputs() > 0,
                 "the sequence operators: an eager graph of a captured leaf is still alive; release its outputs before the capture");
+    if (!elsewhere) open.push_back(node);
+  };
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (t->is_leaf()) look(torch::autograd::impl::try_get_grad_accumulator(*t).get());
+    else look(t->grad_fn().get());
+  }
+  while (!open.empty()) {
+    torch::autograd::Node* node = open.back();
+    open.pop_back();
+    for (const auto& edge : node->next_edges()) look(edge.function.get());
   }
 }
 
