@@ -49,6 +49,8 @@ int type_of(const Tensor& t) {
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// (the stride of a dimension of one element means nothing and may be anything)
+int64_t step(const Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
 Tensor like(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); }
 Tensor floats(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.options().dtype(at::kFloat)); }
 // contiguous and 16-byte aligned: an incoming gradient may be any view
@@ -117,10 +119,10 @@ std::pair<Tensor, Tensor> rotary_launch(Tensor q, Tensor k, const Tensor& positi
   Tensor q_out = like(q), k_out = like(k);
   if (q.size(0) == 0 || q.size(1) == 0) return {q_out, k_out};
   const bool batched = positions.defined() && positions.dim() == 2;
-  check(entry.rotary(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), q_out.data_ptr(), (int)q.size(2), ptr(k), both ? k.stride(0) : 0,
-                     both ? k.stride(1) : 0, both ? k.stride(2) : 0, ptr(k_out), both ? (int)k.size(2) : 0, ptr(positions),
-                     positions.defined() && positions.scalar_type() == at::kLong, batched ? positions.stride(0) : 0,
-                     positions.defined() ? positions.stride(-1) : 0, t.freq, (int)q.size(0), (int)q.size(1), (int)q.size(3), 2 * t.pairs,
+  check(entry.rotary(q.data_ptr(), step(q, 0), step(q, 1), step(q, 2), q_out.data_ptr(), (int)q.size(2), ptr(k), both ? step(k, 0) : 0,
+                     both ? step(k, 1) : 0, both ? step(k, 2) : 0, ptr(k_out), both ? (int)k.size(2) : 0, ptr(positions),
+                     positions.defined() && positions.scalar_type() == at::kLong, batched ? step(positions, 0) : 0,
+                     positions.defined() ? step(positions, -1) : 0, t.freq, (int)q.size(0), (int)q.size(1), (int)q.size(3), 2 * t.pairs,
                      t.interleaved, inverse, (float)t.amplitude, type_of(q), stream_of(q)),
         "is_rotary");
   return {q_out, k_out};
@@ -167,16 +169,16 @@ std::pair<Tensor, OptTensor> rotary(const Tensor& q, const OptTensor& k_, const 
 // (B, n, heads, width) as the kernels read it: a copy where the innermost dimension is not laid out element by element, or the rows (query heads,
 // the two maps' keys) of one tile lie too far apart for their 32-bit offsets
 Tensor sequence_rows(const Tensor& t, int64_t heads) {
-  const bool fits = (t.stride(3) == 1 || t.size(3) == 1) && t.stride(1) < (1 << 23) && t.stride(2) * heads < (1 << 27);
+  const bool fits = (t.stride(3) == 1 || t.size(3) == 1) && step(t, 1) < (1 << 23) && step(t, 2) * heads < (1 << 27);
   return fits ? t : t.contiguous();
 }
 
 IsDiffAttention diff_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& lengths, int64_t causal, double scale) {
   IsDiffAttention a = {};
   a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.lam = lam.data_ptr(), a.lengths = static_cast<const int*>(ptr(lengths));
-  a.q_b = q.stride(0), a.q_n = q.stride(1), a.q_h = q.stride(2);
-  a.k_b = k.stride(0), a.k_n = k.stride(1), a.k_h = k.stride(2);
-  a.v_b = v.stride(0), a.v_n = v.stride(1), a.v_h = v.stride(2);
+  a.q_b = step(q, 0), a.q_n = step(q, 1), a.q_h = step(q, 2);
+  a.k_b = step(k, 0), a.k_n = step(k, 1), a.k_h = step(k, 2);
+  a.v_b = step(v, 0), a.v_n = step(v, 1), a.v_h = step(v, 2);
   a.batch = (int)q.size(0), a.nq = (int)q.size(1), a.nk = (int)v.size(1), a.heads = (int)q.size(2) / 2, a.kv_heads = (int)v.size(2);
   a.d = (int)q.size(3), a.dv = (int)v.size(3), a.causal = (int)causal, a.type = type_of(q), a.lam_type = type_of(lam);
   a.splits = a.row_splits = 1;
@@ -262,7 +264,7 @@ Tensor differential_attention(const Tensor& q, const Tensor& k, const Tensor& v,
 IsGroupNorm norm_args(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& lengths, int64_t groups, double eps, int64_t activation) {
   IsGroupNorm a = {};
   a.x = x.data_ptr(), a.weight = ptr(weight), a.bias = ptr(bias), a.lengths = static_cast<const int*>(ptr(lengths));
-  a.x_b = x.stride(0), a.x_n = x.stride(1);
+  a.x_b = step(x, 0), a.x_n = step(x, 1);
   a.batch = (int)x.size(0), a.n = (int)x.size(1), a.channels = (int)x.size(2), a.groups = (int)groups;
   a.activation = (int)activation, a.type = type_of(x), a.weight_type = weight.defined() ? type_of(weight) : 0;
   a.eps = (float)eps;
