@@ -132,8 +132,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
   // (tensors that may be missing are optional: an undefined one is no input to autograd's bookkeeping)
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_, const OptTensor& positions_, const Tensor& freq, bool interleaved, double amplitude) {
     const Tensor k = value(k_), positions = value(positions_);
-    ctx->save_for_backward({positions});
-    ctx->saved_data["freq"] = freq;
+    ctx->save_for_backward({positions, freq});      // (both: changed in place before the backward they are an error)
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["amplitude"] = amplitude;
     ctx->set_materialize_grads(false);
@@ -144,7 +143,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once();
-    const Tensor positions = ctx->get_saved_variables()[0], freq = ctx->saved_data["freq"].toTensor();
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &positions = saved[0], &freq = saved[1];
     const Turn t = {freq.const_data_ptr<double>(), (int)freq.numel(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["amplitude"].toDouble()};
     Tensor gq = ctx->needs_input_grad(0) ? g[0] : Tensor(), gk = g.size() > 1 && ctx->needs_input_grad(1) ? g[1] : Tensor();
     if (gq.defined()) std::tie(gq, gk) = rotary_launch(gq, gk, positions, t, true);

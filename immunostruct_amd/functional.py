@@ -1800,6 +1800,8 @@ def rotary(q, k, freq, positions=None, layout="half", amplitude=1.0):
     _check_sizes("rotary", *q.shape, 0 if k is None else k.shape[2])
     if freq.is_cuda or freq.dtype != torch.float64 or freq.dim() != 1 or not 1 <= freq.numel() <= 256 or 2 * freq.numel() > q.shape[3]:
         raise ValueError("rotary: freq has to be a float64 host tensor of 1 ... min(256, width / 2) frequencies")
+    if freq.requires_grad:
+        raise ValueError("rotary: there is no gradient of freq")
     if layout not in ("half", "interleaved"):
         raise ValueError(f"rotary: unknown layout {layout!r}")
     if positions is not None and (positions.dtype not in (torch.int32, torch.int64)

@@ -31,3 +31,11 @@ def test_group_norm(cuda_device, b, n, c):
     dy = torch.ones_like(x)
     run = lambda t: (lambda y: (y,) + torch.autograd.grad(y, t, dy))(HF.group_norm(t, 2, activation="silu"))
     assert all(torch.equal(p, r) for p, r in zip(run(x), run(_odd(x))))
+
+
+def test_frequencies_changed_before_the_backward(cuda_device):
+    freq, q = FREQ.clone(), torch.randn(1, 5, 2, 8, device="cuda", requires_grad=True)
+    out = HF.rotary(q, None, freq)[0]
+    freq.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()

@@ -39,3 +39,8 @@ def test_turns_under_a_device_context(cuda_device):
 def test_scalings_that_are_none(scaling):
     with pytest.raises(ValueError, match="RotaryEmbedding: unknown scaling"):
         RotaryEmbedding(16, scaling=scaling)
+
+
+def test_frequencies_have_no_gradient():
+    with pytest.raises(ValueError, match="no gradient"):
+        HF.rotary(torch.zeros(1, 2, 1, 8), None, torch.ones(4, dtype=torch.float64, requires_grad=True))
