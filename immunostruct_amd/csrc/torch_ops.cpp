@@ -53,12 +53,15 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 int64_t step(const Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
 Tensor like(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); }
 Tensor floats(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.options().dtype(at::kFloat)); }
+// the tensor as its memory says (torch keeps the sign of a conjugate's imaginary part as a mark)
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // contiguous and 16-byte aligned: an incoming gradient may be any view
 Tensor aligned(const Tensor& t) {
-  const Tensor c = t.contiguous();
+  const Tensor c = plain(t).contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
-Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+Tensor value(const OptTensor& t) { return t.has_value() ? plain(*t) : Tensor(); }
+OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the sequence operators are differentiable once: no create_graph=True"); }
 
@@ -111,6 +114,7 @@ struct Turn {
 std::pair<Tensor, Tensor> rotary_launch(Tensor q, Tensor k, const Tensor& positions, const Turn& t, bool inverse) {
   const c10::DeviceGuard guard(q.device());
   auto rows = [](Tensor& x) {
+    x = plain(x);
     if (x.defined() && x.stride(3) != 1 && x.size(3) != 1) x = x.contiguous();
   };
   rows(q);
@@ -153,12 +157,12 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
 };
 
-std::pair<Tensor, OptTensor> rotary(const Tensor& q, const OptTensor& k_, const Tensor& freq, const OptTensor& positions_, bool interleaved, double amplitude) {
-  const Tensor k = value(k_), positions = value(positions_);
+std::pair<Tensor, OptTensor> rotary(const Tensor& q_, const OptTensor& k_, const Tensor& freq, const OptTensor& positions_, bool interleaved, double amplitude) {
+  const Tensor q = plain(q_), k = value(k_), positions = value(positions_);
   direct({&q, &k});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k))) {
     capturable({&q, &k});
-    variable_list out = Rotary::apply(q, k_, positions_, freq, interleaved, amplitude);
+    variable_list out = Rotary::apply(q, optional(k), positions_, freq, interleaved, amplitude);
     return {out[0], k.defined() ? OptTensor(out[1]) : std::nullopt};
   }
   auto out = rotary_launch(q, k, positions, {freq.const_data_ptr<double>(), (int)freq.numel(), interleaved, amplitude}, false);
@@ -251,7 +255,8 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
   }
 };
 
-Tensor differential_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptTensor& lengths, int64_t causal, double scale) {
+Tensor differential_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& lam_, const OptTensor& lengths, int64_t causal, double scale) {
+  const Tensor q = plain(q_), k = plain(k_), v = plain(v_), lam = plain(lam_);
   direct({&q, &k, &v, &lam});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v) || wanted(lam))) {
     capturable({&q, &k, &v, &lam});
@@ -321,12 +326,12 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
   }
 };
 
-Tensor group_norm(const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, const OptTensor& lengths_, int64_t groups, double eps, int64_t activation) {
-  const Tensor weight = value(weight_), bias = value(bias_), lengths = value(lengths_);
+Tensor group_norm(const Tensor& x_, const OptTensor& weight_, const OptTensor& bias_, const OptTensor& lengths_, int64_t groups, double eps, int64_t activation) {
+  const Tensor x = plain(x_), weight = value(weight_), bias = value(bias_), lengths = value(lengths_);
   direct({&x, &weight, &bias});
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight) || wanted(bias))) {
     capturable({&x, &weight, &bias});
-    return GroupNorm::apply(x, weight_, bias_, lengths_, groups, eps, activation);
+    return GroupNorm::apply(x, optional(weight), optional(bias), lengths_, groups, eps, activation);
   }
   return norm_forward(unit_rows(x), weight, bias, lengths, groups, eps, activation).first;
 }

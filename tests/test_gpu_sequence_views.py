@@ -39,3 +39,22 @@ def test_frequencies_changed_before_the_backward(cuda_device):
     freq.mul_(2.0)
     with pytest.raises(RuntimeError, match="inplace"):
         out.sum().backward()
+
+
+def test_views_of_conjugates(cuda_device):
+    """a float view whose memory holds the opposite sign (torch keeps that as a mark on the tensor)"""
+    def conjugate(t):
+        return torch.complex(torch.zeros_like(t), -t.detach()).conj().imag.requires_grad_(True)
+
+    gen = torch.Generator().manual_seed(5)
+    make = lambda *s: torch.randn(*s, generator=gen).cuda().requires_grad_(True)
+    q, k, v, lam, x, w, o = make(1, 7, 2, 8), make(1, 9, 2, 8), make(1, 9, 1, 16), make(1), make(3, 5, 8), make(8), make(8)
+    assert conjugate(q).is_neg() and torch.equal(conjugate(q), q)
+    for call, inputs in ((HF.differential_attention, (q, k, v, lam)), (lambda a, b: torch.cat(HF.rotary(a, b, FREQ), dim=1), (q, make(1, 7, 2, 8))),
+                         (lambda a, b, c: HF.group_norm(a, 2, b, c, activation="silu"), (x, w, o))):
+        want, marked = call(*inputs), [conjugate(t) for t in inputs]
+        dy = torch.randn(want.shape, generator=gen).cuda()
+        with torch.no_grad():
+            assert torch.equal(call(*marked), want)
+        full = torch.autograd.grad(want, inputs, dy)
+        assert all(torch.equal(a, b) for a, b in zip(full, torch.autograd.grad(call(*marked), marked, conjugate(dy).detach())))
