@@ -31,9 +31,10 @@ namespace da {
 
 typedef IsDiffAttention Args;
 // The forward's weights are taken as 2^LIFT exp(score - running maximum), which may fall behind the true one by 2^SLACK.  fp16 has no steps below 2^-24:
-// there the largest weight is kept at 2^11 ... 2^15, so that what is lost lies below 2^-36 of it (unlifted, 4000 keys of weight 2^-26 beside one of weight 1
-// came out as nothing).  The other types have fp32's range; the larger slack makes rescaling rarer.
-template <typename T> constexpr float lift_of() { return __is_same(T, _Float16) ? 11.0f : 0.0f; }
+// there the largest weight is kept at 2^8 ... 2^12, so that what is lost lies below 2^-33 of it (unlifted, 4000 keys of weight 2^-26 beside one of weight 1
+// came out as nothing).  Four bits stay free above: the exponents are taken against a rounded maximum, which at scores of 10^7 and more is off by whole
+// units.  The other types have fp32's range; the larger slack makes rescaling rarer.
+template <typename T> constexpr float lift_of() { return __is_same(T, _Float16) ? 8.0f : 0.0f; }
 template <typename T> constexpr float slack_of() { return __is_same(T, _Float16) ? 4.0f : 8.0f; }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -514,7 +515,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
   zero_acc(dk);
   zero_acc(dv);
   ColumnScale<T> range;
-  float lift = 0.0f;      // fp16: the weights are taken 2^lift times as large, up to 2^15 (over thousands of keys they lie below its normal range)
+  float lift = 0.0f;      // fp16: the weights are taken 2^lift times as large, up to 2^12 (over thousands of keys they lie below its normal range; as in the forward)
   bool flip = false;
   const int seen_from = wg_key < len ? first_query(a, wg_key, len) * a.group / RT * RT : R;
   const int per = ((R - seen_from + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
@@ -547,7 +548,7 @@ __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_w
       flip = flip || lam < 0.0f;
       largest = fmaxf(largest, fabsf(lam));
     }
-    if constexpr (ColumnScale<T>::USED) lift = largest < 0x1p100f ? (float)(15 - __builtin_amdgcn_frexp_expf(largest)) : 0.0f;
+    if constexpr (ColumnScale<T>::USED) lift = largest < 0x1p100f ? (float)(12 - __builtin_amdgcn_frexp_expf(largest)) : 0.0f;
     static_assert(NTH >= 6 * RT, "a thread stages one statistic");
     const int sw = tid >> 5, sm = sw >= 3 ? 1 : 0, sk = sw - 3 * sm;      // which statistic of which map
     // a tile of 32 rows holds whole queries where the group divides 32: its rows' offsets then are the same in every tile

@@ -26,6 +26,9 @@ SHAPES = [(2, 150, 150, 2, 1, 32, 64, [150, 97], None), (1, 200, 200, 4, 2, 64, 
 CASES = [(t, s) for s in SHAPES for t in (torch.bfloat16, torch.float16)]
 
 
+each_16_bit = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+
+
 @pytest.mark.parametrize("dtype,shape", CASES, ids=lambda x: str(x)[6:] if isinstance(x, torch.dtype) else "-".join(str(i) for i in x[:7]) + f"-{x[8]}")
 def test_only_the_results_are_rounded(cuda_device, dtype, shape):
     b, nq, nk, h, hk, d, dv, lengths, causal = shape
@@ -81,8 +84,8 @@ def test_half_weights_of_the_second_map(cuda_device, lam):
 
 
 def test_half_weights_far_below_the_largest(cuda_device):
-    """one key of weight 1 with a value of 0 and 3999 of weight 2^-26 each with a value of 100: 0.006, not 0.  A weight may be off by 2^-36 (half a step
-    below fp16's normal range is 2^-25, the largest weight at 2^11 or above): 2^-10 of its own, so is their sum; the result's rounding adds 2^-11"""
+    """one key of weight 1 with a value of 0 and 3999 of weight 2^-26 each with a value of 100: 0.006, not 0.  The largest weight is kept
+    at 2^8, the others then are 2^-18, which fp16 holds; a few 2^-24 from the exponentials, 2^-11 from the result's rounding"""
     b, nq, nk, d = 64, 40, 4000, 16      # (enough rows that no keys are split: all weights are relative to the one)
     q = torch.zeros(b, nq, 4, d, dtype=torch.float16, device="cuda")
     k = torch.zeros(b, nk, 4, d, dtype=torch.float16, device="cuda")
@@ -94,4 +97,20 @@ def test_half_weights_far_below_the_largest(cuda_device):
     tail = 3999 * 2.0 ** -26
     for h in range(2):
         want = (1.0 - float(lam[h])) * 100.0 * tail / (1.0 + tail)
-        assert float((out[:, :, h] - want).abs().max()) <= 3.1 * 2.0 ** -11 * want
+        assert float((out[:, :, h] - want).abs().max()) <= 1.1 * 2.0 ** -11 * want
+
+
+@each_16_bit
+@pytest.mark.parametrize("size", [30.0, 300.0, 3000.0])
+def test_scores_of_any_size(cuda_device, dtype, size):
+    """scores up to 10^7 times the scale: every row's weight lies on one key, the result is that key's value and the gradients of the scores are none.
+    (The weight's own error is what a 32-bit score of that size allows in the backward, where it is exp2(score - lse): up to half a unit of their
+    rounding, 2^-24 of |lse|, so dV is only asked to be finite)"""
+    q = torch.randn(1, 40, 2, 64, generator=torch.Generator().manual_seed(6)).sign() * size
+    q, k = q.to(dtype).cuda(), q.to(dtype).cuda()
+    v, do = _randn(1, 40, 1, 128, dtype=dtype, seed=7), _randn(1, 40, 1, 128, dtype=dtype, seed=8)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, torch.tensor([0.5], device="cuda"))]
+    out = HF.differential_attention(*leaves)
+    assert torch.equal(out, (v[:, :, :1].float() * 0.5).to(dtype))
+    grads = torch.autograd.grad(out, leaves, do)
+    assert all(bool(torch.isfinite(g).all()) for g in grads)
