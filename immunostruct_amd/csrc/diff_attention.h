@@ -10,8 +10,9 @@
 //   waves     a wave works on 32 rows (or 32 keys) of ONE map; two neighbouring waves hold the two maps of the same rows and meet once at the end,
 //             lane to lane through LDS.  That halves a wave's registers (one accumulator set, one resident operand), so that two to four
 //             waves share a SIMD and hide each other's latencies.  The forward repeats nothing by it; the backward computes dP = dO V^T
-//             and the product with dO once per map (48 matrix instructions per 32 x 32 tile at d = 64 for 32) and is still far ahead:
-//             with both maps in one wave dK / dV took 849 us at (2, 4096, 16 / 4 heads, 64 / 128, bf16, causal), one wave per SIMD.
+//             and the product with dO once per map (dK / dV: 72 matrix instructions per 32 x 32 tile at d = 64 for 48) and is still far ahead:
+//             with both maps in one wave, one wave per SIMD, dK / dV took 849 us for 535 at (2, 4096, 16 / 4 heads, 64 / 128, bf16, causal), P and
+//             dS as one term.
 //   forward   one pass over the keys: S^T = K Q^T (a lane owns one query), running maximum and sum in 32 bits, O^T += V^T P^T.
 //             The maximum only moves when a score passes it by 2^8 (the weights stay <= 2^8, far inside every type), which makes
 //             the rescaling of the accumulators rare.
@@ -20,7 +21,7 @@
 //             dK / dV: a wave owns 32 keys and walks the rows; dQ: a wave owns 32 rows and walks the keys.
 // Scores, sums, lse, D, the maps' own products that D is formed from and all accumulators are 32-bit; only results are rounded to the inputs' type.  P
 // and dS are the left operands of 16-bit matrix instructions: they enter as two terms (mm_transposed), for any number of rows.  At (2, 4096, 16 / 4 heads,
-// 64 / 128, bf16, causal) that is 1430 us a training pass where one rounding took 1016, and results are as far from 64 bits as their own rounding is (0.0017
+// 64 / 128, bf16, causal) that is 1350 - 1430 us a training pass where one rounding took 1016, and results are as far from 64 bits as their own rounding is (0.0017
 // of the norm in bf16, 0.0002 in fp16; one rounding: 0.0027, 0.0003); single tokens are bound by the cache's bytes and pay nothing.
 #pragma once
 #include "../../include/immunostruct_hip.h"
@@ -49,12 +50,17 @@ __device__ __forceinline__ void two_buffers(int first, int last, F step) {
   }
 }
 
-// Row (key) groups of a workgroup: two waves each.  More groups share a staged tile, fewer let the workgroups of a CU drift apart, so that one
-// multiplies while another forms weights.  Measured at (2, 4096, 16 / 4 heads, 64 / 128, bf16, causal) for 2 / 4 groups: forward 284 / 317 us,
-// dK / dV 610 / 550, dQ 378 / 368; at (5, 517 x 1531, 6 / 2 heads, 128 / 256, fp16): forward 120 / 108, dQ 85 / 89, dK / dV two only (registers).
-template <typename T, int D> constexpr int fwd_groups() { return D * sizeof(T) <= 128 ? 2 : 4; }
-template <typename T, int D> constexpr int key_groups() { return D * sizeof(T) <= 128 ? 4 : 2; }
-template <typename T, int D> constexpr int dq_groups() { return D * sizeof(T) <= 128 ? 4 : 2; }
+// Row (key) groups of a workgroup: two waves each.  More groups share a staged tile, fewer let the workgroups of a CU drift apart, so that one multiplies
+// while another forms weights, and waste less on the last rows of short samples.  Measured (us) for 2 / 4 groups, where a build of 4 fits its registers and LDS:
+//   width 32   fp32 (128, 190, 1 head, ragged): forward 30.1 / 31.9, dK / dV 49.2 / 50.9, dQ 31.8 / 33.0; bf16 (4, 1024, 8 / 4 heads, causal): 31 / 41,
+//              46 / 56, 29 / 37; bf16 (128, 190, 2 heads, ragged): 19 / 23, 24 / 34, 14 / 16
+//   width 64   bf16 (2, 4096, 16 / 4 heads, causal): 422 / 429, 725 / 688, 431 / 442; fp32 (1, 2048, 2 heads, causal): 59 / 67, - , 282 / 488; fp32 (16, 300,
+//              4 / 2 heads, ragged): 77 / 74, - , 99 / 89
+//   width 128  fp16 (5, 517 over 1531, 6 / 2 heads): 103 / 117, - , 109 / 110
+// Two groups, then, but for the 16-bit dK / dV at width 64.
+template <typename T, int D> constexpr int fwd_groups() { return 2; }
+template <typename T, int D> constexpr int key_groups() { return sizeof(T) == 2 && D == 64 ? 4 : 2; }
+template <typename T, int D> constexpr int dq_groups() { return 2; }
 
 template <typename T>
 __device__ __forceinline__ float lam_at(const Args& a, int head) {
@@ -181,10 +187,10 @@ struct ColumnScale {
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
 // grid: (row tiles x splits x kv_heads x batch), GROUPS x 2 waves of 32 rows and one map.  splits > 1: every workgroup takes one range of the
 // keys and leaves unnormalised sums with their maxima in the workspace; join_kernel puts them together.
-// Bound by matrix instructions and the exponentials between them: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 283 us = 0.73 PFLOP/s executed
-// (the product with V once per map; a large library product reaches 1.18); (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 88 us; (128, 190, 1, 32 / 64, fp32)
-// 28 us, where fp32 matrix instructions share the vector pipe.  Single tokens are bound by the cache: (16, 1 x 16384 ragged, 16 / 4, 64 / 128, bf16)
-// 77 us = 4.7 TB/s.
+// Bound by matrix instructions and the exponentials between them: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 430 us = 0.80 PFLOP/s executed
+// (the product with V once per map and term; a large library product reaches 1.18); (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 103 us, where the two-wave cap
+// of 256 registers makes 128-wide heads spill 35 - 50 of them to scratch; (128, 190, 1, 32 / 64, fp32) 29 us, where fp32 matrix instructions
+// share the vector pipe.  Single tokens are bound by the cache: (16, 1 x 16384 ragged, 16 / 4, 64 / 128, bf16) 77 us = 4.7 TB/s.
 template <typename T, int D, int GROUPS, bool VEC>
 __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2))) void fwd_kernel(const Args a) {
   constexpr int DV = 2 * D, KT = 32, NT = DV / 32, NJ = D / (2 * Vec<T>::N), NTH = 128 * GROUPS, SZ = sizeof(T);
@@ -336,8 +342,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // The splits of one row put together by WAVES waves.  lane = split for the maxima and sums (at most 64 splits; every wave forms the weights), then
 // a wave takes every WAVES-th split and a lane two columns: the first sums are loaded before their weights are known.  Single tokens have
-// few rows and many splits: four waves a row (a workgroup), 4.8 us for 256 rows of 16 splits, 12.4 by one.  More rows: one, (1, 512 over 4096, 8 / 2
-// heads, 64) bf16 52 us with the forward, 59 by four.
+// few rows and many splits: four waves a row (a workgroup), 4.8 us for 256 rows of 16 splits, 12.4 by one.  More rows: one, 7 us less than by four at
+// (1, 512 over 4096, 8 / 2 heads, 64) bf16.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   constexpr int BATCH = 4;
@@ -419,7 +425,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
-// D_1 = dO . O_1 and D_2 = dO . O_2 of every row (16 lanes per row), of the maps' own unrounded products; bound by bytes
+// D_1 = dO . O_1 and D_2 = dO . O_2 of every row (16 lanes per row), of the maps' own unrounded products; bound by bytes: 25 us for 134 MB
+// of products and 34 of dO (6.7 TB/s, partly cached)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void rowdot_kernel(const Args a) {
   constexpr int N = Vec<T>::N;
@@ -488,8 +495,8 @@ __global__ __launch_bounds__(1024) void dlam_kernel(const Args a) {
 // the last by few, and one workgroup per key tile would leave half the chip idle half the time.
 // Both waves run the same code on (lse, D): map 1's weight is taken as +|lam| P_2 with |lam| folded into lse, and its results are negated when they
 // leave the wave.  Only where a lam of the group is negative do its rows' signs have to be put back (flip).
-// Bound by matrix instructions: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 535 us = 0.77 PFLOP/s executed (582 with lam applied to each weight);
-// (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 145 us, 120 workgroups; (128, 190, 1, 32 / 64, fp32) 49 us.
+// Bound by matrix instructions: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 700 us = 0.88 PFLOP/s executed (lam applied to each weight cost 47 more);
+// (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 174 us, 480 workgroups of 64 keys and half of the rows, of which 8 in 10 have keys; (128, 190, 1, 32 / 64, fp32) 49 us.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((128 * key_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) <= 128 ? 2 : 1))) void dkv_kernel(const Args a) {
   constexpr int GROUPS = key_groups<T, D>(), NTH = 128 * GROUPS, KEYS = 32 * GROUPS;
@@ -681,8 +688,8 @@ __global__ __launch_bounds__(256) void key_join_kernel(const Args a) {
 }
 
 // dQ of 32 rows per wave: grid (row tiles x kv_heads x batch), GROUPS x 2 waves; dO of the workgroup's rows stays in LDS (the registers hold
-// Q, the sums and two tiles of scores).  Bound by matrix instructions: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 385 us = 0.71 PFLOP/s executed;
-// (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 87 us; (128, 190, 1, 32 / 64, fp32) 33 us.
+// Q, the sums and two tiles of scores).  Bound by matrix instructions: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 433 us = 0.79 PFLOP/s executed;
+// (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 108 us; (128, 190, 1, 32 / 64, fp32) 32 us.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__((128 * dq_groups<T, D>())) __attribute__((amdgpu_waves_per_eu(2))) void dq_kernel(const Args a) {
   constexpr int GROUPS = dq_groups<T, D>(), NTH = 128 * GROUPS, ROWS = 32 * GROUPS;

@@ -46,10 +46,10 @@ int run(const da::Args& a, bool backward, const char* entry, void* stream) {
 extern "C" {
 
 // Splits of the keys, where the rows alone do not fill the chip.  Up to 32 rows (single tokens) a workgroup is one pair of waves and the call is
-// bound by the cache's bytes: 1024 workgroups, at least 128 keys each.  More rows: 256 workgroups in all, and only while a split has work enough to
-// pay for leaving its sums in memory: 512 keys in the 16-bit types, 128 in the 8 to 16 times slower 32-bit one.  Measured (us) for at
-// least 128 / 512 / 1024 keys: (1, 512 over 4096, 8 / 2 heads, 64) bf16 81 / 53 / 46, (2, 300 over 300, 8, 64) bf16 28 / 14 / 14, (1, 128 over 2048,
-// 4 / 1, 64) bf16 29 / 25 / 33, (1, 2048 over 2048, 2, 64) fp32 98 / 120 / 207; with 256 workgroups instead of 512 the last takes 76.
+// bound by the cache's bytes: 1024 workgroups, at least 128 keys each.  More rows: 256 times 128 rows in all (the kernels take them as two workgroups of 64),
+// and only while a split has work enough to pay for leaving its sums in memory: 512 keys in the 16-bit types, 128 in the 8 to 16 times slower 32-bit one.
+// Measured (us) for at least 128 / 512 / 1024 keys: (1, 512 over 4096, 8 / 2 heads, 64) bf16 61 / 61 / 55, (2, 300 over 300, 8, 64) bf16 30 / 16 / 16, (1, 128
+// over 2048, 4 / 1, 64) bf16 24 / 26 / 38, (1, 2048 over 2048, 2, 64) fp32 67 / 75 / 123; with twice the splits the last takes 94.
 int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk, int type) {
   if (batch < 1 || kv_heads < 1 || rows < 1 || nk < 1) return 1;
   const long long groups = (rows <= 32 ? 1LL : (rows + 127LL) / 128) * kv_heads * batch;
@@ -58,8 +58,9 @@ int is_diff_attention_splits(int batch, int kv_heads, int rows, int nk, int type
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
-// Row splits of the key gradients: workgroups of 128 keys are alone on their CU.  With a mask the first tiles have all the work, two parts of
-// each fill the gaps the last ones leave; few key tiles are split until 256 workgroups are there, at least 256 rows each, 16 parts at most.
+// Row splits of the key gradients, counted in tiles of 128 keys, which the kernels take as one workgroup (16-bit heads of 33 ... 64) or two (others).  With a
+// mask the first tiles have all the work, two parts of each fill the gaps the last ones leave; few key tiles are split until 256 are there, at least
+// 256 rows each, 16 parts at most.  For 128-wide heads that is twice the workgroups that would fill the chip, and a join on top: not measured without.
 int is_diff_attention_row_splits(int batch, int kv_heads, int rows, int nk, int causal) {
   if (batch < 1 || kv_heads < 1 || rows < 1 || nk < 1) return 1;
   const long long groups = (nk + 127LL) / 128 * kv_heads * batch, most = (rows + 255LL) / 256;
