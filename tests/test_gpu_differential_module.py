@@ -54,3 +54,30 @@ def test_end_is_the_order_of_a_samples_last_rows(cuda_device):
     q, k, v = m.project(x)
     there = (torch.arange(9, device="cuda") < lens[:, None])[:, :, None]
     assert torch.equal(m(x, lengths=lens, causal="end"), torch.where(there, m.attend_cached(q, k, v, lens, "end"), 0.0))
+
+
+@pytest.mark.parametrize("dtype,half", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("causal,ragged", [("start", False), (None, True)])
+def test_16_bit_training_pass(cuda_device, dtype, half, causal, ragged):
+    """values and gradients of the 16-bit block against the block in 64 bits with the same (rounded) parameters.  Between an input and a gradient lie
+    fourteen tensors of the type (projected, turned, attended, normalised, projected; the same back, and what the backward multiplies them with), each
+    off by at most half a step of every element and so of its norm, with random signs; the norm of the whole is asked to stay within their plain sum"""
+    from tests.test_gpu_sequence_ops import _plain_block
+    m = _module(dtype, input_dim=20)
+    x = torch.randn(3, 83, 20, generator=torch.Generator().manual_seed(4)).to(dtype).cuda().requires_grad_(True)
+    pos, lens = torch.arange(83, device="cuda"), torch.tensor([83, 40, 11], dtype=torch.int32, device="cuda") if ragged else None
+    want, xd, p = _plain_block(m, x, pos, lens, causal)
+    dy = torch.randn(want.shape, generator=torch.Generator().manual_seed(5)).to(dtype)
+    got = m(x, pos, lens, causal)
+    got.backward(dy.cuda())
+    want.backward(dy.double())
+
+    def close(a, b, what):
+        off = float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm())
+        assert off <= 14 * half, f"{what}: {off / half:.1f} half steps of the norm"
+
+    close(got, want, "out")
+    close(x.grad, xd.grad, "dx")
+    for name, par in m.named_parameters():
+        if not name.startswith("lambda") and name != "w_k.bias":      # (sums of many cancelling terms: their rounding is relative to the terms)
+            close(par.grad, p[name].grad, name)
