@@ -189,7 +189,7 @@ struct ColumnScale {
 // keys and leaves unnormalised sums with their maxima in the workspace; join_kernel puts them together.
 // Bound by matrix instructions and the exponentials between them: (2, 4096, 16 / 4 heads, 64 / 128, bf16, "start") 430 us = 0.80 PFLOP/s executed
 // (the product with V once per map and term; a large library product reaches 1.18); (5, 517 x 1531, 6 / 2, 128 / 256, fp16) 103 us, where the two-wave cap
-// of 256 registers makes 128-wide heads spill 35 - 50 of them to scratch; (128, 190, 1, 32 / 64, fp32) 29 us, where fp32 matrix instructions
+// of 256 registers makes 128-wide heads spill 28 - 40 of them to scratch; (128, 190, 1, 32 / 64, fp32) 29 us, where fp32 matrix instructions
 // share the vector pipe.  Single tokens are bound by the cache: (16, 1 x 16384 ragged, 16 / 4, 64 / 128, bf16) 77 us = 4.7 TB/s.
 template <typename T, int D, int GROUPS, bool VEC>
 __global__ __launch_bounds__(128 * GROUPS) __attribute__((amdgpu_waves_per_eu(2))) void fwd_kernel(const Args a) {

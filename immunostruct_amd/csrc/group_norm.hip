@@ -13,7 +13,7 @@
 //         ((8192, 1, 4096) bf16, one group: 43 us forward, 92 backward; as row blocks 174 and 379).
 //   slab  a workgroup holds all rows of one sample's slice of whole groups in registers (up to 16 chunks a thread): one read, exact two-step
 //         variance, one write.  Slices are as narrow as 64-byte row segments allow, so that small batches still fill the chip
-//         ((128, 190, 64) fp32, 8 groups: 6.5 us forward, 9.2 + 3.3 backward).
+//         ((128, 190, 64) fp32, 8 groups: 6.4 us forward, 10.0 + 3.8 backward).
 //   long  a sample does not fit: row blocks leave (mean, M2) / (sum t, sum t xhat) of every group, a small launch joins a sample's blocks (one
 //         wave per sample and group; done by every workgroup of the next pass it cost 50 us at (2, 65536, 512), 32 groups), a third
 //         writes.  Block sums are taken about each thread's own first value, so a large mean costs no precision
