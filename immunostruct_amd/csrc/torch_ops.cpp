@@ -11,6 +11,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <memory>
 #include <unordered_set>
 #include <vector>
 
@@ -82,6 +83,7 @@ void capturable(std::initializer_list<const Tensor*> inputs) {
   const c10::DeviceGuard guard((*inputs.begin())->device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto captured = c10::hip::getCurrentHIPStream().id();
+  std::vector<std::shared_ptr<torch::autograd::Node>> held;      // (a leaf's node is held by the graphs that use it alone)
   std::vector<torch::autograd::Node*> open;
   std::unordered_set<torch::autograd::Node*> seen;
   auto look = [&](torch::autograd::Node* node) {
@@ -94,8 +96,8 @@ void capturable(std::initializer_list<const Tensor*> inputs) {
   };
   for (const Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad()) continue;
-    if (t->is_leaf()) look(torch::autograd::impl::try_get_grad_accumulator(*t).get());
-    else look(t->grad_fn().get());
+    held.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    look(held.back().get());
   }
   while (!open.empty()) {
     torch::autograd::Node* node = open.back();

@@ -1824,6 +1824,7 @@ def differential_attention(q, k, v, lam, lengths=None, causal=None, scale=None):
     ``causal``: None; "start": query i is position i and sees keys <= i; "end": the queries are the sample's last nq positions, i.e. new
     tokens over a cache, and see keys <= i + length - nq.  ``scale``: a positive number, d ** -0.5 by default.
     Keys that no query sees may hold anything; a key that the order hides from some queries only has to hold numbers (its weight there is 0).
+    (An infinite value that a query sees gives it NaN.)
     A query that sees no key gives zeros and passes no gradient.  Returns (B, nq, heads, dv).  Deterministic; scores, softmax weights
     and statistics, score gradients and sums are 32-bit: nothing but the results is rounded to the inputs' type."""
     _sequence_type("differential_attention", q, k, v)
